@@ -28,9 +28,9 @@ extern "C" {
 #endif
 
 /* ABI version of this header: qbnn_version() of the loaded library must equal it (bumped whenever a prototype below changes;
- * 2 = round 5: qbnn_block_chain_i8_multi_launch takes a_hi and w_layout, qbnn_block_down_i8_multi_launch w_layout, qbnn_block_desc carries w_layout; round 4's `stream` argument
+ * 3: the 8-bit floating-point linear layers and routed experts; 2 = round 5: qbnn_block_chain_i8_multi_launch takes a_hi and w_layout, qbnn_block_down_i8_multi_launch w_layout, qbnn_block_desc carries w_layout; round 4's `stream` argument
  * of the _multi_prepare calls). */
-#define QBNN_ABI_VERSION 2
+#define QBNN_ABI_VERSION 3
 
 #define QBNN_OK 0
 #define QBNN_E_INVALID (-1)     /* bad argument / unsupported shape   */
@@ -629,6 +629,73 @@ int qbnn_classification_metrics(const float* probs, const int64_t* target, int32
  * per block of 256 rows, partials[blk][0..2] = sum of the Gaussian NLL 0.5 log(2 pi var + 1e-8) + (t - mean)^2 / (2 var + 1e-8),
  * of the squared error and of the absolute error.  var == NULL: variance 1 (a mean-only model, :154). */
 int qbnn_regression_metrics(const float* mean, const float* var, const float* target, int32_t B, float* partials, void* stream);
+
+/* ---- 8-bit floating-point linear layers with one scale per block of 128, and routed layers of experts ---------------------------- */
+
+/* Floating types at the interface. */
+#define QBNN_F32 0
+#define QBNN_BF16 1
+#define QBNN_F16 2
+#define QBNN_F8 3               /* e4m3 values + block exponents */
+
+/* Operand format: e4m3 (OCP, no infinities) values [rows][Kp], Kp = K up to a multiple of 128 with zeros behind the last column, and one
+ * biased exponent byte per block (127 = 2^0) [row blocks][Sp], Sp = ceil(K / 128) up to a multiple of 4.  A block is 128 columns of one row
+ * (activations) or of 128 rows (weights); its scale is the smallest power of two >= 2^-126 that brings its largest finite magnitude to 448 or
+ * below (2^0 for a block of zeros).  Values are rounded to nearest, ties to even; one that is not finite becomes NaN. */
+
+/* x [batch][R][K] (strides in elements, columns contiguous, any alignment) -> q [batch][R][Kp], exponents [batch][R or ceil(R / 128)][Sp].
+ * block_rows: 1 or 128. */
+int qbnn_quantize_f8(const void* x, int32_t x_type, int64_t x_batch_stride, int64_t x_row_stride, int64_t batch, int32_t R, int32_t K,
+                     int32_t block_rows, uint8_t* q, uint8_t* exponents, void* stream);
+
+/* y[s][m][n] = act( sum_k x[s][m][k] w[s][n][k] + bias[s][n] ).  exact (fp32 and e4m3 results): products and sums in fp32, at half the
+ * matrix rate; without it the e4m3 matrix instruction, which cuts the products of 8 neighbouring columns off 2^-13 below the largest of them
+ * before it adds them, and sums in fp32 from there (1.3e-5 of the result's norm on normal data).  x: block_rows 1, w: block_rows 128.  Strides
+ * per sample in bytes for the operands (0 = shared by the samples), in elements for the bias; y [n_samples][M][N] dense, or for QBNN_F8 in
+ * the operand format (y_exp, block_rows 1).  Replaces the fp32 / int8 product of a stochastic Linear (bbb/linear.py:42-50). */
+typedef struct qbnn_f8_linear {
+  const uint8_t* x; const uint8_t* x_exp; int64_t x_ss, x_exp_ss;
+  const uint8_t* w; const uint8_t* w_exp; int64_t w_ss, w_exp_ss;
+  const float* bias; int64_t bias_ss;
+  void* y; uint8_t* y_exp;
+  int32_t M, N, K, n_samples, relu, y_type, exact;
+} qbnn_f8_linear;
+
+int qbnn_linear_f8_mc(const qbnn_f8_linear* host_desc, void* stream);
+
+/* The same over ragged groups of rows: rows offsets[g] .. offsets[g + 1] - 1 (device, ascending, offsets[groups] <= M) take weight set and bias
+ * g % w_groups (strides w_ss, w_exp_ss, bias_ss).  x_rows != NULL: row i reads x row (x_rows[i] / topk) % x_row_count.  y_rows != NULL: row i's
+ * result goes to y row y_rows[i], times y_weights[y_rows[i]] (0 where that weight is 0).  Rows behind the last group are neither read nor written. */
+typedef struct qbnn_f8_routed {
+  const int32_t* offsets; int32_t groups, w_groups;
+  const int32_t* x_rows; int32_t topk, x_row_count;
+  const int32_t* y_rows; const float* y_weights;
+} qbnn_f8_routed;
+
+int qbnn_linear_f8_routed(const qbnn_f8_linear* host_desc, const qbnn_f8_routed* host_routed, void* stream);
+
+#define QBNN_ROUTE_MAX_EXPERTS 1024
+#define QBNN_ROUTE_MAX_CHOICES 32
+
+/* Router: logits [S][T][E] (strides in elements, experts contiguous) -> weights / experts [S][T][top_k] (descending keys), offsets [S E + 1] and rows
+ * [S T top_k]: the flat indices of the choices sorted by (sample, expert), stable.
+ *   score s = softmax or sigmoid of the logits; key = s + bias[e] (compared as 64-bit values, ties to the lowest index); with groups > 1 only the
+ *   top_groups groups of E / groups neighbours with the largest sum of their two largest keys take part; weight = s, divided by the sum of the chosen with
+ *   `renormalize` (0 if that is 0), times scale.  A logit of -inf or of the type's lowest value is masked: behind all others, weight 0.  A NaN in a
+ *   row makes its weights NaN; its experts are valid indices all the same.  workspace: qbnn_route_workspace_ints(S, T, E) ints. */
+typedef struct qbnn_route {
+  const void* logits; int64_t logits_ss, logits_rs;
+  const float* bias;
+  float* weights; int32_t* experts; int32_t* offsets; int32_t* rows; int32_t* workspace;
+  int32_t S, T, E, top_k, groups, top_groups, sigmoid, renormalize, type;
+  float scale;
+} qbnn_route;
+
+int64_t qbnn_route_workspace_ints(int32_t S, int32_t T, int32_t E);
+int qbnn_route_experts(const qbnn_route* host_desc, void* stream);
+
+/* y[t][n] = sum_j o[t * top_k + j][n], in the order of j, rounded once to y_type. */
+int qbnn_combine_routed(const float* o, int32_t rows, int32_t top_k, int32_t N, void* y, int32_t y_type, void* stream);
 
 const char* qbnn_last_error(void);
 int qbnn_version(void);

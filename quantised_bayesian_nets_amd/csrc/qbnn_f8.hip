@@ -1,0 +1,401 @@
+// libqbnn_hip.so: 8-bit floating-point linear layers with one scale for each block of 128 (format: qbnn_f8.h).
+//   quantiser   float rows / weights -> e4m3 + block exponents
+//   product     y[s][b][n] = act( sum_k x[s][b][k] w[s][n][k] + bias[n] ) for S Monte-Carlo samples in one launch, or over ragged
+//               groups of rows, one weight set each (the experts of a routed layer)
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "../../include/qbnn.h"
+#include "qbnn_common.h"
+#include "qbnn_f8.h"
+
+using namespace qbnn;
+
+namespace {
+
+static inline int f8_fail(const char* fmt, long a = 0, long b = 0) {
+  char buf[512];
+  snprintf(buf, sizeof(buf), fmt, a, b);
+  return qbnn_fail_msg(QBNN_E_INVALID, buf);
+}
+
+// ================================================================================================================================
+// Quantiser.  ROWS = 1: a block is 128 columns of one row, 16 lanes x 8 columns; ROWS = 128: a block is 128 x 128, a workgroup each,
+// held in registers between the maximum and the conversion, so that the input is read once.
+// ================================================================================================================================
+struct QuantF8Args {
+  const void* x; int64_t x_bs, x_rs;       // batch / row stride in elements; columns are contiguous
+  uint8_t* q; uint8_t* e;                  // [batch][R][Kp], [batch][Rb][Sp]
+  int R, K, Kb, Sp; int64_t blocks;        // blocks = batch * Rb * Kb
+};
+
+// 8 columns from `col` of a row of K (zeros behind the last); rows may start at any element's address
+template <int T> __device__ __forceinline__ void f8_load8(const f8_type<T>* row, int col, int K, float (&v)[8]) {
+  if (col + 8 <= K) {
+    f8_type<T> t[8];
+    __builtin_memcpy(t, row + col, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = f8_load<T>(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < K ? f8_load<T>(row[col + i]) : 0.f;
+  }
+}
+__device__ __forceinline__ uint32_t f8_max8(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, f8_magnitude(v[i]));
+  return m;
+}
+__device__ __forceinline__ uint32_t f8_max16(uint32_t m) {      // over the 16 lanes of a row's block
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+  return m;
+}
+__device__ __forceinline__ f8_v2i f8_scale8(const float (&v)[8], float down) {
+  return (f8_v2i){(int)f8_pack4(v[0] * down, v[1] * down, v[2] * down, v[3] * down), (int)f8_pack4(v[4] * down, v[5] * down, v[6] * down, v[7] * down)};
+}
+// the exponent of block kb; the lane that writes the last block's also clears the pad behind it
+__device__ __forceinline__ void f8_put_exponent(uint8_t* row, int kb, int Kb, int Sp, int e) {
+  row[kb] = (uint8_t)(e + 127);
+  if (kb == Kb - 1)
+    for (int i = Kb; i < Sp; ++i) row[i] = 0;
+}
+
+template <int T> __global__ __launch_bounds__(256) void quantize_f8_rows_kernel(const QuantF8Args a) {
+  const int64_t b = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (b >= a.blocks) return;                                        // (all 16 lanes of a block)
+  const int64_t r = b / a.Kb;
+  const int kb = (int)(b - r * a.Kb), j = threadIdx.x & 15;
+  const int64_t bt = r / a.R;
+  const f8_type<T>* row = (const f8_type<T>*)a.x + bt * a.x_bs + (r - bt * a.R) * a.x_rs;
+  float v[8];
+  f8_load8<T>(row, kb * 128 + j * 8, a.K, v);
+  const int e = f8_exponent(f8_max16(f8_max8(v)));
+  *(f8_v2i*)(a.q + r * ((int64_t)a.Kb * 128) + kb * 128 + j * 8) = f8_scale8(v, f8_pow2(-e));
+  if (j == 0) f8_put_exponent(a.e + r * a.Sp, kb, a.Kb, a.Sp, e);
+}
+
+template <int T> __global__ __launch_bounds__(256) void quantize_f8_blocks_kernel(const QuantF8Args a) {
+  __shared__ uint32_t red[4];
+  const int Rb = (a.R + 127) >> 7;
+  const int64_t b = blockIdx.x;
+  const int64_t br = b / a.Kb;
+  const int kb = (int)(b - br * a.Kb), j = threadIdx.x & 15, sub = threadIdx.x >> 4;
+  const int64_t bt = br / Rb;
+  const int r0 = (int)(br - bt * Rb) * 128;
+  const f8_type<T>* x = (const f8_type<T>*)a.x + bt * a.x_bs;
+  float v[8][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 16 * i + sub;
+    if (r < a.R) f8_load8<T>(x + r * a.x_rs, kb * 128 + j * 8, a.K, v[i]);
+    else
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[i][c] = 0.f;
+    m = max(m, f8_max8(v[i]));
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  const int e = f8_exponent(max(max(red[0], red[1]), max(red[2], red[3])));
+  const float down = f8_pow2(-e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 16 * i + sub;
+    if (r < a.R) *(f8_v2i*)(a.q + (bt * a.R + r) * ((int64_t)a.Kb * 128) + kb * 128 + j * 8) = f8_scale8(v[i], down);
+  }
+  if (threadIdx.x == 0) f8_put_exponent(a.e + br * a.Sp, kb, a.Kb, a.Sp, e);
+}
+
+template <int T> int launch_quantize(const QuantF8Args& a, int block_rows, hipStream_t st) {
+  const int64_t grid = block_rows == 1 ? (a.blocks + 15) / 16 : a.blocks;
+  if (grid > 0x7fffffff) return f8_fail("qbnn_quantize_f8: too many blocks (%ld)", (long)a.blocks);
+  if (block_rows == 1) hipLaunchKernelGGL((quantize_f8_rows_kernel<T>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((quantize_f8_blocks_kernel<T>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  return qbnn_check_launch_msg("qbnn_quantize_f8");
+}
+
+// ================================================================================================================================
+// Product
+// ================================================================================================================================
+struct F8Args {
+  const uint8_t* x; const uint8_t* xe; int64_t x_ss, xe_ss;
+  const uint8_t* w; const uint8_t* we; int64_t w_ss, we_ss;
+  const float* bias; int64_t bias_ss;
+  uint8_t* y; uint8_t* ye; int64_t y_ss;        // y_ss in elements
+  int M, N, Kb, Sp, relu, y_rs, ye_rs;          // y row pitch in elements, exponent pitch of an e4m3 result
+  // ragged groups: rows offsets[g] .. offsets[g + 1] of the routed order, with weight set g % w_groups
+  const int32_t* offsets; int groups, w_groups;
+  const int32_t* rows; int topk, x_rows;        // rows != null: x row of routed row i = (rows[i] / topk) % x_rows, else i
+  const int32_t* y_rows; const float* scale;    // y_rows != null: result row i goes to y_rows[i], times scale[y_rows[i]]
+};
+
+struct F8Tile { int m0, m1, set, sample; };     // rows m0 .. m1 - 1, weight set, sample (0 for groups: rows are global)
+
+// The tile of this workgroup.  Groups: tile `t` of the sequence of every group's ceil(rows / TM) tiles; each wave finds it with one pass
+// over the offsets, 64 groups at a time; false if there are fewer tiles (the grid is sized for the worst split of the rows).
+template <int TM, bool GROUPED> __device__ __forceinline__ bool f8_find_tile(const F8Args& a, int t, int z, F8Tile& o) {
+  if constexpr (!GROUPED) {
+    o.m0 = t * TM; o.m1 = min(a.M, o.m0 + TM); o.set = z; o.sample = z;
+    return true;
+  } else {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int g0 = 0; g0 < a.groups; g0 += 64) {
+      const int g = g0 + lane;
+      int b = 0, n = 0;
+      if (g < a.groups) { b = a.offsets[g]; n = a.offsets[g + 1] - b; }
+      const int tiles = (n + TM - 1) / TM;
+      int incl = tiles;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) { const int u = __shfl_up(incl, d); if (lane >= d) incl += u; }
+      const int total = __shfl(incl, 63);
+      if (t < before + total) {
+        const int mine = before + incl - tiles;
+        const unsigned long long hit = __ballot(t >= mine && t < mine + tiles);
+        const int src = __ffsll(hit) - 1;
+        const int k = t - __shfl(mine, src), bb = __shfl(b, src), nn = __shfl(n, src);
+        o.m0 = bb + k * TM; o.m1 = min(bb + nn, o.m0 + TM); o.set = (g0 + src) % a.w_groups; o.sample = 0;
+        return true;
+      }
+      before += total;
+    }
+    return false;
+  }
+}
+template <bool GROUPED> __device__ __forceinline__ int f8_x_row(const F8Args& a, int i) {
+  if constexpr (GROUPED) { if (a.rows) return (a.rows[i] / a.topk) % a.x_rows; }
+  return i;
+}
+
+// four consecutive results (weight rows n .. n + 3) of activation row i
+template <int OUT, bool GROUPED> __device__ __forceinline__ void f8_put4(const F8Args& a, const F8Tile& t, int i, int n, f8_v4f v) {
+  const float* bias = a.bias ? a.bias + (int64_t)t.set * a.bias_ss : nullptr;
+  int64_t row = i;
+  float s = 1.f;
+  bool weighed = false;
+  if constexpr (GROUPED) { if (a.y_rows) { row = a.y_rows[i]; s = a.scale[row]; weighed = true; } }
+  f8_type<OUT> o[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    float u = v[c];
+    if (bias && n + c < a.N) u += bias[n + c];
+    if (a.relu) u = u > 0.f ? u : (u != u ? u : 0.f);          // (a NaN stays one)
+    if (weighed) u = s == 0.f ? 0.f : u * s;                   // (an expert of weight 0 adds nothing, whatever it computed)
+    o[c] = f8_store<OUT>(u);
+  }
+  f8_type<OUT>* y = (f8_type<OUT>*)a.y + (int64_t)t.sample * a.y_ss + row * a.y_rs + n;
+  if (n + 4 <= a.N) __builtin_memcpy(y, o, sizeof(o));
+  else
+    for (int c = 0; c < 4; ++c) if (n + c < a.N) y[c] = o[c];
+}
+
+// Direct form: operands straight from memory into the matrix instruction's registers, the waves of a workgroup split the columns and
+// join their sums in LDS in a fixed order.  For few rows, where the weights are read once and nothing is used twice.
+template <int MT, int NT, int NW, int OUT, bool EXACT, bool GROUPED>
+__global__ __launch_bounds__(NW * 64) void linear_f8_direct_kernel(const F8Args a) {
+  __shared__ __attribute__((aligned(16))) f8_v4f red[NW > 1 ? NW : 1][MT * NT * 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, h = lane >> 4;
+  F8Tile t;
+  if (!f8_find_tile<16 * MT, GROUPED>(a, blockIdx.y, blockIdx.z, t)) return;
+  const int n0 = blockIdx.x * (16 * NT);
+  const int64_t pitch = (int64_t)a.Kb * 128;
+  const uint8_t* xp[MT]; const uint8_t* xep[MT];
+  const uint8_t* wp[NT]; const uint8_t* wep[NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int row = f8_x_row<GROUPED>(a, min(t.m0 + 16 * i + r16, t.m1 - 1));      // a row behind the last repeats it: its result is not stored
+    xp[i] = a.x + (int64_t)t.sample * a.x_ss + row * pitch + h * 16;
+    xep[i] = a.xe + (int64_t)t.sample * a.xe_ss + (int64_t)row * a.Sp;
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int row = min(n0 + 16 * j + r16, a.N - 1);
+    wp[j] = a.w + (int64_t)t.set * a.w_ss + row * pitch + h * 16;
+    wep[j] = a.we + (int64_t)t.set * a.we_ss + (int64_t)(row >> 7) * a.Sp;
+  }
+  f8_v4f acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = (f8_v4f){0.f, 0.f, 0.f, 0.f};
+  for (int kb = wave; kb < a.Kb; kb += NW) {
+    f8_v8i xf[MT], wf[NT];
+    int xs[MT], ws[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      wf[j] = f8_join(*(const f8_v4i*)(wp[j] + kb * 128), *(const f8_v4i*)(wp[j] + kb * 128 + 64));
+      ws[j] = wep[j][kb];
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      xf[i] = f8_join(*(const f8_v4i*)(xp[i] + kb * 128), *(const f8_v4i*)(xp[i] + kb * 128 + 64));
+      xs[i] = xep[i][kb];
+    }
+    if constexpr (EXACT) {
+      F8Wide xw[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xw[i] = f8_widen(xf[i]);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const F8Wide ww = f8_widen(wf[j]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][j] = f8_mfma_exact(ww, xw[i], acc[i][j], ws[j], xs[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f8_mfma(wf[j], xf[i], acc[i][j], ws[j], xs[i]);
+    }
+  }
+  if constexpr (OUT == QBNN_F8) {
+    static_assert(NT == 8, "a block of an e4m3 result is 128 columns of a row");
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) red[wave][(i * NT + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    // 16 threads per row: thread c sums and converts columns 8 c .. + 7 = parts 2 (c & 1), + 1 of weight tile c / 2
+    const float* bias = a.bias ? a.bias + (int64_t)t.set * a.bias_ss : nullptr;
+    for (int u = threadIdx.x; u < MT * 256; u += NW * 64) {
+      const int i = u >> 8, r = (u >> 4) & 15, c = u & 15, row = t.m0 + 16 * i + r;
+      float v[8];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int at = (i * NT + (c >> 1)) * 64 + (2 * (c & 1) + p) * 16 + r;
+        f8_v4f s = red[0][at];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) s += red[k][at];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = n0 + c * 8 + p * 4 + q;
+          float o = s[q];
+          if (bias && n < a.N) o += bias[n];
+          if (a.relu) o = o > 0.f ? o : (o != o ? o : 0.f);
+          v[p * 4 + q] = n < a.N ? o : 0.f;
+        }
+      }
+      const int e = f8_exponent(f8_max16(f8_max8(v)));
+      if (row < t.m1) {
+        *(f8_v2i*)(a.y + (int64_t)t.sample * a.y_ss + (int64_t)row * a.y_rs + n0 + c * 8) = f8_scale8(v, f8_pow2(-e));
+        if (c == 0) f8_put_exponent(a.ye + ((int64_t)t.sample * a.M + row) * a.ye_rs, blockIdx.x, gridDim.x, a.ye_rs, e);
+      }
+    }
+  } else {
+    if constexpr (NW > 1) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) red[wave][(i * NT + j) * 64 + lane] = acc[i][j];
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if ((i * NT + j) % NW != wave) continue;
+        f8_v4f s = acc[i][j];
+        if constexpr (NW > 1) {
+          s = red[0][(i * NT + j) * 64 + lane];
+#pragma unroll
+          for (int k = 1; k < NW; ++k) s += red[k][(i * NT + j) * 64 + lane];
+        }
+        const int row = t.m0 + 16 * i + r16, n = n0 + 16 * j + 4 * h;
+        if (row < t.m1 && n < a.N) f8_put4<OUT == QBNN_F8 ? QBNN_F32 : OUT, GROUPED>(a, t, row, n, s);
+      }
+  }
+}
+
+template <int MT, int NT, int NW, int OUT, bool EXACT, bool GROUPED> int launch_direct(const F8Args& a, int tiles, int z, hipStream_t st) {
+  if (tiles > 65535 || z > 65535) return f8_fail("qbnn_linear_f8: %ld row tiles x %ld samples do not fit a grid", tiles, z);
+  hipLaunchKernelGGL((linear_f8_direct_kernel<MT, NT, NW, OUT, EXACT, GROUPED>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)tiles, (unsigned)z),
+                     dim3(NW * 64), 0, st, a);
+  return qbnn_check_launch_msg("qbnn_linear_f8");
+}
+
+// rows: the rows of one sample, or all routed rows
+template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, int rows, int z, hipStream_t st) {
+  const int spare = GROUPED ? a.groups : 0;        // each group may end inside a tile
+  const int per = GROUPED ? (rows + a.groups - 1) / a.groups : rows;
+  if constexpr (OUT == QBNN_F8) {
+    if (per <= 16) return launch_direct<1, 8, 4, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
+    return launch_direct<2, 8, 4, OUT, EXACT, GROUPED>(a, (rows + 31) / 32 + spare, z, st);
+  } else {
+    if (per <= 16) return launch_direct<1, 1, 8, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
+    return launch_direct<4, 4, 4, OUT, EXACT, GROUPED>(a, (rows + 63) / 64 + spare, z, st);
+  }
+}
+template <bool GROUPED> int launch_linear_any(const F8Args& a, int rows, int z, int y_type, int exact, hipStream_t st) {
+  switch (y_type) {
+    case QBNN_F32: return exact ? launch_linear<QBNN_F32, true, GROUPED>(a, rows, z, st) : launch_linear<QBNN_F32, false, GROUPED>(a, rows, z, st);
+    case QBNN_BF16: return launch_linear<QBNN_BF16, false, GROUPED>(a, rows, z, st);
+    case QBNN_F16: return launch_linear<QBNN_F16, false, GROUPED>(a, rows, z, st);
+    default: return exact ? launch_linear<QBNN_F8, true, GROUPED>(a, rows, z, st) : launch_linear<QBNN_F8, false, GROUPED>(a, rows, z, st);
+  }
+}
+
+int fill_args(F8Args& a, const qbnn_f8_linear* d) {
+  if (!d || !d->x || !d->x_exp || !d->w || !d->w_exp || !d->y || d->N <= 0 || d->K <= 0 || d->M < 0 || d->n_samples < 0 || d->y_type < QBNN_F32 || d->y_type > QBNN_F8 ||
+      (d->y_type == QBNN_F8 && !d->y_exp) || d->x_ss < 0 || d->w_ss < 0 ||
+      (d->exact && d->y_type != QBNN_F32 && d->y_type != QBNN_F8))
+    return f8_fail("qbnn_linear_f8: bad argument");
+  const uintptr_t low = (uintptr_t)d->x | (uintptr_t)d->w | (uintptr_t)d->x_ss | (uintptr_t)d->w_ss | (d->y_type == QBNN_F8 ? (uintptr_t)d->y : 0);
+  const uintptr_t low4 = (uintptr_t)d->x_exp | (uintptr_t)d->w_exp | (uintptr_t)d->x_exp_ss | (uintptr_t)d->w_exp_ss;
+  if ((low & 15) || (low4 & 3)) return f8_fail("qbnn_linear_f8: e4m3 operands start at multiples of 16 bytes, exponents of 4");
+  a = F8Args{};
+  a.Kb = (int)(((int64_t)d->K + 127) / 128);
+  a.Sp = (a.Kb + 3) / 4 * 4;
+  a.x = d->x; a.xe = d->x_exp; a.x_ss = d->x_ss; a.xe_ss = d->x_exp_ss;
+  a.w = d->w; a.we = d->w_exp; a.w_ss = d->w_ss; a.we_ss = d->w_exp_ss;
+  a.bias = d->bias; a.bias_ss = d->bias_ss;
+  a.y = (uint8_t*)d->y; a.ye = d->y_exp;
+  a.M = d->M; a.N = d->N; a.relu = d->relu;
+  const int Nb = (int)(((int64_t)d->N + 127) / 128);
+  a.y_rs = d->y_type == QBNN_F8 ? Nb * 128 : d->N;
+  a.ye_rs = (Nb + 3) / 4 * 4;
+  a.y_ss = (int64_t)d->M * a.y_rs;
+  return QBNN_OK;
+}
+
+}  // namespace
+
+QBNN_EXPORT int qbnn_quantize_f8(const void* x, int32_t x_type, int64_t x_batch_stride, int64_t x_row_stride, int64_t batch, int32_t R, int32_t K,
+                                 int32_t block_rows, uint8_t* q, uint8_t* exponents, void* stream) {
+  if (x_type < QBNN_F32 || x_type > QBNN_F16 || batch < 0 || R < 0 || K <= 0 || (block_rows != 1 && block_rows != 128)) return f8_fail("qbnn_quantize_f8: bad argument");
+  if (batch == 0 || R == 0) return QBNN_OK;
+  if (!x || !q || !exponents || ((uintptr_t)q & 15) || K > 0x7fffff00) return f8_fail("qbnn_quantize_f8: bad argument (q starts at a multiple of 16 bytes)");
+  QuantF8Args a;
+  a.x = x; a.x_bs = x_batch_stride; a.x_rs = x_row_stride; a.q = q; a.e = exponents;
+  a.R = R; a.K = K; a.Kb = (K + 127) / 128; a.Sp = (a.Kb + 3) / 4 * 4;
+  a.blocks = batch * (block_rows == 1 ? R : (R + 127) / 128) * a.Kb;
+  switch (x_type) {
+    case QBNN_F32: return launch_quantize<QBNN_F32>(a, block_rows, (hipStream_t)stream);
+    case QBNN_BF16: return launch_quantize<QBNN_BF16>(a, block_rows, (hipStream_t)stream);
+    default: return launch_quantize<QBNN_F16>(a, block_rows, (hipStream_t)stream);
+  }
+}
+
+QBNN_EXPORT int qbnn_linear_f8_mc(const qbnn_f8_linear* host_desc, void* stream) {
+  F8Args a;
+  if (int rc = fill_args(a, host_desc)) return rc;
+  if (a.M == 0 || host_desc->n_samples == 0) return QBNN_OK;
+  return launch_linear_any<false>(a, a.M, host_desc->n_samples, host_desc->y_type, host_desc->exact, (hipStream_t)stream);
+}
+
+QBNN_EXPORT int qbnn_linear_f8_routed(const qbnn_f8_linear* host_desc, const qbnn_f8_routed* r, void* stream) {
+  F8Args a;
+  if (int rc = fill_args(a, host_desc)) return rc;
+  if (!r || !r->offsets || r->groups <= 0 || r->w_groups <= 0 || (r->x_rows && (r->topk <= 0 || r->x_row_count <= 0)) || (r->y_rows && !r->y_weights) ||
+      (r->y_rows && host_desc->y_type == QBNN_F8))
+    return f8_fail("qbnn_linear_f8_routed: bad argument");
+  if (a.M == 0) return QBNN_OK;
+  a.offsets = r->offsets; a.groups = r->groups; a.w_groups = r->w_groups;
+  a.rows = r->x_rows; a.topk = r->topk; a.x_rows = r->x_row_count;
+  a.y_rows = r->y_rows; a.scale = r->y_weights;
+  return launch_linear_any<true>(a, a.M, 1, host_desc->y_type, host_desc->exact, (hipStream_t)stream);
+}

@@ -34,25 +34,31 @@ class Linear(nn.Module):
         sigma, mu, sp = F.softplus(self.std), self.weight, self.std_prior
         return 0.5 * (2 * torch.log(sp / sigma) - 1 + (sigma / sp).pow(2) + ((0 - mu) / sp).pow(2)).sum()
 
+    def sampled(self, device, eps=None):
+        """W_s = mu + eps_s * sigma of the active mc_context: fp32 [S, out_features * in_features]."""
+        S = _MC.samples
+        if self._sigma is None or self._sigma.device != device:
+            self._sigma = F.softplus(self.std.detach().cpu().float()).to(device).contiguous()   # one-time, same op as the reference
+            self._mu_dev = self.weight.detach().to(device).contiguous()                          # device copies made once (they were
+            self._bias_dev = None if self.bias is None else self.bias.detach().to(device).contiguous()   # re-uploaded on every call)
+        n = self._mu_dev.numel()
+        w = _take_presampled(self, device) if eps is None else None
+        if w is None:
+            w = torch.empty((S, n), dtype=torch.float32, device=device)
+            if eps is not None:
+                eps = eps.to(device=device, dtype=torch.float32).contiguous()
+            with timed("sample_weights_f32"):
+                _lib.check(_lib.lib().qbnn_sample_weights_f32(_lib.ptr(self._mu_dev), _lib.ptr(self._sigma), n, _MC.seed, self.layer_id,
+                                                              _MC.sample_begin, S, _lib.ptr(eps), _lib.ptr(w), _lib.current_stream()))
+        return w
+
     def forward(self, x, act=0, eps=None):
         """x fp32 [S or 1, B, in_features] -> [S, B, out_features]."""
         if x.device.type != "cuda":
             raise RuntimeError("qbnn layers run on an MI355X only (no CPU fallback)")
         S = _MC.samples
-        if self._sigma is None or self._sigma.device != x.device:
-            self._sigma = F.softplus(self.std.detach().cpu().float()).to(x.device).contiguous()   # one-time, same op as the reference
-            self._mu_dev = self.weight.detach().to(x.device).contiguous()                        # device copies made once (they were
-            self._bias_dev = None if self.bias is None else self.bias.detach().to(x.device).contiguous()   # re-uploaded on every call)
-        mu = self._mu_dev
-        n = mu.numel()
-        w = _take_presampled(self, x.device) if eps is None else None
-        if w is None:
-            w = torch.empty((S, n), dtype=torch.float32, device=x.device)
-            if eps is not None:
-                eps = eps.to(device=x.device, dtype=torch.float32).contiguous()
-            with timed("sample_weights_f32"):
-                _lib.check(_lib.lib().qbnn_sample_weights_f32(_lib.ptr(mu), _lib.ptr(self._sigma), n, _MC.seed, self.layer_id,
-                                                              _MC.sample_begin, S, _lib.ptr(eps), _lib.ptr(w), _lib.current_stream()))
+        w = self.sampled(x.device, eps)
+        n = w.shape[1]
         B = x.shape[1]
         y = torch.empty((S, B, self.out_features), dtype=torch.float32, device=x.device)
         xs = 0 if x.shape[0] == 1 else x[0].numel()

@@ -1,0 +1,382 @@
+"""The 8-bit float linear layers, the router and the routed experts on the GPU against plain 64-bit forms (f8_oracle.py).  The quantiser and the router's choices are
+held to the bit; sums to the bound that counts their roundings."""
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+import f8_oracle as orc
+
+pytestmark = pytest.mark.gpu
+q = pytest.importorskip("quantised_bayesian_nets_amd")
+DEV = "cuda"
+NAME = {torch.float32: "float32", torch.bfloat16: "bfloat16", torch.float16: "float16"}
+FLOATS = list(NAME)
+
+
+def rnd(seed, *shape, by=1.0, dtype=torch.float32):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * by).to(dtype)
+
+
+def f64(t):
+    return t.detach().to(torch.float64).cpu().numpy()
+
+
+def held(t):
+    """The values an F8Tensor stands for, from its bytes."""
+    d = t.data.cpu().to(torch.float64).numpy()[..., :t.columns]
+    e = t.exponent.cpu().numpy().astype(np.int64) - 127
+    lead = d.shape[:-2]
+    out = np.stack([m * orc.expand(x, t.block_rows, *m.shape) for m, x in zip(d.reshape(-1, *d.shape[-2:]), e.reshape(-1, *e.shape[-2:]))]) if d.size else d
+    return out.reshape(*lead, *d.shape[-2:])
+
+
+def check(y, want, bound):
+    y = f64(y)
+    assert np.array_equal(np.isnan(y), np.isnan(want))
+    ok = np.isnan(want) | (np.abs(y - want) <= bound)
+    assert ok.all(), (np.abs(y - want) / bound)[~ok].max()
+
+
+# ---------------------------------------------------------------------------------------------------------------- quantiser
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 127), (2, 5, 128), (130, 129), (2, 200, 513), (1, 640), (3, 128, 256)])
+def test_quantiser_is_exact(shape, dtype, rows):
+    x = rnd(1, *shape, by=3.0) * torch.exp2(rnd(2, *shape[:-1], 1, by=12.0))
+    x = x.clamp(-6e4, 6e4).to(dtype)
+    t = q.quantize_fp8(x.to(DEV), rows)
+    v = f64(x)
+    want = np.stack([orc.quantised(m, rows) for m in v.reshape(-1, *v.shape[-2:])]).reshape(v.shape)
+    assert np.array_equal(held(t), want)
+    assert np.array_equal(f64(t.dequantize(torch.float64)), want)
+    assert not t.data.cpu().view(torch.uint8)[..., t.columns:].any()                 # the pad
+    kb = -(-shape[-1] // 128)
+    assert not t.exponent.cpu()[..., kb:].any()
+
+
+def test_quantiser_at_the_borders():
+    """Ties, the largest value, a magnitude just above it, subnormals, zeros, and fp32's smallest."""
+    rows = [[448.0, 440.0, 424.0, 8.5, 2.0 ** -10, 3 * 2.0 ** -10, -(2.0 ** -9)], [448.1, 449.0, 17.0, 19.0, 0.03125], [0.0, -0.0], [2.0 ** -149, 2.0 ** -140],
+            [3e38, 1.0, -3e38], [1.75 * 2.0 ** -118, 2.0 ** -126], [2.0 ** -127 * 1.5]]
+    x = torch.zeros(len(rows), 128)
+    for r, v in enumerate(rows):
+        x[r, :len(v)] = torch.tensor(v)
+    t = q.quantize_fp8(x.to(DEV))
+    assert np.array_equal(held(t), orc.quantised(f64(x), 1))
+    assert np.array_equal(t.exponent.cpu().numpy()[:, 0].astype(int) - 127, orc.block_exponents(f64(x), 1)[:, 0])
+
+
+@pytest.mark.parametrize("rows", [1, 128])
+def test_quantiser_values_that_are_not_finite(rows):
+    x = rnd(3, 4, 300)
+    x[1, 7], x[2, 130], x[3, 299] = float("inf"), float("nan"), float("-inf")
+    x[0, 0] = 1000.0
+    t = q.quantize_fp8(x.to(DEV), rows)
+    want = orc.quantised(f64(x), rows)
+    assert np.array_equal(held(t), want, equal_nan=True) and np.isnan(want).sum() == 3
+
+
+def test_quantiser_strides_and_alignment():
+    big = rnd(4, 3, 40, 777, dtype=torch.bfloat16).to(DEV)
+    for v in (big[1:, 3:20, 5:400], big[:, ::2, 1:130], big[0, 7:9, 333:334], big.transpose(1, 2)[:, :50], big[1].T[3:9]):
+        t = q.quantize_fp8(v)
+        w = f64(v)
+        assert np.array_equal(held(t), np.stack([orc.quantised(m, 1) for m in w.reshape(-1, *w.shape[-2:])]).reshape(w.shape))
+    assert q.quantize_fp8(big[:, :0]).shape == (3, 0, 777) and q.quantize_fp8(big[:0], 128).shape == (0, 40, 777)
+
+
+# ---------------------------------------------------------------------------------------------------------------- product
+def linear_case(seed, S, sx, sw, B, N, K, dtype, bias, relu, out=None):
+    x = rnd(seed, sx, B, K, dtype=dtype)
+    w = rnd(seed + 1, sw, N, K, by=K ** -0.5) * torch.exp2(rnd(seed + 2, 1, N, 1, by=2.0))
+    b = rnd(seed + 3, N) if bias == 1 else rnd(seed + 3, S, N) if bias == 2 else None
+    wq = q.quantize_fp8(w.to(DEV), 128)
+    y = q.linear_fp8(x.to(DEV), wq, None if b is None else b.to(DEV), relu=relu, out_dtype=out)
+    wv = held(wq)
+    out = out or dtype
+    want, bound = [], []
+    for s in range(S):
+        xv = orc.quantised(f64(x[s if sx > 1 else 0]), 1)
+        bv = None if b is None else f64(b[s] if bias == 2 else b)
+        want.append(orc.product(xv, wv[s if sw > 1 else 0], bv, relu))
+        bound.append(orc.product_bound(xv, wv[s if sw > 1 else 0], bv, exact=out == torch.float32))
+    want, bound = np.stack(want), np.stack(bound)
+    return y, want, bound, out
+
+
+SIZES = [(1, 1, 1), (1, 16, 128), (2, 130, 100), (5, 257, 1000), (16, 96, 384), (17, 128, 256), (33, 129, 127), (64, 64, 640), (65, 1, 513), (100, 500, 800), (128, 256, 512),
+         (129, 384, 1024), (255, 300, 129), (256, 256, 256), (300, 520, 2048), (513, 777, 1111)]
+
+
+@pytest.mark.parametrize("dtype,out", [(torch.bfloat16, None), (torch.float32, None), (torch.float16, None), (torch.bfloat16, torch.float32), (torch.float32, torch.float16)])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_linear(size, dtype, out):
+    y, want, bound, out = linear_case(7, 1, 1, 1, *size, dtype, 1, False, out)
+    assert y.dtype == out and tuple(y.shape) == want.shape
+    check(y, want, bound + orc.rounding(want, NAME[out]) + bound * orc.HALF_STEP[NAME[out]])
+
+
+@pytest.mark.parametrize("sx,sw,bias", [(3, 3, 2), (1, 3, 1), (3, 1, 2), (3, 3, 0), (1, 1, 0)])
+@pytest.mark.parametrize("size", [(1, 40, 200), (20, 150, 300), (200, 260, 384)], ids=str)
+def test_linear_samples(size, sx, sw, bias):
+    S = max(sx, sw)
+    y, want, bound, out = linear_case(11, S, sx, sw, *size, torch.float32, bias, True)
+    assert y.shape[0] == S
+    check(y, want, bound + orc.rounding(want, "float32"))
+
+
+@pytest.mark.parametrize("size", [(1, 1, 5), (3, 128, 128), (16, 300, 256), (40, 513, 200), (130, 256, 512), (300, 1000, 384)], ids=str)
+def test_linear_result_in_blocks(size):
+    """The e4m3 result lies within half a step of the 64-bit one, with a block scale that one within the product's bound of it has."""
+    B, N, K = size
+    x, w, b = rnd(1, 2, B, K, dtype=torch.bfloat16).to(DEV), q.quantize_fp8(rnd(2, 2, N, K).to(DEV), 128), rnd(3, N).to(DEV)
+    for relu in (False, True):
+        t = q.linear_fp8(x, w, b, relu=relu, out_dtype=torch.float8_e4m3fn)
+        xv, wv = f64(q.quantize_fp8(x).dequantize()), held(w)
+        for s in range(2):
+            y = orc.product(xv[s], wv[s], f64(b), relu)
+            off = orc.product_bound(xv[s], wv[s], f64(b), exact=False)
+            g = held(t)[s]
+            e = t.exponent.cpu().numpy()[s].astype(int)[:, :-(-N // 128)] - 127
+            lo, hi = orc.block_exponents(np.sign(y) * np.maximum(np.abs(y) - off, 0), 1), orc.block_exponents(y + np.sign(y) * off, 1)
+            assert ((e >= lo) & (e <= hi) | (e == orc.block_exponents(y, 1))).all()
+            step = np.maximum(np.abs(y) + off, np.repeat(np.ldexp(1.0, e - 6), 128, 1)[:, :N]) * 2.0 ** -4      # half a step, of a subnormal too
+            assert (np.abs(g - y) <= off + step * (1 + 2.0 ** -10)).all()
+        assert not t.data.cpu().view(torch.uint8)[..., N:].any()
+        assert not t.exponent.cpu()[..., -(-N // 128):].any()
+
+
+def test_linear_rows_stand_alone():
+    """A row does not depend on its neighbours: one with NaN and infinities leaves the others their bits, at every row count's kernel."""
+    w = q.quantize_fp8(rnd(2, 200, 300).to(DEV), 128)
+    for B in (3, 20, 70, 300):
+        x = rnd(1, B, 300, dtype=torch.bfloat16).to(DEV)
+        y = q.linear_fp8(x, w)
+        bad = x.clone()
+        bad[1, 5], bad[2, 299] = float("nan"), float("inf")
+        z = q.linear_fp8(bad, w)
+        keep = [r for r in range(B) if r not in (1, 2)]
+        assert torch.equal(y[keep], z[keep]) and torch.isnan(z[1:3]).all()
+
+
+def test_linear_empty_and_repeated():
+    w = q.quantize_fp8(rnd(2, 3, 40, 100).to(DEV), 128)
+    assert q.linear_fp8(rnd(1, 0, 100).to(DEV), w).shape == (3, 0, 40)
+    x = rnd(1, 70, 100).to(DEV)
+    first = q.linear_fp8(x, w)
+    assert all(torch.equal(first, q.linear_fp8(x, w)) for _ in range(3))
+
+
+# ---------------------------------------------------------------------------------------------------------------- router
+def route_check(logits, k, **kw):
+    r = q.route_experts(logits.to(DEV), k, **{n: (v.to(DEV) if isinstance(v, torch.Tensor) else v) for n, v in kw.items()})
+    E = logits.shape[-1]
+    l = f64(logits).reshape(-1, logits.shape[-2], E)
+    okw = {n: (f64(v) if isinstance(v, torch.Tensor) else v) for n, v in kw.items()}
+    if okw.get("groups", 1) > 1:
+        okw.setdefault("top_groups", okw["groups"])
+    both = [orc.route(m, torch.finfo(logits.dtype).min, k, **okw) for m in l]
+    W, X = np.stack([b[0] for b in both]), np.stack([b[1] for b in both])
+    lead = logits.shape[:-1]
+    assert tuple(r.weights.shape) == tuple(r.experts.shape) == (*lead, k)
+    assert np.array_equal(r.experts.cpu().numpy().reshape(X.shape), X)
+    g = f64(r.weights).reshape(W.shape)
+    assert np.array_equal(np.isnan(g), np.isnan(W))
+    # scores in 64 bits, rounded once; a score of the fp32 path is off by the exponential's argument (2^-24 |l - max|), its own rounding and the sum's
+    spread = np.nanmax(np.abs(np.where(np.isfinite(l), l, 0)), initial=0) * 2
+    ok = np.isnan(W) | (np.abs(g - W) <= np.abs(W) * (2.0 ** -24 * min(spread, 180.0) + (E + 16) * 2.0 ** -24) + 2.0 ** -126)
+    assert ok.all()
+    off, rows = orc.order_of(X, E)
+    assert np.array_equal(r.offsets.cpu().numpy(), off) and np.array_equal(r.rows.cpu().numpy(), rows)
+    return r
+
+
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 8, 2), (5, 3, 3), (63, 60, 4), (64, 64, 6), (65, 65, 8), (300, 128, 1), (129, 130, 7), (1000, 256, 8), (77, 512, 16), (40, 1024, 32), (4097, 16, 2)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_router(T, E, k, dtype):
+    for score, renorm in itertools.product(("softmax", "sigmoid"), (False, True)):
+        route_check(rnd(5, T, E, by=2.0, dtype=dtype), k, score=score, renormalize=renorm)
+
+
+@pytest.mark.parametrize("T,E,k,groups,kept", [(70, 8, 2, 2, 1), (33, 60, 5, 4, 3), (100, 256, 8, 8, 4), (9, 12, 3, 12, 5), (50, 512, 6, 64, 2), (21, 64, 4, 1, 1), (64, 192, 32, 3, 1), (13, 1024, 8, 16, 4)])
+def test_router_groups_and_bias(T, E, k, groups, kept):
+    for dtype, score in itertools.product((torch.float32, torch.bfloat16), ("softmax", "sigmoid")):
+        l = rnd(6, T, E, by=1.5, dtype=dtype)
+        route_check(l, k, score=score, groups=groups, top_groups=kept, renormalize=True, scale=2.5)
+        route_check(l, k, score=score, groups=groups, top_groups=kept, bias=rnd(7, E, by=0.2))
+
+
+def test_router_samples_and_strides():
+    wide = rnd(8, 3, 50, 100, dtype=torch.float16)
+    route_check(wide, 3)
+    for v in (wide[:, 1::2, 3:40], wide[1, :, 5:6], wide.transpose(0, 1), wide[:, :, ::3]):
+        route_check(v, 1)
+    assert q.route_experts(wide[:, :0].to(DEV), 2).offsets.tolist() == [0] * 301
+    assert q.route_experts(wide[0, :0].to(DEV), 2).experts.shape == (0, 2)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(score="sigmoid"), dict(bias=True), dict(score="sigmoid", bias=True, groups=4, top_groups=2), dict(groups=4, top_groups=3, renormalize=True), dict(renormalize=True, bias=True)], ids=str)
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_router_masks_and_ties(dtype, kw):
+    """Rows with equal logits, masked with -inf or the type's lowest value (all but one, all), with NaN and with +inf."""
+    E = 16
+    l = rnd(9, 12, E, dtype=dtype)
+    low = torch.finfo(dtype).min
+    l[0] = 1.0
+    l[1, 3:] = l[1, 3]
+    l[2, ::2] = float("-inf")
+    l[3, 1:] = float("-inf")
+    l[4] = float("-inf")
+    l[5, :9] = low
+    l[6] = low
+    l[7, 4] = float("nan")
+    l[8] = float("nan")
+    l[10] = -0.0
+    l[10, ::2] = 0.0
+    l[11, 5:11] = 100.0 if dtype != torch.float16 else 60000.0
+    kw = dict(kw)
+    if kw.get("bias"):
+        kw["bias"] = rnd(10, E, by=0.3)
+    for k in (1, 3, 8):
+        route_check(l, k, **kw)
+
+
+def test_router_infinite_logit():
+    l = rnd(9, 3, 16)
+    l[1, 6] = float("inf")
+    r = q.route_experts(l.to(DEV), 3)
+    assert torch.isfinite(r.weights[[0, 2]]).all() and torch.isnan(r.weights[1]).all() and r.experts[1, 0].item() == 6
+    s = q.route_experts(l.to(DEV), 3, score="sigmoid")
+    assert s.weights[1, 0].item() == 1.0 and torch.isfinite(s.weights).all()
+
+
+@pytest.mark.parametrize("groups", [1, 4])
+def test_router_near_ties_under_a_bias(groups):
+    """Scores that differ by less than fp32's last place are told apart: their keys are compared in 64 bits."""
+    E, T = 64, 200
+    l = (1.0 + rnd(11, T, E, by=3e-7)).float()
+    bias = torch.full((E,), 0.5)
+    for score in ("softmax", "sigmoid"):
+        route_check(l, 8, score=score, bias=bias, groups=groups, top_groups=max(1, groups // 2))
+
+
+# ---------------------------------------------------------------------------------------------------------------- experts
+def experts_case(seed, S, T, E, k, D, H, N, dtype, bias, own=True, shared_x=False, logits=None):
+    lead = (S,) if own else ()
+    x = rnd(seed, 1 if shared_x else S, T, D, dtype=dtype)
+    l = rnd(seed + 1, S, T, E, by=2.0) if logits is None else logits
+    up, down = (q.quantize_fp8(rnd(seed + i, *lead, E, r, c, by=c ** -0.5).to(DEV), 128) for i, r, c in ((2, H, D), (3, N, H)))
+    bu, bd = (rnd(seed + 4, *lead, E, H, by=0.2), rnd(seed + 5, *lead, E, N, by=0.2)) if bias else (None, None)
+    r = q.route_experts(l.to(DEV), k, renormalize=True)
+    y = q.experts_fp8(x.to(DEV), r, up, down, *(None if b is None else b.to(DEV) for b in (bu, bd)))
+    uv, dv = held(up), held(down)
+    at = (lambda m: (lambda s, e: m[s, e])) if own else (lambda m: (lambda s, e: m[e]))
+    xv = np.stack([orc.quantised(m, 1) for m in f64(x)])
+    xv = np.repeat(xv, S, 0) if shared_x else xv
+    want, bound = orc.experts(xv, f64(r.weights), r.experts.cpu().numpy(), at(uv), at(dv), *(None if b is None else at(f64(b)) for b in (bu, bd)), NAME[dtype])
+    assert y.dtype == dtype
+    check(y, want, bound)
+    return x, r, up, down, y
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("case", [(1, 1, 1, 1, 1, 1, 1), (1, 1, 8, 2, 128, 256, 128), (1, 7, 4, 4, 100, 70, 130), (2, 40, 6, 3, 129, 200, 90), (1, 300, 5, 2, 256, 384, 256), (3, 100, 12, 1, 77, 300, 77),
+                                  (1, 700, 3, 2, 200, 260, 300), (1, 20, 100, 6, 64, 64, 64)], ids=str)
+def test_experts(case, dtype):
+    experts_case(20, *case, dtype, True)
+    experts_case(21, *case, dtype, False, own=False, shared_x=True)
+
+
+def test_experts_uneven():
+    """Every row to one expert; experts without a row; one row behind a tile's end."""
+    for T in (16, 17, 64, 65, 129, 257):
+        l = torch.zeros(1, T, 9)
+        l[..., 4] = 5.0
+        l[0, 0, 7] = 6.0
+        experts_case(30, 1, T, 9, 1, 128, 130, 100, torch.bfloat16, True, logits=l)
+
+
+def test_experts_masked_choice_adds_nothing():
+    """A masked expert that fills up a row's choices has weight 0: what it computes, NaN included, is left out."""
+    T, E, D, H, k = 10, 4, 64, 64, 2
+    l = rnd(1, T, E)
+    l[:, 1:] = float("-inf")
+    up, down = rnd(2, E, H, D), rnd(3, E, D, H)
+    r = q.route_experts(l.to(DEV), k)
+    x = rnd(4, T, D).to(DEV)
+    y = q.experts_fp8(x, r, q.quantize_fp8(up.to(DEV), 128), q.quantize_fp8(down.to(DEV), 128))
+    down[1:] = float("nan")
+    z = q.experts_fp8(x, r, q.quantize_fp8(up.to(DEV), 128), q.quantize_fp8(down.to(DEV), 128))
+    assert torch.equal(y, z) and torch.isfinite(y).all()
+
+
+def test_experts_empty():
+    r = q.route_experts(torch.zeros(2, 0, 4, device=DEV), 2)
+    w = q.quantize_fp8(torch.randn(4, 64, 64, device=DEV), 128)
+    assert q.experts_fp8(torch.zeros(2, 0, 64, device=DEV), r, w, w).shape == (2, 0, 64)
+
+
+# ---------------------------------------------------------------------------------------------------------------- together, as used
+def test_stochastic_layer():
+    """fp8.Linear: its samples' weights are models_f32.Linear's, quantised; the result is the 64-bit product of what both operands hold."""
+    from quantised_bayesian_nets_amd import fp8
+    torch.manual_seed(0)
+    m = fp8.Linear(200, 70, True)
+    m.layer_id = 3
+    x = rnd(1, 1, 9, 200).to(DEV)
+    with q.mc_context(4, 77, 2):
+        w = m.sampled(x.device).view(4, 70, 200)
+        y = m(x, act=1)
+    xv = orc.quantised(f64(x[0]), 1)
+    for s in range(4):
+        wv = orc.quantised(f64(w[s]), 128)
+        check(y[s], orc.product(xv, wv, f64(m.bias), True), orc.product_bound(xv, wv, f64(m.bias)) + 2.0 ** -149)
+    assert not torch.equal(w[0], w[1])
+
+
+def test_captured_graph_replays():
+    """Router, quantiser and products in one captured graph: every replay, on new inputs, equals the eager call."""
+    S, T, E, D, H = 2, 33, 6, 150, 260
+    up, down = (q.quantize_fp8(rnd(i, E, r, c, by=0.1).to(DEV), 128) for i, r, c in ((2, H, D), (3, D, H)))
+    gate = q.quantize_fp8(rnd(4, E, D).to(DEV), 128)
+
+    def step(x):
+        r = q.route_experts(q.linear_fp8(x, gate, out_dtype=torch.float32), 2, renormalize=True)
+        return q.experts_fp8(x, r, up, down)
+
+    x = rnd(1, S, T, D, dtype=torch.bfloat16).to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(x)
+        graphs.append((g, out))
+    for i in range(4):
+        x.copy_(rnd(50 + i, S, T, D, dtype=torch.bfloat16))
+        want = step(x)
+        g, out = graphs[i % 2]
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_two_streams_at_once():
+    w = q.quantize_fp8(rnd(2, 300, 500).to(DEV), 128)
+    xs = [rnd(i, 40, 500).to(DEV) for i in range(2)]
+    want = [q.linear_fp8(x, w) for x in xs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(q.linear_fp8(xs[i], w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
