@@ -5,9 +5,12 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
+#include <atomic>
+#include <type_traits>
 
 #include "../../include/qbnn.h"
 #include "qbnn_common.h"
+#include "qbnn_conv.h"          // LDS-DMA requests, their counted waits, LDS-only barrier
 #include "qbnn_f8.h"
 
 using namespace qbnn;
@@ -136,8 +139,21 @@ struct F8Args {
 
 struct F8Tile { int m0, m1, set, sample; };     // rows m0 .. m1 - 1, weight set, sample (0 for groups: rows are global)
 
-// The tile of this workgroup.  Groups: tile `t` of the sequence of every group's ceil(rows / TM) tiles; each wave finds it with one pass
-// over the offsets, 64 groups at a time; false if there are fewer tiles (the grid is sized for the worst split of the rows).
+// Groups: the tiles of every group's rows in a row, ceil(rows / TM) each.  One wave-wide pass over the offsets, 64 groups at a time.
+template <int TM> __device__ __forceinline__ int f8_group_tiles(const F8Args& a, int g, int& b, int& n) {
+  b = 0; n = 0;
+  if (g < a.groups) { b = a.offsets[g]; n = a.offsets[g + 1] - b; }
+  return (n + TM - 1) / TM;
+}
+template <int TM> __device__ __forceinline__ int f8_count_tiles(const F8Args& a) {
+  const int lane = threadIdx.x & 63;
+  int sum = 0, b, n;
+  for (int g0 = 0; g0 < a.groups; g0 += 64) sum += f8_group_tiles<TM>(a, g0 + lane, b, n);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  return __builtin_amdgcn_readfirstlane(sum);
+}
+// tile t (of a grid sized for the worst split of the rows); false if there are fewer
 template <int TM, bool GROUPED> __device__ __forceinline__ bool f8_find_tile(const F8Args& a, int t, int z, F8Tile& o) {
   if constexpr (!GROUPED) {
     o.m0 = t * TM; o.m1 = min(a.M, o.m0 + TM); o.set = z; o.sample = z;
@@ -146,10 +162,8 @@ template <int TM, bool GROUPED> __device__ __forceinline__ bool f8_find_tile(con
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int g0 = 0; g0 < a.groups; g0 += 64) {
-      const int g = g0 + lane;
-      int b = 0, n = 0;
-      if (g < a.groups) { b = a.offsets[g]; n = a.offsets[g + 1] - b; }
-      const int tiles = (n + TM - 1) / TM;
+      int b, n;
+      const int tiles = f8_group_tiles<TM>(a, g0 + lane, b, n);
       int incl = tiles;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) { const int u = __shfl_up(incl, d); if (lane >= d) incl += u; }
@@ -159,7 +173,9 @@ template <int TM, bool GROUPED> __device__ __forceinline__ bool f8_find_tile(con
         const unsigned long long hit = __ballot(t >= mine && t < mine + tiles);
         const int src = __ffsll(hit) - 1;
         const int k = t - __shfl(mine, src), bb = __shfl(b, src), nn = __shfl(n, src);
-        o.m0 = bb + k * TM; o.m1 = min(bb + nn, o.m0 + TM); o.set = (g0 + src) % a.w_groups; o.sample = 0;
+        o.m0 = __builtin_amdgcn_readfirstlane(bb + k * TM);
+        o.m1 = __builtin_amdgcn_readfirstlane(min(bb + nn, bb + k * TM + TM));
+        o.set = __builtin_amdgcn_readfirstlane((g0 + src) % a.w_groups); o.sample = 0;
         return true;
       }
       before += total;
@@ -318,10 +334,295 @@ template <int MT, int NT, int NW, int OUT, bool EXACT, bool GROUPED> int launch_
   return qbnn_check_launch_msg("qbnn_linear_f8");
 }
 
+// Tiled form: TM activation rows x TN weight rows per workgroup, WM x WN waves of (32 MI) x 128 each, one block of 128 columns per step.
+// Both operands' rows go to LDS by DMA, two steps in two buffers; a row's eight 16-byte pieces lie permuted (piece c of row r at c ^ f(r)), so that
+// eight lanes in a row start in different banks.  What bounds it at large sizes is the matrix unit: 4 waves of 128 x 128 read 2 x 16 KiB each and step, 128 KiB at
+// 128 B/clk = 1024 cycles, for 32 instructions of 64 cycles; with waves of 128 x 64 the LDS would be the bound.  The 32 x 32 form of the instruction, because
+// its accumulators are tied in place (the 16 x 16 form's are renamed, which cost 3 register moves per instruction here) and it reads half the operand registers.
+// One barrier per step, in front of the last activation fragment's products: before it the wave waits for its share of the next step's bytes; behind it
+// the buffer just read is requested again and the next step's first fragments are read, each weight fragment's registers as soon as their products are issued.
+// Weight fragment j holds rows 32 j + 16 (r / 16) + 8 ((r / 4) & 1) + 4 ((r / 8) & 1) + r % 4 (r = 0 .. 31) of the wave's 128, so that a lane ends up with runs of 8
+// neighbouring results of a row and a pair of lanes with 16: whole sectors per store.
+template <int MI, int WM, int WN> struct F8Tiled {
+  static constexpr int TM = 32 * MI * WM, TN = 128 * WN, WAVES = WM * WN, XB = TM * 128, WB = TN * 128, LDS = 2 * (XB + WB);
+  static constexpr int PX = TM / 8 / WAVES, PW = TN / 8 / WAVES;      // DMA requests (8 rows each) per wave and step
+  static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && LDS <= 160 * 1024 && 2 * XB <= 65536 && 2 * WB <= 65536, "immediate offsets of the reads");
+};
+typedef float f8_v16f __attribute__((ext_vector_type(16)));
+
+// 8 neighbouring results n .. n + 7 of an activation row
+template <int OUT> __device__ __forceinline__ void f8_put8(const F8Args& a, f8_type<OUT>* y, int n, const float (&v)[8]) {
+  f8_type<OUT> o[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) o[c] = f8_store<OUT>(v[c]);
+  if (n + 8 <= a.N) __builtin_memcpy(y + n, o, sizeof(o));
+  else
+    for (int c = 0; c < 8; ++c) if (n + c < a.N) y[n + c] = o[c];
+}
+
+template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED>
+__global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const F8Args a, int tiles_m, int tiles_n) {
+  using C = F8Tiled<MI, WM, WN>;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, h = lane >> 5;
+  const int wm = wave / WN, wn = wave % WN;
+
+  // Workgroups of one XCD (every eighth) take neighbouring tiles, in columns of 4 row tiles: what they read at a time shares its L2
+  F8Tile t;
+  int n0;
+  {
+    const int tm = GROUPED ? f8_count_tiles<C::TM>(a) : tiles_m, total = tm * tiles_n;
+    const int p = blockIdx.x;
+    if (p >= total) return;
+    const int per = total >> 3, rest = total & 7, xcd = p & 7;
+    const int q = xcd * per + min(xcd, rest) + (p >> 3);
+    const int band = q / (4 * tiles_n), in = q - band * (4 * tiles_n), rows = min(4, tm - band * 4);
+    const int col = in / rows;
+    n0 = col * C::TN;
+    if (!f8_find_tile<C::TM, GROUPED>(a, band * 4 + in - col * rows, blockIdx.z, t)) return;
+  }
+  const int64_t pitch = (int64_t)a.Kb * 128;
+  const uint8_t* xg = a.x + (int64_t)t.sample * a.x_ss;
+  const uint8_t* wg = a.w + (int64_t)t.set * a.w_ss + n0 * pitch;
+  if constexpr (!GROUPED) xg += t.m0 * pitch;
+
+  // per-lane byte offsets of this wave's DMA requests; rows behind the last repeat it (their results are not stored)
+  uint32_t xo[C::PX], wo[C::PW];
+#pragma unroll
+  for (int p = 0; p < C::PX; ++p) {
+    const int r = (p * C::WAVES + wave) * 8 + (lane >> 3), i = min(t.m0 + r, t.m1 - 1);
+    const int row = GROUPED ? f8_x_row<GROUPED>(a, i) : i - t.m0;
+    xo[p] = (uint32_t)(row * pitch) + (((lane & 7) ^ (r & 7)) << 4);
+  }
+#pragma unroll
+  for (int p = 0; p < C::PW; ++p) {
+    const int r = (p * C::WAVES + wave) * 8 + (lane >> 3);
+    wo[p] = (uint32_t)(min(r, a.N - 1 - n0) * pitch) + (((lane & 7) ^ ((r & 3) | ((r >> 1) & 4))) << 4);
+  }
+  const uint32_t lds0 = lds_addr_of(lds);
+  auto request = [&](int kb, int buf) {
+    const uint32_t at = lds0 + wave * 1024;
+#pragma unroll
+    for (int p = 0; p < C::PX; ++p) dma16_s(xg + kb * 128, xo[p], at + buf * C::XB + p * (C::WAVES * 1024));
+#pragma unroll
+    for (int p = 0; p < C::PW; ++p) dma16_s(wg + kb * 128, wo[p], at + 2 * C::XB + buf * C::WB + p * (C::WAVES * 1024));
+  };
+
+  // exponents: dwords of four blocks
+  const uint8_t* xeg = a.xe + (int64_t)t.sample * a.xe_ss;
+  uint32_t xeo[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) xeo[i] = (uint32_t)f8_x_row<GROUPED>(a, min(t.m0 + (wm * MI + i) * 32 + r32, t.m1 - 1)) * (uint32_t)a.Sp;
+  const uint32_t* we = (const uint32_t*)(a.we + (int64_t)t.set * a.we_ss + (int64_t)min((n0 >> 7) + wn, (a.N - 1) >> 7) * a.Sp);
+  uint32_t xs[MI], xn[MI], ws = we[0], wnx = ws;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) xs[i] = xn[i] = *(const uint32_t*)(xeg + xeo[i]);
+
+  // a fragment of 32 rows x 128 columns: instruction s = 0, 1 of the two takes pieces 4 s + h and 4 s + 2 + h
+  struct Frag { f8_v8i k[2]; };
+  const uint8_t* xl = lds + wm * MI * 4096 + r32 * 128;
+  const uint8_t* wl = lds + 2 * C::XB + wn * 16384 + ((r32 >> 4) * 16 + ((r32 >> 2) & 1) * 8 + ((r32 >> 3) & 1) * 4 + (r32 & 3)) * 128;
+  const int piece = (h ^ (r32 & 7)) << 4;
+  const uint8_t *x0 = xl + piece, *x1 = xl + (piece ^ 32), *x2 = xl + (piece ^ 64), *x3 = xl + (piece ^ 96);
+  const uint8_t *w0 = wl + piece, *w1 = wl + (piece ^ 32), *w2 = wl + (piece ^ 64), *w3 = wl + (piece ^ 96);
+  auto read_x = [&](int buf, int i) {
+    const int at = buf * C::XB + i * 4096;
+    return Frag{{f8_join(*(const f8_v4i*)(x0 + at), *(const f8_v4i*)(x1 + at)), f8_join(*(const f8_v4i*)(x2 + at), *(const f8_v4i*)(x3 + at))}};
+  };
+  auto read_w = [&](int buf, int j) {
+    const int at = buf * C::WB + j * 4096;
+    return Frag{{f8_join(*(const f8_v4i*)(w0 + at), *(const f8_v4i*)(w1 + at)), f8_join(*(const f8_v4i*)(w2 + at), *(const f8_v4i*)(w3 + at))}};
+  };
+  f8_v16f acc[MI][4];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 16; ++c) acc[i][j][c] = 0.f;
+
+  // a request past the last step repeats the last one's bytes, into a buffer that is not read again: the loop stays free of branches, over which the
+  // compiler would move the matrix instructions and spill their operands
+  const int last = a.Kb - 1;
+  request(0, 0);
+  request(min(1, last), 1);
+  wait_vmcnt<C::PX + C::PW>();
+  lds_barrier();
+
+  if constexpr (!EXACT) {
+    Frag wf[4], xf[2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) wf[j] = read_w(0, j);
+    xf[0] = read_x(0, 0);
+    // even and odd steps differ in the buffer and in the byte B of xs / ws that holds their exponents
+    auto step = [&](auto Bc, int kb) {
+      constexpr int B = decltype(Bc)::value;
+      constexpr int X0 = MI & 1 ? B : 0;      // registers of the step's first activation fragment
+      auto mfma = [&](int i, int j, int s) {
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j].k[s], xf[(i + X0) & 1].k[s], acc[i][j], 0, 0, B, (int)ws, B, (int)xs[i]);
+      };
+#pragma unroll
+      for (int i = 0; i < MI - 1; ++i) {
+        xf[(i + 1 + X0) & 1] = read_x(B, i + 1);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) mfma(i, u & 3, u >> 2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      wait_vmcnt<0>();
+      lds_barrier();
+      if constexpr (B == 0) {
+        const int at = min(kb + 2, last) >> 2;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) xn[i] = *(const uint32_t*)(xeg + xeo[i] + at * 4);
+        wnx = we[at];
+      }
+      xf[(MI + X0) & 1] = read_x(B ^ 1, 0);
+      request(min(kb + 2, last), B);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mfma(MI - 1, j + (u & 1), u >> 1);
+        wf[j] = read_w(B ^ 1, j);
+        wf[j + 1] = read_w(B ^ 1, j + 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    int kb = 0;
+    for (; kb < last; kb += 2) {
+      step(std::integral_constant<int, 0>{}, kb);
+      step(std::integral_constant<int, 1>{}, kb + 1);
+      const int by = ((kb + 2) & 2) * 8;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) xs[i] = xn[i] >> by;
+      ws = wnx >> by;
+    }
+    if (kb == last) step(std::integral_constant<int, 0>{}, kb);
+  } else {
+    for (int kb = 0; kb < a.Kb; ++kb) {
+      const int buf = kb & 1;
+      if ((kb & 3) == 0) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) xs[i] = *(const uint32_t*)(xeg + xeo[i] + kb);
+        ws = we[kb >> 2];
+      }
+      F8Wide xw[MI][2];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const Frag f = read_x(buf, i);
+        xw[i][0] = f8_widen(f.k[0]);
+        xw[i][1] = f8_widen(f.k[1]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const Frag f = read_w(buf, j);
+        const F8Wide ww[2] = {f8_widen(f.k[0]), f8_widen(f.k[1])};
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          f8_v16f c;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) c[k] = 0.f;
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ww[s].part[g], xw[i][s].part[g], c, 0, 0, 0);
+          const int e = (int)(ws & 255) + (int)(xs[i] & 255) - 254;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) acc[i][j][k] += __builtin_ldexpf(c[k], e);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MI; ++i) xs[i] >>= 8;
+      ws >>= 8;
+      wait_vmcnt<0>();
+      lds_barrier();
+      request(min(kb + 2, last), buf);
+    }
+  }
+  wait_vmcnt<0>();          // (no request outlives the workgroup's LDS)
+
+  // lane: activation row r32 of fragment i, weight rows 32 j + 16 p + 8 h .. + 7 in registers 8 p .. + 7
+  const int nw = n0 + wn * 128;
+  if (nw >= a.N) return;
+  const float* bias = a.bias ? a.bias + (int64_t)t.set * a.bias_ss : nullptr;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int row = t.m0 + (wm * MI + i) * 32 + r32;
+    int64_t to = row;
+    float s = 1.f;
+    bool weighed = false;
+    if constexpr (GROUPED && OUT != QBNN_F8) {
+      if (a.y_rows && row < t.m1) { to = a.y_rows[row]; s = a.scale[to]; weighed = true; }
+    }
+    auto values = [&](int q, float (&v)[8]) {
+      const int n = nw + q * 16 + h * 8;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        float u = acc[i][q >> 1][(q & 1) * 8 + c];
+        if (bias) u += bias[min(n + c, a.N - 1)];
+        if (a.relu) u = u > 0.f ? u : (u != u ? u : 0.f);
+        if (weighed) u = s == 0.f ? 0.f : u * s;
+        if (OUT == QBNN_F8 && n + c >= a.N) u = 0.f;
+        v[c] = u;
+      }
+    };
+    if constexpr (OUT == QBNN_F8) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        float v[8];
+        values(q, v);
+        m = max(m, f8_max8(v));
+      }
+      m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+      const int e = f8_exponent(m);
+      const float down = f8_pow2(-e);
+      if (row < t.m1) {
+        uint8_t* y = a.y + (int64_t)t.sample * a.y_ss + (int64_t)row * a.y_rs + nw + h * 8;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          float v[8];
+          values(q, v);
+          *(f8_v2i*)(y + q * 16) = f8_scale8(v, down);
+        }
+        if (h == 0) f8_put_exponent(a.ye + ((int64_t)t.sample * a.M + row) * a.ye_rs, nw >> 7, (a.N + 127) >> 7, a.ye_rs, e);
+      }
+    } else if (row < t.m1) {
+      f8_type<OUT>* y = (f8_type<OUT>*)a.y + (int64_t)t.sample * a.y_ss + to * a.y_rs;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        float v[8];
+        values(q, v);
+        f8_put8<OUT>(a, y, nw + q * 16 + h * 8, v);
+      }
+    }
+  }
+}
+
+template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED> int launch_tiled(const F8Args& a, int rows, int z, hipStream_t st) {
+  using C = F8Tiled<MI, WM, WN>;
+  static std::atomic<uint64_t> attr{0};
+  if (int rc = qbnn_ensure_dyn_lds((const void*)linear_f8_tiled_kernel<MI, WM, WN, OUT, EXACT, GROUPED>, &attr, C::LDS)) return rc;
+  const int64_t tm = (rows + C::TM - 1) / C::TM + (GROUPED ? a.groups : 0), tn = (a.N + C::TN - 1) / C::TN;
+  if (tm * tn > 0x7fffffff || z > 65535) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
+  hipLaunchKernelGGL((linear_f8_tiled_kernel<MI, WM, WN, OUT, EXACT, GROUPED>), dim3((unsigned)(tm * tn), 1, (unsigned)z), dim3(C::WAVES * 64), C::LDS, st, a,
+                     (int)tm, (int)tn);
+  return qbnn_check_launch_msg("qbnn_linear_f8");
+}
+
 // rows: the rows of one sample, or all routed rows
 template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, int rows, int z, hipStream_t st) {
   const int spare = GROUPED ? a.groups : 0;        // each group may end inside a tile
   const int per = GROUPED ? (rows + a.groups - 1) / a.groups : rows;
+  // offsets are 32 bits wide in the tiled form: of a gathered row's bytes from the first, of any row's exponents, of a weight row's in its tile
+  const int64_t far = GROUPED ? (int64_t)(a.rows ? a.x_rows : rows) * a.Kb * 128 : (int64_t)rows * a.Sp;
+  const bool near = far < ((int64_t)1 << 32) && a.Kb < (1 << 16);
+  if (per > 64 && near) {
+    if constexpr (!EXACT) {
+      if (per >= 192) return launch_tiled<4, 2, 2, OUT, EXACT, GROUPED>(a, rows, z, st);
+    }
+    return launch_tiled<2, 2, 2, OUT, EXACT, GROUPED>(a, rows, z, st);
+  }
   if constexpr (OUT == QBNN_F8) {
     if (per <= 16) return launch_direct<1, 8, 4, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
     return launch_direct<2, 8, 4, OUT, EXACT, GROUPED>(a, (rows + 31) / 32 + spare, z, st);
