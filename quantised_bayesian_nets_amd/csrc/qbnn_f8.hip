@@ -360,6 +360,88 @@ template <int OUT> __device__ __forceinline__ void f8_put8(const F8Args& a, f8_t
     for (int c = 0; c < 8; ++c) if (n + c < a.N) y[n + c] = o[c];
 }
 
+// Workgroups of one XCD (every eighth) take neighbouring tiles, in columns of 4 row tiles: what they read at a time shares its L2.  false: no tile.
+template <int TM, int TN, bool GROUPED> __device__ __forceinline__ bool f8_locate(const F8Args& a, int tiles_m, int tiles_n, F8Tile& t, int& n0) {
+  const int tm = GROUPED ? f8_count_tiles<TM>(a) : tiles_m, total = tm * tiles_n;
+  const int p = blockIdx.x;
+  if (p >= total) return false;
+  const int per = total >> 3, rest = total & 7, xcd = p & 7;
+  const int q = xcd * per + min(xcd, rest) + (p >> 3);
+  const int band = q / (4 * tiles_n), in = q - band * (4 * tiles_n), rows = min(4, tm - band * 4);
+  const int col = in / rows;
+  n0 = col * TN;
+  return f8_find_tile<TM, GROUPED>(a, band * 4 + in - col * rows, blockIdx.z, t);
+}
+
+// Results of a wave's (32 MI) x 128 tile from row m, weight row nw on.  Lane: activation row r32 of fragment i, weight rows 16 q + 8 h .. + 7 in registers
+// 8 (q & 1) .. + 7 of fragment q / 2.
+template <int MI, int OUT, bool GROUPED> __device__ __forceinline__ void f8_finish(const F8Args& a, const F8Tile& t, int m, int nw, f8_v16f (&acc)[MI][4]) {
+  const int r32 = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
+  if (nw >= a.N) return;
+  const float* bias = a.bias ? a.bias + (int64_t)t.set * a.bias_ss : nullptr;
+  int64_t to[MI];
+  float s[MI];
+  bool weighed = false;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int row = m + i * 32 + r32;
+    to[i] = row;
+    s[i] = 1.f;
+    if constexpr (GROUPED && OUT != QBNN_F8) {
+      weighed = a.y_rows;
+      if (weighed && row < t.m1) { to[i] = a.y_rows[row]; s[i] = a.scale[to[i]]; }
+    }
+  }
+  uint32_t top[MI] = {};
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const int n = nw + q * 16 + h * 8;
+    float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (bias) {
+      if (n + 8 <= a.N) __builtin_memcpy(b, bias + n, sizeof(b));
+      else
+        for (int c = 0; c < 8; ++c) b[c] = bias[min(n + c, a.N - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      float v[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        float u = acc[i][q >> 1][(q & 1) * 8 + c] + b[c];
+        if (a.relu) u = u > 0.f ? u : (u != u ? u : 0.f);
+        if (GROUPED && weighed) u = s[i] == 0.f ? 0.f : u * s[i];
+        if (OUT == QBNN_F8 && n + c >= a.N) u = 0.f;
+        v[c] = u;
+      }
+      if constexpr (OUT == QBNN_F8) {
+        top[i] = max(top[i], f8_max8(v));
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[i][q >> 1][(q & 1) * 8 + c] = v[c];
+      } else if (m + i * 32 + r32 < t.m1) {
+        f8_put8<OUT>(a, (f8_type<OUT>*)a.y + (int64_t)t.sample * a.y_ss + to[i] * a.y_rs, n, v);
+      }
+    }
+  }
+  if constexpr (OUT == QBNN_F8) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int row = m + i * 32 + r32;
+      const int e = f8_exponent(max(top[i], (uint32_t)__shfl_xor((int)top[i], 32)));
+      const float down = f8_pow2(-e);
+      if (row >= t.m1) continue;
+      uint8_t* y = a.y + (int64_t)t.sample * a.y_ss + (int64_t)row * a.y_rs + nw + h * 8;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        float v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = acc[i][q >> 1][(q & 1) * 8 + c];
+        *(f8_v2i*)(y + q * 16) = f8_scale8(v, down);
+      }
+      if (h == 0) f8_put_exponent(a.ye + ((int64_t)t.sample * a.M + row) * a.ye_rs, nw >> 7, (a.N + 127) >> 7, a.ye_rs, e);
+    }
+  }
+}
+
 template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED>
 __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const F8Args a, int tiles_m, int tiles_n) {
   using C = F8Tiled<MI, WM, WN>;
@@ -367,20 +449,9 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, h = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
 
-  // Workgroups of one XCD (every eighth) take neighbouring tiles, in columns of 4 row tiles: what they read at a time shares its L2
   F8Tile t;
   int n0;
-  {
-    const int tm = GROUPED ? f8_count_tiles<C::TM>(a) : tiles_m, total = tm * tiles_n;
-    const int p = blockIdx.x;
-    if (p >= total) return;
-    const int per = total >> 3, rest = total & 7, xcd = p & 7;
-    const int q = xcd * per + min(xcd, rest) + (p >> 3);
-    const int band = q / (4 * tiles_n), in = q - band * (4 * tiles_n), rows = min(4, tm - band * 4);
-    const int col = in / rows;
-    n0 = col * C::TN;
-    if (!f8_find_tile<C::TM, GROUPED>(a, band * 4 + in - col * rows, blockIdx.z, t)) return;
-  }
+  if (!f8_locate<C::TM, C::TN, GROUPED>(a, tiles_m, tiles_n, t, n0)) return;
   const int64_t pitch = (int64_t)a.Kb * 128;
   const uint8_t* xg = a.x + (int64_t)t.sample * a.x_ss;
   const uint8_t* wg = a.w + (int64_t)t.set * a.w_ss + n0 * pitch;
@@ -541,62 +612,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
   }
   wait_vmcnt<0>();          // (no request outlives the workgroup's LDS)
 
-  // lane: activation row r32 of fragment i, weight rows 32 j + 16 p + 8 h .. + 7 in registers 8 p .. + 7
-  const int nw = n0 + wn * 128;
-  if (nw >= a.N) return;
-  const float* bias = a.bias ? a.bias + (int64_t)t.set * a.bias_ss : nullptr;
-#pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int row = t.m0 + (wm * MI + i) * 32 + r32;
-    int64_t to = row;
-    float s = 1.f;
-    bool weighed = false;
-    if constexpr (GROUPED && OUT != QBNN_F8) {
-      if (a.y_rows && row < t.m1) { to = a.y_rows[row]; s = a.scale[to]; weighed = true; }
-    }
-    auto values = [&](int q, float (&v)[8]) {
-      const int n = nw + q * 16 + h * 8;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        float u = acc[i][q >> 1][(q & 1) * 8 + c];
-        if (bias) u += bias[min(n + c, a.N - 1)];
-        if (a.relu) u = u > 0.f ? u : (u != u ? u : 0.f);
-        if (weighed) u = s == 0.f ? 0.f : u * s;
-        if (OUT == QBNN_F8 && n + c >= a.N) u = 0.f;
-        v[c] = u;
-      }
-    };
-    if constexpr (OUT == QBNN_F8) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        float v[8];
-        values(q, v);
-        m = max(m, f8_max8(v));
-      }
-      m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-      const int e = f8_exponent(m);
-      const float down = f8_pow2(-e);
-      if (row < t.m1) {
-        uint8_t* y = a.y + (int64_t)t.sample * a.y_ss + (int64_t)row * a.y_rs + nw + h * 8;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          float v[8];
-          values(q, v);
-          *(f8_v2i*)(y + q * 16) = f8_scale8(v, down);
-        }
-        if (h == 0) f8_put_exponent(a.ye + ((int64_t)t.sample * a.M + row) * a.ye_rs, nw >> 7, (a.N + 127) >> 7, a.ye_rs, e);
-      }
-    } else if (row < t.m1) {
-      f8_type<OUT>* y = (f8_type<OUT>*)a.y + (int64_t)t.sample * a.y_ss + to * a.y_rs;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        float v[8];
-        values(q, v);
-        f8_put8<OUT>(a, y, nw + q * 16 + h * 8, v);
-      }
-    }
-  }
+  f8_finish<MI, OUT, GROUPED>(a, t, t.m0 + wm * MI * 32, n0 + wn * 128, acc);
 }
 
 template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED> int launch_tiled(const F8Args& a, int rows, int z, hipStream_t st) {
@@ -610,6 +626,143 @@ template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED> int launch_
   return qbnn_check_launch_msg("qbnn_linear_f8");
 }
 
+// The largest tile, 256 x 256: the tiled form's data paths with a deeper ring.  A step's two operands are 32 KiB each and take turns in five slots, so that
+// three requests (96 KiB) are in flight, each for three half steps (3072 matrix cycles): with the two buffers of the form above the wait for a request one
+// step old was a quarter of the time.  A step has two halves of 16 instructions, a barrier in front of each:
+//   first   x0, x1 times w;  reads x2, x3 and the next step's w0, w1      frees the slot of this step's w, needs the next step's w
+//   second  x2, x3 times w;  reads the next step's w2, w3, x0, x1         frees the slot of this step's x, needs the next step's x
+// so that every fragment is read half a step before it is used and 16 reads go with 16 instructions.
+template <int OUT, bool GROUPED>
+__global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, int tiles_m, int tiles_n) {
+  constexpr int SLOT = 32768, SLOTS = 5;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, h = lane >> 5;
+  const int wm = wave >> 1, wn = wave & 1;
+  F8Tile t;
+  int n0;
+  if (!f8_locate<256, 256, GROUPED>(a, tiles_m, tiles_n, t, n0)) return;
+  const int64_t pitch = (int64_t)a.Kb * 128;
+  const uint8_t* xg = a.x + (int64_t)t.sample * a.x_ss;
+  const uint8_t* wg = a.w + (int64_t)t.set * a.w_ss + n0 * pitch;
+  if constexpr (!GROUPED) xg += t.m0 * pitch;
+  uint32_t xo[8], wo[8];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const int r = (p * 4 + wave) * 8 + (lane >> 3), i = min(t.m0 + r, t.m1 - 1);
+    xo[p] = (uint32_t)((GROUPED ? f8_x_row<GROUPED>(a, i) : i - t.m0) * pitch) + (((lane & 7) ^ (r & 7)) << 4);
+    wo[p] = (uint32_t)(min(r, a.N - 1 - n0) * pitch) + (((lane & 7) ^ ((r & 3) | ((r >> 1) & 4))) << 4);
+  }
+  const uint32_t lds0 = lds_addr_of(lds) + wave * 1024;
+  const int last = a.Kb - 1;
+  // requests past the last step repeat its bytes, into slots that are not read again (no branch in the loop)
+  auto request_x = [&](int kb, int slot, int p) { dma16_s(xg + min(kb, last) * 128, xo[p], lds0 + slot + p * 4096); };
+  auto request_w = [&](int kb, int slot, int p) { dma16_s(wg + min(kb, last) * 128, wo[p], lds0 + slot + p * 4096); };
+  auto after = [](int slot, int by) { slot += by * SLOT; return slot >= SLOTS * SLOT ? slot - SLOTS * SLOT : slot; };
+
+  const uint8_t* xeg = a.xe + (int64_t)t.sample * a.xe_ss;
+  uint32_t xeo[4], xs[4], xn[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    xeo[i] = (uint32_t)f8_x_row<GROUPED>(a, min(t.m0 + (wm * 4 + i) * 32 + r32, t.m1 - 1)) * (uint32_t)a.Sp;
+    xs[i] = xn[i] = *(const uint32_t*)(xeg + xeo[i]);
+  }
+  const uint32_t* we = (const uint32_t*)(a.we + (int64_t)t.set * a.we_ss + (int64_t)min((n0 >> 7) + wn, (a.N - 1) >> 7) * a.Sp);
+  uint32_t ws = we[0], wnx = ws;
+
+  struct Frag { f8_v8i k[2]; };
+  const int xl = wm * 16384 + r32 * 128 + ((h ^ (r32 & 7)) << 4);
+  const int wl = wn * 16384 + ((r32 >> 4) * 16 + ((r32 >> 2) & 1) * 8 + ((r32 >> 3) & 1) * 4 + (r32 & 3)) * 128 + ((h ^ (r32 & 7)) << 4);
+  // fragment f at base: instruction s = 0, 1 of the two takes pieces 4 s + h and 4 s + 2 + h
+  auto read_half = [&](Frag& o, int base, int f, int s) {
+    const uint8_t* p = lds + f * 4096;
+    o.k[s] = f8_join(*(const f8_v4i*)(p + (base ^ (64 * s))), *(const f8_v4i*)(p + (base ^ (64 * s + 32))));
+  };
+  auto read = [&](Frag& o, int base, int f) { read_half(o, base, f, 0); read_half(o, base, f, 1); };
+  f8_v16f acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 16; ++c) acc[i][j][c] = 0.f;
+
+  // slots in the order of the requests: w0 x0 w1 x1 w2
+#pragma unroll
+  for (int k = 0; k < 5; ++k)
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      if (k & 1) request_x(k >> 1, k * SLOT, p);
+      else request_w(k >> 1, k * SLOT, p);
+    }
+  wait_vmcnt<24>();
+  lds_barrier();
+  Frag wf[2][4], xf[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) read(wf[0][j], wl, j);
+  read(xf[0], xl + SLOT, 0);
+  read(xf[1], xl + SLOT, 1);
+  int slot = 0;                              // of this step's w; x lies one, the next step's w two, its x three further on
+  auto step = [&](auto Bc, int kb) {
+    constexpr int B = decltype(Bc)::value;
+    auto mfma = [&](int i, int j, int s) {
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[B][j].k[s], xf[i].k[s], acc[i][j], 0, 0, B, (int)ws, B, (int)xs[i]);
+    };
+    const int sx = after(slot, 1), sw1 = after(slot, 2), sx1 = after(slot, 3);
+    wait_vmcnt<16>();                        // the next step's w has landed (its x and the w after it may be in flight)
+    lds_barrier();
+    if constexpr (B == 0) {
+      const int at = min(kb + 2, last) >> 2;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xn[i] = *(const uint32_t*)(xeg + xeo[i] + at * 4);
+      wnx = we[at];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {            // two instructions, two reads, one request
+      request_x(kb + 2, slot, g);
+      if (g < 4) read_half(xf[2 + (g >> 1)], xl + sx, 2 + (g >> 1), g & 1);
+      else read_half(wf[B ^ 1][(g >> 1) - 2], wl + sw1, (g >> 1) - 2, g & 1);
+      mfma((g >> 1) & 1, (g >> 2) * 2, g & 1);
+      mfma((g >> 1) & 1, (g >> 2) * 2 + 1, g & 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_vmcnt<16>();                        // the next step's x has landed (the two requests after it may be in flight)
+    lds_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      request_w(kb + 3, sx, g);
+      if (g < 4) read_half(wf[B ^ 1][2 + (g >> 1)], wl + sw1, 2 + (g >> 1), g & 1);
+      else read_half(xf[(g >> 1) - 2], xl + sx1, (g >> 1) - 2, g & 1);
+      mfma(2 + ((g >> 1) & 1), (g >> 2) * 2, g & 1);
+      mfma(2 + ((g >> 1) & 1), (g >> 2) * 2 + 1, g & 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    slot = sw1;
+  };
+  int kb = 0;
+  for (; kb < last; kb += 2) {
+    step(std::integral_constant<int, 0>{}, kb);
+    step(std::integral_constant<int, 1>{}, kb + 1);
+    const int by = ((kb + 2) & 2) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xs[i] = xn[i] >> by;
+    ws = wnx >> by;
+  }
+  if (kb == last) step(std::integral_constant<int, 0>{}, kb);
+  wait_vmcnt<0>();          // (no request outlives the workgroup's LDS)
+  f8_finish<4, OUT, GROUPED>(a, t, t.m0 + wm * 128, n0 + wn * 128, acc);
+}
+
+template <int OUT, bool GROUPED> int launch_big(const F8Args& a, int rows, int z, hipStream_t st) {
+  static std::atomic<uint64_t> attr{0};
+  if (int rc = qbnn_ensure_dyn_lds((const void*)linear_f8_big_kernel<OUT, GROUPED>, &attr, 163840)) return rc;
+  const int64_t tm = (rows + 255) / 256 + (GROUPED ? a.groups : 0), tn = (a.N + 255) / 256;
+  if (tm * tn > 0x7fffffff || z > 65535) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
+  hipLaunchKernelGGL((linear_f8_big_kernel<OUT, GROUPED>), dim3((unsigned)(tm * tn), 1, (unsigned)z), dim3(256), 163840, st, a, (int)tm, (int)tn);
+  return qbnn_check_launch_msg("qbnn_linear_f8");
+}
+
 // rows: the rows of one sample, or all routed rows
 template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, int rows, int z, hipStream_t st) {
   const int spare = GROUPED ? a.groups : 0;        // each group may end inside a tile
@@ -619,7 +772,7 @@ template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, 
   const bool near = far < ((int64_t)1 << 32) && a.Kb < (1 << 16);
   if (per > 64 && near) {
     if constexpr (!EXACT) {
-      if (per >= 192) return launch_tiled<4, 2, 2, OUT, EXACT, GROUPED>(a, rows, z, st);
+      if (per >= 192) return launch_big<OUT, GROUPED>(a, rows, z, st);
     }
     return launch_tiled<2, 2, 2, OUT, EXACT, GROUPED>(a, rows, z, st);
   }
