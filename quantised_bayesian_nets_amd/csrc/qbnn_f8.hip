@@ -366,116 +366,92 @@ template <int TM, int TN, bool GROUPED> __device__ __forceinline__ bool f8_locat
 }
 
 // Results of a wave's (32 MI) x 128 tile from row m, weight row nw on; `stage`: F8_STAGE bytes of LDS of this wave's own, no longer read by anyone.
-// Lane: activation row r32 of fragment i, weight rows 16 q + 8 h .. + 7 in registers 8 (q & 1) .. + 7 of fragment q / 2.
-// A tile that ends inside its 128 columns goes through `stage` row by row in a short loop: with the bounds in the unrolled code, 30 KiB of it, the instruction
-// fetches of every tile's end took 20 us.
+// A lane's registers hold activation row r32 of fragment i, weight rows 16 q + 8 h .. + 7 in 8 (q & 1) .. + 7 of fragment q / 2: stored from there they are 32 bytes
+// of each of 32 rows per instruction, and with the bounds unrolled 30 KiB of code (27,000 cycles a tile, a tenth of the whole at K = 8192).  So 32 rows at a
+// time go through LDS, and 16 lanes write 128 neighbouring columns of a row.
 constexpr int F8_STAGE = 32 * 132 * 4;
 __device__ __forceinline__ float f8_act(float u, float low) { return u < low ? low : u; }      // (a NaN stays one)
 template <int MI, int OUT, bool GROUPED> __device__ __forceinline__ void f8_finish(const F8Args& a, const F8Tile& t, int m, int nw, f8_v16f (&acc)[MI][4], uint8_t* stage) {
-  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5, n = (lane & 15) * 8;
   if (nw >= a.N) return;
-  const float* bias = a.bias ? a.bias + (int64_t)t.set * a.bias_ss + nw : nullptr;
   const float low = a.relu ? 0.f : -INFINITY;
-  constexpr bool WEIGHED = GROUPED && OUT != QBNN_F8;
-  if (nw + 128 <= a.N) {
-    int64_t to[MI];
-    float s[MI];
-    uint32_t top[MI] = {};
+  const bool whole = nw + n + 8 <= a.N;
+  float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (a.bias) {
+    const float* bias = a.bias + (int64_t)t.set * a.bias_ss + nw;
+    if (whole) __builtin_memcpy(b, bias + n, sizeof(b));
+    else
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int row = m + i * 32 + r32;
-      to[i] = row;
-      s[i] = 1.f;
-      if (WEIGHED && a.y_rows && row < t.m1) { to[i] = a.y_rows[row]; s[i] = a.scale[to[i]]; }
-    }
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int n = q * 16 + h * 8;
-      float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (bias) __builtin_memcpy(b, bias + n, sizeof(b));
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        float v[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          float u = f8_act(acc[i][q >> 1][(q & 1) * 8 + c] + b[c], low);
-          if (WEIGHED) u = s[i] == 0.f ? 0.f : u * s[i];
-          v[c] = u;
-        }
-        if constexpr (OUT == QBNN_F8) {
-          top[i] = max(top[i], f8_max8(v));
-#pragma unroll
-          for (int c = 0; c < 8; ++c) acc[i][q >> 1][(q & 1) * 8 + c] = v[c];
-        } else if (m + i * 32 + r32 < t.m1) {
-          f8_type<OUT> o[8];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) o[c] = f8_store<OUT>(v[c]);
-          __builtin_memcpy((f8_type<OUT>*)a.y + (int64_t)t.sample * a.y_ss + to[i] * a.y_rs + nw + n, o, sizeof(o));
-        }
-      }
-    }
-    if constexpr (OUT == QBNN_F8) {
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const int row = m + i * 32 + r32;
-        const int e = f8_exponent(max(top[i], (uint32_t)__shfl_xor((int)top[i], 32)));
-        const float down = f8_pow2(-e);
-        if (row < t.m1) {
-          uint8_t* y = a.y + (int64_t)t.sample * a.y_ss + (int64_t)row * a.y_rs + nw + h * 8;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            float v[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) v[c] = acc[i][q >> 1][(q & 1) * 8 + c];
-            *(f8_v2i*)(y + q * 16) = f8_scale8(v, down);
-          }
-          if (h == 0) f8_put_exponent(a.ye + ((int64_t)t.sample * a.M + row) * a.ye_rs, nw >> 7, (a.N + 127) >> 7, a.ye_rs, e);
-        }
-      }
-    }
-    return;
+      for (int c = 0; c < 8; ++c) b[c] = nw + n + c < a.N ? bias[n + c] : 0.f;
   }
+  float* st = (float*)stage;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    float* st = (float*)stage;
 #pragma unroll
     for (int q = 0; q < 8; ++q)
 #pragma unroll
-      for (int c = 0; c < 8; c += 4)
-        *(f8_v4f*)(st + r32 * 132 + q * 16 + h * 8 + c) = (f8_v4f){acc[i][q >> 1][(q & 1) * 8 + c], acc[i][q >> 1][(q & 1) * 8 + c + 1], acc[i][q >> 1][(q & 1) * 8 + c + 2], acc[i][q >> 1][(q & 1) * 8 + c + 3]};
-    const int n = lane * 2;                                    // two columns of every row; the wave's own LDS: no barrier
-    const bool in0 = nw + n < a.N, in1 = nw + n + 1 < a.N;
-    const float b0 = bias && in0 ? bias[n] : 0.f, b1 = bias && in1 ? bias[n + 1] : 0.f;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 1
-    for (int r = 0; r < 32; ++r) {
-      const int row = m + i * 32 + r;
-      if (row >= t.m1) break;
-      float u0 = in0 ? f8_act(st[r * 132 + n] + b0, low) : 0.f, u1 = in1 ? f8_act(st[r * 132 + n + 1] + b1, low) : 0.f;
-      if constexpr (OUT == QBNN_F8) {
-        uint32_t top = max(f8_magnitude(u0), f8_magnitude(u1));
+      for (int c = 0; c < 8; c += 4) {
+        const f8_v16f& f = acc[i][q >> 1];
+        const int k = (q & 1) * 8 + c;
+        *(f8_v4f*)(st + r32 * 132 + q * 16 + h * 8 + c) = (f8_v4f){f[k], f[k + 1], f[k + 2], f[k + 3]};
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // (the wave's own LDS: no barrier)
+#pragma unroll 2
+    for (int p = 0; p < 8; ++p) {
+      const int r = p * 4 + (lane >> 4), row = m + i * 32 + r;
+      const f8_v4f lo = *(const f8_v4f*)(st + r * 132 + n), hi = *(const f8_v4f*)(st + r * 132 + n + 4);
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-        const int e = f8_exponent(top);
-        const float down = f8_pow2(-e);
-        *(uint16_t*)(a.y + (int64_t)t.sample * a.y_ss + (int64_t)row * a.y_rs + nw + n) = (uint16_t)f8_pack4(u0 * down, u1 * down, 0.f, 0.f);
-        if (lane == 0) f8_put_exponent(a.ye + ((int64_t)t.sample * a.M + row) * a.ye_rs, nw >> 7, (a.N + 127) >> 7, a.ye_rs, e);
-      } else {
+      for (int c = 0; c < 8; ++c) v[c] = f8_act(v[c] + b[c], low);
+      if constexpr (OUT == QBNN_F8) {
+        if (!whole)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) if (nw + n + c >= a.N) v[c] = 0.f;
+        const int e = f8_exponent(f8_max16(f8_max8(v)));
+        if (row < t.m1) {
+          *(f8_v2i*)(a.y + (int64_t)t.sample * a.y_ss + (int64_t)row * a.y_rs + nw + n) = f8_scale8(v, f8_pow2(-e));
+          if (n == 0) f8_put_exponent(a.ye + ((int64_t)t.sample * a.M + row) * a.ye_rs, nw >> 7, (a.N + 127) >> 7, a.ye_rs, e);
+        }
+      } else if (row < t.m1) {
         int64_t to = row;
-        if (WEIGHED && a.y_rows) {
+        if (GROUPED && a.y_rows) {
           to = a.y_rows[row];
           const float s = a.scale[to];
-          u0 = s == 0.f ? 0.f : u0 * s;
-          u1 = s == 0.f ? 0.f : u1 * s;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[c] = s == 0.f ? 0.f : v[c] * s;
         }
+        f8_type<OUT> o[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) o[c] = f8_store<OUT>(v[c]);
         f8_type<OUT>* y = (f8_type<OUT>*)a.y + (int64_t)t.sample * a.y_ss + to * a.y_rs + nw + n;
-        if (in0) y[0] = f8_store<OUT>(u0);
-        if (in1) y[1] = f8_store<OUT>(u1);
+        if (whole) __builtin_memcpy(y, o, sizeof(o));
+        else
+#pragma unroll
+          for (int c = 0; c < 8; ++c) if (nw + n + c < a.N) y[c] = o[c];
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
+
+// The exponents of 16 steps of a row: four dwords, used from the bottom and moved down two bytes every two steps.  A load's result may only be waited for
+// together with every request issued before it, so they are loaded 16 steps at a time and waited for at once, outside of the loop over the steps.
+struct F8Exponents {
+  uint32_t d[4];
+  __device__ __forceinline__ void load(const uint8_t* row, int kb, int Sp) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = *(const uint32_t*)(row + min(kb + 4 * i, Sp - 4));
+  }
+  __device__ __forceinline__ void arrive() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(d[i]));
+  }
+  __device__ __forceinline__ void down() {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) d[i] = __builtin_amdgcn_alignbit(d[i + 1], d[i], 16);
+    d[3] >>= 16;
+  }
+};
 
 template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED>
 __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const F8Args a, int tiles_m, int tiles_n) {
@@ -514,15 +490,12 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
     for (int p = 0; p < C::PW; ++p) dma16_s(wg + kb * 128, wo[p], at + 2 * C::XB + buf * C::WB + p * (C::WAVES * 1024));
   };
 
-  // exponents: dwords of four blocks
   const uint8_t* xeg = a.xe + (int64_t)t.sample * a.xe_ss;
   uint32_t xeo[MI];
 #pragma unroll
   for (int i = 0; i < MI; ++i) xeo[i] = (uint32_t)f8_x_row<GROUPED>(a, min(t.m0 + (wm * MI + i) * 32 + r32, t.m1 - 1)) * (uint32_t)a.Sp;
-  const uint32_t* we = (const uint32_t*)(a.we + (int64_t)t.set * a.we_ss + (int64_t)min((n0 >> 7) + wn, (a.N - 1) >> 7) * a.Sp);
-  uint32_t xs[MI], xn[MI], ws = we[0], wnx = ws;
-#pragma unroll
-  for (int i = 0; i < MI; ++i) xs[i] = xn[i] = *(const uint32_t*)(xeg + xeo[i]);
+  const uint8_t* we = a.we + (int64_t)t.set * a.we_ss + (int64_t)min((n0 >> 7) + wn, (a.N - 1) >> 7) * a.Sp;
+  F8Exponents xs[MI], ws;
 
   // a fragment of 32 rows x 128 columns: instruction s = 0, 1 of the two takes pieces 4 s + h and 4 s + 2 + h
   struct Frag { f8_v8i k[2]; };
@@ -565,7 +538,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
       constexpr int B = decltype(Bc)::value;
       constexpr int X0 = MI & 1 ? B : 0;      // registers of the step's first activation fragment
       auto mfma = [&](int i, int j, int s) {
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j].k[s], xf[(i + X0) & 1].k[s], acc[i][j], 0, 0, B, (int)ws, B, (int)xs[i]);
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j].k[s], xf[(i + X0) & 1].k[s], acc[i][j], 0, 0, B, (int)ws.d[0], B, (int)xs[i].d[0]);
       };
 #pragma unroll
       for (int i = 0; i < MI - 1; ++i) {
@@ -576,12 +549,6 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
       }
       wait_vmcnt<0>();
       lds_barrier();
-      if constexpr (B == 0) {
-        const int at = min(kb + 2, last) >> 2;
-#pragma unroll
-        for (int i = 0; i < MI; ++i) xn[i] = *(const uint32_t*)(xeg + xeo[i] + at * 4);
-        wnx = we[at];
-      }
       xf[(MI + X0) & 1] = read_x(B ^ 1, 0);
       request(min(kb + 2, last), B);
       __builtin_amdgcn_sched_barrier(0);
@@ -594,24 +561,36 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    int kb = 0;
-    for (; kb < last; kb += 2) {
-      step(std::integral_constant<int, 0>{}, kb);
-      step(std::integral_constant<int, 1>{}, kb + 1);
-      const int by = ((kb + 2) & 2) * 8;
+    for (int k0 = 0; k0 < a.Kb; k0 += 16) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i) xs[i] = xn[i] >> by;
-      ws = wnx >> by;
+      for (int i = 0; i < MI; ++i) xs[i].load(xeg + xeo[i], k0, a.Sp);
+      ws.load(we, k0, a.Sp);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) xs[i].arrive();
+      ws.arrive();
+      const int end = min(k0 + 16, a.Kb);
+      int kb = k0;
+      for (; kb + 1 < end; kb += 2) {
+        step(std::integral_constant<int, 0>{}, kb);
+        step(std::integral_constant<int, 1>{}, kb + 1);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) xs[i].down();
+        ws.down();
+      }
+      if (kb < end) step(std::integral_constant<int, 0>{}, kb);
     }
-    if (kb == last) step(std::integral_constant<int, 0>{}, kb);
   } else {
     for (int kb = 0; kb < a.Kb; ++kb) {
       const int buf = kb & 1;
-      if ((kb & 3) == 0) {
+      if ((kb & 15) == 0) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i) xs[i] = *(const uint32_t*)(xeg + xeo[i] + kb);
-        ws = we[kb >> 2];
+        for (int i = 0; i < MI; ++i) xs[i].load(xeg + xeo[i], kb, a.Sp);
+        ws.load(we, kb, a.Sp);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) xs[i].arrive();
+        ws.arrive();
       }
+      const int byte = (kb & 1) * 8;
       F8Wide xw[MI][2];
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
@@ -632,14 +611,16 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
           for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int g = 0; g < 4; ++g) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ww[s].part[g], xw[i][s].part[g], c, 0, 0, 0);
-          const int e = (int)(ws & 255) + (int)(xs[i] & 255) - 254;
+          const int e = (int)((ws.d[0] >> byte) & 255) + (int)((xs[i].d[0] >> byte) & 255) - 254;
 #pragma unroll
           for (int k = 0; k < 16; ++k) acc[i][j][k] += __builtin_ldexpf(c[k], e);
         }
       }
+      if (kb & 1) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i) xs[i] >>= 8;
-      ws >>= 8;
+        for (int i = 0; i < MI; ++i) xs[i].down();
+        ws.down();
+      }
       wait_vmcnt<0>();
       lds_barrier();
       request(min(kb + 2, last), buf);
@@ -696,14 +677,11 @@ __global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, i
   auto after = [](int slot, int by) { slot += by * SLOT; return slot >= SLOTS * SLOT ? slot - SLOTS * SLOT : slot; };
 
   const uint8_t* xeg = a.xe + (int64_t)t.sample * a.xe_ss;
-  uint32_t xeo[4], xs[4], xn[4];
+  uint32_t xeo[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    xeo[i] = (uint32_t)f8_x_row<GROUPED>(a, min(t.m0 + (wm * 4 + i) * 32 + r32, t.m1 - 1)) * (uint32_t)a.Sp;
-    xs[i] = xn[i] = *(const uint32_t*)(xeg + xeo[i]);
-  }
-  const uint32_t* we = (const uint32_t*)(a.we + (int64_t)t.set * a.we_ss + (int64_t)min((n0 >> 7) + wn, (a.N - 1) >> 7) * a.Sp);
-  uint32_t ws = we[0], wnx = ws;
+  for (int i = 0; i < 4; ++i) xeo[i] = (uint32_t)f8_x_row<GROUPED>(a, min(t.m0 + (wm * 4 + i) * 32 + r32, t.m1 - 1)) * (uint32_t)a.Sp;
+  const uint8_t* we = a.we + (int64_t)t.set * a.we_ss + (int64_t)min((n0 >> 7) + wn, (a.N - 1) >> 7) * a.Sp;
+  F8Exponents xs[4], ws;
 
   struct Frag { f8_v8i k[2]; };
   const int xl = wm * 16384 + r32 * 128 + ((h ^ ((r32 >> 1) & 7)) << 4);
@@ -741,17 +719,11 @@ __global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, i
   auto step = [&](auto Bc, int kb) {
     constexpr int B = decltype(Bc)::value;
     auto mfma = [&](int i, int j, int s) {
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[B][j].k[s], xf[i].k[s], acc[i][j], 0, 0, B, (int)ws, B, (int)xs[i]);
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[B][j].k[s], xf[i].k[s], acc[i][j], 0, 0, B, (int)ws.d[0], B, (int)xs[i].d[0]);
     };
     const int sx = after(slot, 1), sw1 = after(slot, 2), sx1 = after(slot, 3);
     wait_vmcnt<16>();                        // the next step's w has landed (its x and the w after it may be in flight)
     lds_barrier();
-    if constexpr (B == 0) {
-      const int at = min(kb + 2, last) >> 2;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xn[i] = *(const uint32_t*)(xeg + xeo[i] + at * 4);
-      wnx = we[at];
-    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int g = 0; g < 8; ++g) {            // two instructions, two reads, one request
@@ -776,16 +748,24 @@ __global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, i
     }
     slot = sw1;
   };
-  int kb = 0;
-  for (; kb < last; kb += 2) {
-    step(std::integral_constant<int, 0>{}, kb);
-    step(std::integral_constant<int, 1>{}, kb + 1);
-    const int by = ((kb + 2) & 2) * 8;
+  for (int k0 = 0; k0 < a.Kb; k0 += 16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) xs[i] = xn[i] >> by;
-    ws = wnx >> by;
+    for (int i = 0; i < 4; ++i) xs[i].load(xeg + xeo[i], k0, a.Sp);
+    ws.load(we, k0, a.Sp);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xs[i].arrive();
+    ws.arrive();
+    const int end = min(k0 + 16, a.Kb);
+    int kb = k0;
+    for (; kb + 1 < end; kb += 2) {
+      step(std::integral_constant<int, 0>{}, kb);
+      step(std::integral_constant<int, 1>{}, kb + 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xs[i].down();
+      ws.down();
+    }
+    if (kb < end) step(std::integral_constant<int, 0>{}, kb);
   }
-  if (kb == last) step(std::integral_constant<int, 0>{}, kb);
   wait_vmcnt<0>();          // (no request outlives the workgroup's LDS)
   lds_barrier();            // ... and no wave reads another's operands any more
   f8_finish<4, OUT, GROUPED>(a, t, t.m0 + wm * 128, n0 + wn * 128, acc, lds + wave * F8_STAGE);

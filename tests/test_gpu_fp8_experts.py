@@ -107,7 +107,7 @@ def linear_case(seed, S, sx, sw, B, N, K, dtype, bias, relu, out=None):
 
 
 SIZES = [(1, 1, 1), (1, 16, 128), (2, 130, 100), (5, 257, 1000), (16, 96, 384), (17, 128, 256), (33, 129, 127), (64, 64, 640), (65, 1, 513), (100, 500, 800), (128, 256, 512),
-         (129, 384, 1024), (255, 300, 129), (256, 256, 256), (300, 520, 2048), (513, 777, 1111)]
+         (129, 384, 1024), (255, 300, 129), (256, 256, 256), (300, 520, 2048), (513, 777, 1111), (200, 140, 2176), (260, 256, 2049), (70, 130, 4100)]
 
 
 @pytest.mark.parametrize("dtype,out", [(torch.bfloat16, None), (torch.float32, None), (torch.float16, None), (torch.bfloat16, torch.float32), (torch.float32, torch.float16)])
