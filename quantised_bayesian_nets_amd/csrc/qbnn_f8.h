@@ -42,6 +42,17 @@ template <int T> __device__ __forceinline__ f8_type<T> f8_store(float v) {
   } else return (f8_type<T>)v;
 }
 
+template <int T> __device__ __forceinline__ int f8_store2(float a, float b) {      // two 16-bit results in a dword
+  if constexpr (T == QBNN_BF16) {
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(int, __builtin_convertvector((f2){a, b}, v2));
+  } else {
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(int, (v2){(_Float16)a, (_Float16)b});
+  }
+}
+
 // ---- block scale ---------------------------------------------------------------------------------------------------------------
 // bits of the largest finite magnitude -> unbiased exponent: the smallest e >= -126 with a <= 448 2^e = 1.75 2^(e + 8); 0 for a = 0
 __device__ __forceinline__ int f8_exponent(uint32_t bits) {
@@ -100,6 +111,20 @@ __device__ __forceinline__ f8_v4f f8_mfma_exact(const F8Wide& w, const F8Wide& x
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i] += __builtin_ldexpf(c[i], n);
   return acc;
+}
+
+// 16 bytes per lane from a uniform address + a 32-bit offset per lane to LDS at lds_addr + 16 * lane; counted by the caller (wait_vmcnt).  m0 is given up, not kept
+// as dma16_s does: two scalar instructions fewer in a gap of 32 cycles.
+__device__ __forceinline__ void f8_dma16(const uint8_t* base, uint32_t lane_off, uint32_t lds_addr) {
+  const uint64_t g = (uint64_t)base;
+  const uint64_t gs = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(g >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)g);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane_off), "s"(gs), "s"(lds_addr) : "memory", "m0");
+}
+
+__device__ __forceinline__ void f8_dma4(const uint8_t* base, uint32_t lane_off, uint32_t lds_addr) {      // 4 bytes per lane
+  const uint64_t g = (uint64_t)base;
+  const uint64_t gs = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(g >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)g);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(lane_off), "s"(gs), "s"(lds_addr) : "memory", "m0");
 }
 
 __device__ __forceinline__ f8_v8i f8_join(f8_v4i lo, f8_v4i hi) { return (f8_v8i){lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}; }

@@ -341,15 +341,11 @@ template <int MT, int NT, int NW, int OUT, bool EXACT, bool GROUPED> int launch_
 // its accumulators are tied in place (the 16 x 16 form's are renamed, which cost 3 register moves per instruction here) and it reads half the operand registers.
 // One barrier per step, in front of the last activation fragment's products: before it the wave waits for its share of the next step's bytes; behind it
 // the buffer just read is requested again and the next step's first fragments are read, each weight fragment's registers as soon as their products are issued.
-// Weight fragment j holds rows 32 j + 16 (r / 16) + 8 ((r / 4) & 1) + 4 ((r / 8) & 1) + r % 4 (r = 0 .. 31) of the wave's 128, so that a lane ends up with runs of 8
-// neighbouring results of a row and a pair of lanes with 16: whole sectors per store.
 template <int MI, int WM, int WN> struct F8Tiled {
   static constexpr int TM = 32 * MI * WM, TN = 128 * WN, WAVES = WM * WN, XB = TM * 128, WB = TN * 128, LDS = 2 * (XB + WB);
   static constexpr int PX = TM / 8 / WAVES, PW = TN / 8 / WAVES;      // DMA requests (8 rows each) per wave and step
   static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && LDS <= 160 * 1024 && 2 * XB <= 65536 && 2 * WB <= 65536, "immediate offsets of the reads");
 };
-// f of weight row r: of the fragment row that reads it (below) bits 1, 2, 3
-__device__ __forceinline__ int f8_swizzle_w(int r) { return ((r >> 1) & 1) | ((r >> 2) & 2) | (r & 4); }
 typedef float f8_v16f __attribute__((ext_vector_type(16)));
 
 // Workgroups of one XCD (every eighth) take neighbouring tiles, in columns of 4 row tiles: what they read at a time shares its L2.  false: no tile.
@@ -365,73 +361,79 @@ template <int TM, int TN, bool GROUPED> __device__ __forceinline__ bool f8_locat
   return f8_find_tile<TM, GROUPED>(a, band * 4 + in - col * rows, blockIdx.z, t);
 }
 
-// Results of a wave's (32 MI) x 128 tile from row m, weight row nw on; `stage`: F8_STAGE bytes of LDS of this wave's own, no longer read by anyone.
-// A lane's registers hold activation row r32 of fragment i, weight rows 16 q + 8 h .. + 7 in 8 (q & 1) .. + 7 of fragment q / 2: stored from there they are 32 bytes
-// of each of 32 rows per instruction, and with the bounds unrolled 30 KiB of code (27,000 cycles a tile, a tenth of the whole at K = 8192).  So 32 rows at a
-// time go through LDS, and 16 lanes write 128 neighbouring columns of a row.
-constexpr int F8_STAGE = 32 * 132 * 4;
-__device__ __forceinline__ float f8_act(float u, float low) { return u < low ? low : u; }      // (a NaN stays one)
-template <int MI, int OUT, bool GROUPED> __device__ __forceinline__ void f8_finish(const F8Args& a, const F8Tile& t, int m, int nw, f8_v16f (&acc)[MI][4], uint8_t* stage) {
-  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5, n = (lane & 15) * 8;
-  if (nw >= a.N) return;
-  const float low = a.relu ? 0.f : -INFINITY;
-  const bool whole = nw + n + 8 <= a.N;
+// Results of a wave's (32 G) x 128 tile from row m, weight row nw on, 32 rows at a time through `stage` (F8_STAGE bytes of LDS of this wave's own, no longer read
+// by anyone; put(i, st) writes rows 32 i .. + 31 there, F8_PITCH floats each): 16 lanes then write 128 neighbouring columns of a row.  Stored from the
+// accumulators' layout they were 32 bytes of each of 32 rows per instruction, and with the bounds unrolled 30 KiB of code: 27,000 cycles a tile, as much as 11 steps.
+constexpr int F8_PITCH = 132, F8_STAGE = 32 * F8_PITCH * 4;
+__device__ __forceinline__ float f8_relu(float u) { return u < 0.f ? 0.f : u; }      // (a NaN stays one)
+template <int G, int OUT, bool GROUPED, bool WHOLE, class Put>
+__device__ __forceinline__ void f8_finish_as(const F8Args& a, const F8Tile& t, int m, int nw, uint8_t* stage, Put put) {
+  const int lane = threadIdx.x & 63, n = (lane & 15) * 8;
+  const int in = WHOLE ? 8 : a.N - nw - n;                      // columns of this lane that exist
   float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (a.bias) {
-    const float* bias = a.bias + (int64_t)t.set * a.bias_ss + nw;
-    if (whole) __builtin_memcpy(b, bias + n, sizeof(b));
+    const float* bias = a.bias + (int64_t)t.set * a.bias_ss + nw + n;
+    if constexpr (WHOLE) __builtin_memcpy(b, bias, sizeof(b));
     else
 #pragma unroll
-      for (int c = 0; c < 8; ++c) b[c] = nw + n + c < a.N ? bias[n + c] : 0.f;
+      for (int c = 0; c < 8; ++c) b[c] = c < in ? bias[c] : 0.f;
   }
   float* st = (float*)stage;
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-#pragma unroll
-      for (int c = 0; c < 8; c += 4) {
-        const f8_v16f& f = acc[i][q >> 1];
-        const int k = (q & 1) * 8 + c;
-        *(f8_v4f*)(st + r32 * 132 + q * 16 + h * 8 + c) = (f8_v4f){f[k], f[k + 1], f[k + 2], f[k + 3]};
-      }
+  for (int i = 0; i < G; ++i) {
+    put(i, st);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // (the wave's own LDS: no barrier)
-#pragma unroll 2
-    for (int p = 0; p < 8; ++p) {
-      const int r = p * 4 + (lane >> 4), row = m + i * 32 + r;
-      const f8_v4f lo = *(const f8_v4f*)(st + r * 132 + n), hi = *(const f8_v4f*)(st + r * 132 + n + 4);
-      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    constexpr int AT_ONCE = WHOLE ? 4 : 1;
+#pragma unroll 1
+    for (int p0 = 0; p0 < 8; p0 += AT_ONCE)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) v[c] = f8_act(v[c] + b[c], low);
-      if constexpr (OUT == QBNN_F8) {
-        if (!whole)
+      for (int p1 = 0; p1 < AT_ONCE; ++p1) {
+        const int r = (p0 + p1) * 4 + (lane >> 4), row = m + i * 32 + r;
+        const f8_v4f lo = *(const f8_v4f*)(st + r * F8_PITCH + n), hi = *(const f8_v4f*)(st + r * F8_PITCH + n + 4);
+        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
-          for (int c = 0; c < 8; ++c) if (nw + n + c >= a.N) v[c] = 0.f;
-        const int e = f8_exponent(f8_max16(f8_max8(v)));
-        if (row < t.m1) {
-          *(f8_v2i*)(a.y + (int64_t)t.sample * a.y_ss + (int64_t)row * a.y_rs + nw + n) = f8_scale8(v, f8_pow2(-e));
-          if (n == 0) f8_put_exponent(a.ye + ((int64_t)t.sample * a.M + row) * a.ye_rs, nw >> 7, (a.N + 127) >> 7, a.ye_rs, e);
+        for (int c = 0; c < 8; ++c) v[c] += b[c];
+        if (a.relu) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[c] = f8_relu(v[c]);
         }
-      } else if (row < t.m1) {
-        int64_t to = row;
-        if (GROUPED && a.y_rows) {
-          to = a.y_rows[row];
-          const float s = a.scale[to];
+        if constexpr (OUT == QBNN_F8) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) v[c] = s == 0.f ? 0.f : v[c] * s;
+          for (int c = 0; c < 8; ++c) if (!WHOLE && c >= in) v[c] = 0.f;
+          const int e = f8_exponent(f8_max16(f8_max8(v)));
+          if (row < t.m1) {
+            *(f8_v2i*)(a.y + (int64_t)t.sample * a.y_ss + (int64_t)row * a.y_rs + nw + n) = f8_scale8(v, f8_pow2(-e));
+            if (n == 0) f8_put_exponent(a.ye + ((int64_t)t.sample * a.M + row) * a.ye_rs, nw >> 7, (a.N + 127) >> 7, a.ye_rs, e);
+          }
+        } else if (row < t.m1) {
+          int64_t to = row;
+          if (GROUPED && a.y_rows) {
+            to = a.y_rows[row];
+            const float s = a.scale[to];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] = s == 0.f ? 0.f : v[c] * s;
+          }
+          f8_type<OUT>* y = (f8_type<OUT>*)a.y + (int64_t)t.sample * a.y_ss + to * a.y_rs + nw + n;
+          if constexpr (!WHOLE) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) if (c < in) y[c] = f8_store<OUT>(v[c]);
+          } else if constexpr (OUT == QBNN_F32) {
+            __builtin_memcpy(y, v, sizeof(v));
+          } else {
+            f8_v4i o;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[c] = f8_store2<OUT>(v[2 * c], v[2 * c + 1]);
+            __builtin_memcpy(y, &o, sizeof(o));
+          }
         }
-        f8_type<OUT> o[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) o[c] = f8_store<OUT>(v[c]);
-        f8_type<OUT>* y = (f8_type<OUT>*)a.y + (int64_t)t.sample * a.y_ss + to * a.y_rs + nw + n;
-        if (whole) __builtin_memcpy(y, o, sizeof(o));
-        else
-#pragma unroll
-          for (int c = 0; c < 8; ++c) if (nw + n + c < a.N) y[c] = o[c];
       }
-    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
+}
+template <int G, int OUT, bool GROUPED, class Put> __device__ __forceinline__ void f8_finish(const F8Args& a, const F8Tile& t, int m, int nw, uint8_t* stage, Put put) {
+  if (nw >= a.N || m >= t.m1) return;
+  if (nw + 128 <= a.N) f8_finish_as<G, OUT, GROUPED, true>(a, t, m, nw, stage, put);
+  else f8_finish_as<G, OUT, GROUPED, false>(a, t, m, nw, stage, put);
 }
 
 // The exponents of 16 steps of a row: four dwords, used from the bottom and moved down two bytes every two steps.  A load's result may only be waited for
@@ -479,15 +481,15 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
 #pragma unroll
   for (int p = 0; p < C::PW; ++p) {
     const int r = (p * C::WAVES + wave) * 8 + (lane >> 3);
-    wo[p] = (uint32_t)(min(r, a.N - 1 - n0) * pitch) + (((lane & 7) ^ f8_swizzle_w(r)) << 4);
+    wo[p] = (uint32_t)(min(r, a.N - 1 - n0) * pitch) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
   }
   const uint32_t lds0 = lds_addr_of(lds);
   auto request = [&](int kb, int buf) {
     const uint32_t at = lds0 + wave * 1024;
 #pragma unroll
-    for (int p = 0; p < C::PX; ++p) dma16_s(xg + kb * 128, xo[p], at + buf * C::XB + p * (C::WAVES * 1024));
+    for (int p = 0; p < C::PX; ++p) f8_dma16(xg + kb * 128, xo[p], at + buf * C::XB + p * (C::WAVES * 1024));
 #pragma unroll
-    for (int p = 0; p < C::PW; ++p) dma16_s(wg + kb * 128, wo[p], at + 2 * C::XB + buf * C::WB + p * (C::WAVES * 1024));
+    for (int p = 0; p < C::PW; ++p) f8_dma16(wg + kb * 128, wo[p], at + 2 * C::XB + buf * C::WB + p * (C::WAVES * 1024));
   };
 
   const uint8_t* xeg = a.xe + (int64_t)t.sample * a.xe_ss;
@@ -500,7 +502,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
   // a fragment of 32 rows x 128 columns: instruction s = 0, 1 of the two takes pieces 4 s + h and 4 s + 2 + h
   struct Frag { f8_v8i k[2]; };
   const uint8_t* xl = lds + wm * MI * 4096 + r32 * 128;
-  const uint8_t* wl = lds + 2 * C::XB + wn * 16384 + ((r32 >> 4) * 16 + ((r32 >> 2) & 1) * 8 + ((r32 >> 3) & 1) * 4 + (r32 & 3)) * 128;
+  const uint8_t* wl = lds + 2 * C::XB + wn * 16384 + r32 * 128;
   const int piece = (h ^ ((r32 >> 1) & 7)) << 4;
   const uint8_t *x0 = xl + piece, *x1 = xl + (piece ^ 32), *x2 = xl + (piece ^ 64), *x3 = xl + (piece ^ 96);
   const uint8_t *w0 = wl + piece, *w1 = wl + (piece ^ 32), *w2 = wl + (piece ^ 64), *w3 = wl + (piece ^ 96);
@@ -629,7 +631,14 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
   wait_vmcnt<0>();          // (no request outlives the workgroup's LDS)
 
   lds_barrier();            // ... and no wave reads another's operands any more
-  f8_finish<MI, OUT, GROUPED>(a, t, t.m0 + wm * MI * 32, n0 + wn * 128, acc, lds + wave * F8_STAGE);
+  // lane: activation row r32 of fragment i, weight rows 8 q + 4 h .. + 3 of fragment j in registers 4 q .. + 3
+  f8_finish<MI, OUT, GROUPED>(a, t, t.m0 + wm * MI * 32, n0 + wn * 128, lds + wave * F8_STAGE, [&](int i, float* st) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *(f8_v4f*)(st + r32 * F8_PITCH + j * 32 + q * 8 + h * 4) = (f8_v4f){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+  });
 }
 
 template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED> int launch_tiled(const F8Args& a, int rows, int z, hipStream_t st) {
@@ -643,17 +652,29 @@ template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED> int launch_
   return qbnn_check_launch_msg("qbnn_linear_f8");
 }
 
-// The largest tile, 256 x 256: the tiled form's data paths with a deeper ring.  A step's two operands are 32 KiB each and take turns in five slots, so that
-// three requests (96 KiB) are in flight, each for three half steps (3072 matrix cycles): with the two buffers of the form above the wait for a request one
-// step old was a quarter of the time.  A step has two halves of 16 instructions, a barrier in front of each:
-//   first   x0, x1 times w;  reads x2, x3 and the next step's w0, w1      frees the slot of this step's w, needs the next step's w
-//   second  x2, x3 times w;  reads the next step's w2, w3, x0, x1         frees the slot of this step's x, needs the next step's x
-// so that every fragment is read half a step before it is used and 16 reads go with 16 instructions.
+// The largest tile, 256 x 256, 4 waves of 128 x 128, two steps of operands (64 KiB each) in LDS.  What the wave issues between two matrix instructions has 32 cycles,
+// so requests and reads go one by one behind one instruction each (eight requests in a row held the wave at the address unit for longer than the
+// matrix unit had work: 528 -> 476 us at 8192^3), and the loop holds nothing that waits for memory but the barrier that hands over a step:
+//   first half   x0 .. x3 times w; reads x4 .. x7; then everything of this step is in registers: barrier, its buffer is requested for the step after the next
+//   second half  wait for the next step, barrier; x4 .. x7 times w; reads the next step's x0 .. x3 and w, each fragment into its registers behind its last product
+// The exponents come the same way, a dword (four steps) of each row every two steps: as loads into registers they were waited for together with every
+// request issued before them, which emptied the ring.
+// At this rate the card is bound by power (1.6 - 1.9 GHz on normal data), and the 16 x 16 x 128 form draws less of it than 32 x 32 x 64 (alone: 4,080 against
+// 3,500 TFLOP/s).  The compiler gives its result other registers than its addend, for which 256 accumulators leave none; so the instruction is written
+// out, in place.  An accumulator is read again 32 instructions later or behind the wait at the end, which is what its hazards ask for.
+template <int B> __device__ __forceinline__ void f8_mfma_in_place(f8_v4f& acc, const f8_v8i& w, const f8_v8i& x, uint32_t ws, uint32_t xs) {      // exponents: byte B
+  static_assert(B == 0 || B == 1, "");
+  if constexpr (B == 0) asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs));
+  else asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs));
+}
+
+constexpr int F8_BIG_LDS = 131072 + 2 * 2048;      // two steps of x and w, two sets of exponents (1 KiB of x, 256 bytes for each wave of w)
+
 template <int OUT, bool GROUPED>
 __global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, int tiles_m, int tiles_n) {
-  constexpr int SLOT = 32768, SLOTS = 5;
+  constexpr int W0 = 65536, E0 = 131072;             // x at 0 and 32768, w at W0 and W0 + 32768, exponents at E0 and E0 + 2048
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, h = lane >> 4;
   const int wm = wave >> 1, wn = wave & 1;
   F8Tile t;
   int n0;
@@ -665,118 +686,119 @@ __global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, i
   uint32_t xo[8], wo[8];
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
-    const int r = (p * 4 + wave) * 8 + (lane >> 3), i = min(t.m0 + r, t.m1 - 1);
-    xo[p] = (uint32_t)((GROUPED ? f8_x_row<GROUPED>(a, i) : i - t.m0) * pitch) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
-    wo[p] = (uint32_t)(min(r, a.N - 1 - n0) * pitch) + (((lane & 7) ^ f8_swizzle_w(r)) << 4);
+    const int r = (p * 4 + wave) * 8 + (lane >> 3), i = min(t.m0 + r, t.m1 - 1), piece = ((lane & 7) ^ ((r >> 1) & 7)) << 4;
+    xo[p] = (uint32_t)((GROUPED ? f8_x_row<GROUPED>(a, i) : i - t.m0) * pitch) + piece;
+    wo[p] = (uint32_t)(min(r, a.N - 1 - n0) * pitch) + piece;
   }
-  const uint32_t lds0 = lds_addr_of(lds) + wave * 1024;
-  const int last = a.Kb - 1;
-  // requests past the last step repeat its bytes, into slots that are not read again (no branch in the loop)
-  auto request_x = [&](int kb, int slot, int p) { dma16_s(xg + min(kb, last) * 128, xo[p], lds0 + slot + p * 4096); };
-  auto request_w = [&](int kb, int slot, int p) { dma16_s(wg + min(kb, last) * 128, wo[p], lds0 + slot + p * 4096); };
-  auto after = [](int slot, int by) { slot += by * SLOT; return slot >= SLOTS * SLOT ? slot - SLOTS * SLOT : slot; };
-
   const uint8_t* xeg = a.xe + (int64_t)t.sample * a.xe_ss;
-  uint32_t xeo[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) xeo[i] = (uint32_t)f8_x_row<GROUPED>(a, min(t.m0 + (wm * 4 + i) * 32 + r32, t.m1 - 1)) * (uint32_t)a.Sp;
-  const uint8_t* we = a.we + (int64_t)t.set * a.we_ss + (int64_t)min((n0 >> 7) + wn, (a.N - 1) >> 7) * a.Sp;
-  F8Exponents xs[4], ws;
-
-  struct Frag { f8_v8i k[2]; };
-  const int xl = wm * 16384 + r32 * 128 + ((h ^ ((r32 >> 1) & 7)) << 4);
-  const int wl = wn * 16384 + ((r32 >> 4) * 16 + ((r32 >> 2) & 1) * 8 + ((r32 >> 3) & 1) * 4 + (r32 & 3)) * 128 + ((h ^ ((r32 >> 1) & 7)) << 4);
-  // fragment f at base: instruction s = 0, 1 of the two takes pieces 4 s + h and 4 s + 2 + h
-  auto read_half = [&](Frag& o, int base, int f, int s) {
-    const uint8_t* p = lds + f * 4096;
-    o.k[s] = f8_join(*(const f8_v4i*)(p + (base ^ (64 * s))), *(const f8_v4i*)(p + (base ^ (64 * s + 32))));
+  const uint8_t* weg = a.we + (int64_t)t.set * a.we_ss + (int64_t)min((n0 >> 7) + wn, (a.N - 1) >> 7) * a.Sp;
+  const uint32_t xeo = (uint32_t)f8_x_row<GROUPED>(a, min(t.m0 + (int)threadIdx.x, t.m1 - 1)) * (uint32_t)a.Sp;      // of row threadIdx.x
+  const uint32_t lds0 = lds_addr_of(lds) + wave * 1024, ldse = lds_addr_of(lds) + E0 + wave * 256;
+  const int last = a.Kb - 1;
+  // requests past the last step repeat its bytes, into buffers that are not read again (no branch in the loop)
+  auto request = [&](int kb, int buf, int p) {       // 16 of a step
+    const int at = min(kb, last) * 128;
+    if (p < 8) f8_dma16(xg + at, xo[p], lds0 + buf * 32768 + p * 4096);
+    else f8_dma16(wg + at, wo[p - 8], lds0 + W0 + buf * 32768 + (p - 8) * 4096);
   };
-  auto read = [&](Frag& o, int base, int f) { read_half(o, base, f, 0); read_half(o, base, f, 1); };
-  f8_v16f acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int c = 0; c < 16; ++c) acc[i][j][c] = 0.f;
+  auto request_exponents = [&](int kb, int set) {    // of step kb (a multiple of 2) and the next
+    const int at = min(kb, last) & ~3;
+    f8_dma4(xeg + at, xeo, ldse + set * 2048);
+    f8_dma4(weg + at, 0, ldse + set * 2048 + 1024);
+  };
 
-  // slots in the order of the requests: w0 x0 w1 x1 w2
+  const int fl = r16 * 128 + ((h ^ ((r16 >> 1) & 7)) << 4);
+  const uint8_t *xl = lds + wm * 16384 + fl, *xh = lds + wm * 16384 + (fl ^ 64), *wl = lds + W0 + wn * 16384 + fl, *wh = lds + W0 + wn * 16384 + (fl ^ 64);
+  auto half = [](f8_v8i& o, int s, const uint8_t* p) {      // a fragment: pieces h and 4 + h of its rows
+    const f8_v4i v = *(const f8_v4i*)p;
 #pragma unroll
-  for (int k = 0; k < 5; ++k)
+    for (int c = 0; c < 4; ++c) o[4 * s + c] = v[c];
+  };
+  f8_v8i wf[8], xf[8];
+  auto read_x = [&](int buf, int f, int s) { half(xf[f], s, (s ? xh : xl) + buf * 32768 + f * 2048); };
+  auto read_w = [&](int buf, int f, int s) { half(wf[f], s, (s ? wh : wl) + buf * 32768 + f * 2048); };
+  uint32_t xs[8], ws;
+  const uint8_t *xel = lds + E0 + (wm * 128 + r16) * 4, *wel = lds + E0 + 1024 + wave * 256 + lane * 4;
+  auto read_exponents = [&](int set, int by) {
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-      if (k & 1) request_x(k >> 1, k * SLOT, p);
-      else request_w(k >> 1, k * SLOT, p);
-    }
-  wait_vmcnt<24>();
+    for (int i = 0; i < 8; ++i) xs[i] = *(const uint32_t*)(xel + set * 2048 + i * 64) >> by;
+    ws = *(const uint32_t*)(wel + set * 2048) >> by;
+  };
+  f8_v4f acc[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = (f8_v4f){0.f, 0.f, 0.f, 0.f};
+
+  request_exponents(0, 0);
+#pragma unroll
+  for (int p = 0; p < 16; ++p) request(0, 0, p);
+#pragma unroll
+  for (int p = 0; p < 16; ++p) request(1, 1, p);
+  wait_vmcnt<16>();
   lds_barrier();
-  Frag wf[2][4], xf[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) read(wf[0][j], wl, j);
-  read(xf[0], xl + SLOT, 0);
-  read(xf[1], xl + SLOT, 1);
-  int slot = 0;                              // of this step's w; x lies one, the next step's w two, its x three further on
-  auto step = [&](auto Bc, int kb) {
+  for (int f = 0; f < 8; ++f) { read_w(0, f, 0); read_w(0, f, 1); }
+#pragma unroll
+  for (int f = 0; f < 4; ++f) { read_x(0, f, 0); read_x(0, f, 1); }
+  read_exponents(0, 0);
+  // even and odd steps differ in the buffer and in the byte of xs / ws; the even one requests the next two steps' exponents, into set `set`
+  auto step = [&](auto Bc, int kb, int set) {
     constexpr int B = decltype(Bc)::value;
-    auto mfma = [&](int i, int j, int s) {
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[B][j].k[s], xf[i].k[s], acc[i][j], 0, 0, B, (int)ws.d[0], B, (int)xs[i].d[0]);
-    };
-    const int sx = after(slot, 1), sw1 = after(slot, 2), sx1 = after(slot, 3);
-    wait_vmcnt<16>();                        // the next step's w has landed (its x and the w after it may be in flight)
-    lds_barrier();
-    __builtin_amdgcn_sched_barrier(0);
+    auto mfma = [&](int i, int j) { f8_mfma_in_place<B>(acc[i][j], wf[j], xf[i], ws, xs[i]); };
+    asm volatile("s_nop 3" : "+v"(ws), "+v"(xs[0]), "+a"(acc[0][0]));      // behind the vector unit's last writes of what the first instructions read
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {            // two instructions, two reads, one request
-      request_x(kb + 2, slot, g);
-      if (g < 4) read_half(xf[2 + (g >> 1)], xl + sx, 2 + (g >> 1), g & 1);
-      else read_half(wf[B ^ 1][(g >> 1) - 2], wl + sw1, (g >> 1) - 2, g & 1);
-      mfma((g >> 1) & 1, (g >> 2) * 2, g & 1);
-      mfma((g >> 1) & 1, (g >> 2) * 2 + 1, g & 1);
+    for (int u = 0; u < 32; ++u) {
+      if (u == 12) lds_barrier();            // the reads above are back
+      mfma(u >> 3, u & 7);
+      if (u < 8) read_x(B, 4 + (u >> 1), u & 1);
+      if (u >= 12 && u % 2 == 1) request(kb + 2, B, (u - 13) / 2);
+      if (u == 31 && B == 0) request_exponents(kb + 2, set);
       __builtin_amdgcn_sched_barrier(0);
     }
-    wait_vmcnt<16>();                        // the next step's x has landed (the two requests after it may be in flight)
+    wait_vmcnt<B == 0 ? 12 : 10>();          // the next step's operands have landed (what this half requested may be in flight)
     lds_barrier();
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      request_w(kb + 3, sx, g);
-      if (g < 4) read_half(wf[B ^ 1][2 + (g >> 1)], wl + sw1, 2 + (g >> 1), g & 1);
-      else read_half(xf[(g >> 1) - 2], xl + sx1, (g >> 1) - 2, g & 1);
-      mfma(2 + ((g >> 1) & 1), (g >> 2) * 2, g & 1);
-      mfma(2 + ((g >> 1) & 1), (g >> 2) * 2 + 1, g & 1);
+    for (int u = 0; u < 32; ++u) {
+      const int g = u >> 2;
+      mfma(4 + (u & 3), g);
+      if (u < 12 && u % 2 == 0) request(kb + 2, B, 10 + u / 2);
+      else if (u < 12 && u % 2 == 1) read_x(B ^ 1, (u / 2) >> 1, (u / 2) & 1);
+      if (u == 12 || u == 13) read_x(B ^ 1, 3, u & 1);
+      if ((u & 1) == 0 && u >= 4) { read_w(B ^ 1, (u - 4) >> 2, 0); }
+      if ((u & 1) == 1 && u >= 4) { read_w(B ^ 1, (u - 4) >> 2, 1); }
       __builtin_amdgcn_sched_barrier(0);
     }
-    slot = sw1;
+    read_w(B ^ 1, 7, 0);
+    read_w(B ^ 1, 7, 1);
   };
-  for (int k0 = 0; k0 < a.Kb; k0 += 16) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) xs[i].load(xeg + xeo[i], k0, a.Sp);
-    ws.load(we, k0, a.Sp);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) xs[i].arrive();
-    ws.arrive();
-    const int end = min(k0 + 16, a.Kb);
-    int kb = k0;
-    for (; kb + 1 < end; kb += 2) {
-      step(std::integral_constant<int, 0>{}, kb);
-      step(std::integral_constant<int, 1>{}, kb + 1);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xs[i].down();
-      ws.down();
-    }
-    if (kb < end) step(std::integral_constant<int, 0>{}, kb);
+  int kb = 0;
+  for (; kb < last; kb += 2) {
+    const int set = (~kb >> 1) & 1;
+    step(std::integral_constant<int, 0>{}, kb, set);
+    step(std::integral_constant<int, 1>{}, kb + 1, set);
+    read_exponents(set, ((kb + 2) & 2) * 8);
   }
+  if (kb == last) step(std::integral_constant<int, 0>{}, kb, (~kb >> 1) & 1);
   wait_vmcnt<0>();          // (no request outlives the workgroup's LDS)
   lds_barrier();            // ... and no wave reads another's operands any more
-  f8_finish<4, OUT, GROUPED>(a, t, t.m0 + wm * 128, n0 + wn * 128, acc, lds + wave * F8_STAGE);
+  asm volatile("s_nop 15\n\ts_nop 15");      // the last products are in their registers
+  __builtin_amdgcn_sched_barrier(0);
+  // lane: activation row r16 of fragment i, weight rows 4 h .. + 3 of fragment j
+  f8_finish<4, OUT, GROUPED>(a, t, t.m0 + wm * 128, n0 + wn * 128, lds + wave * F8_STAGE, [&](int g, float* st) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) *(f8_v4f*)(st + (i * 16 + r16) * F8_PITCH + j * 16 + h * 4) = acc[2 * g + i][j];
+  });
 }
 
 template <int OUT, bool GROUPED> int launch_big(const F8Args& a, int rows, int z, hipStream_t st) {
   static std::atomic<uint64_t> attr{0};
-  if (int rc = qbnn_ensure_dyn_lds((const void*)linear_f8_big_kernel<OUT, GROUPED>, &attr, 163840)) return rc;
+  if (int rc = qbnn_ensure_dyn_lds((const void*)linear_f8_big_kernel<OUT, GROUPED>, &attr, F8_BIG_LDS)) return rc;
   const int64_t tm = (rows + 255) / 256 + (GROUPED ? a.groups : 0), tn = (a.N + 255) / 256;
   if (tm * tn > 0x7fffffff || z > 65535) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
-  hipLaunchKernelGGL((linear_f8_big_kernel<OUT, GROUPED>), dim3((unsigned)(tm * tn), 1, (unsigned)z), dim3(256), 163840, st, a, (int)tm, (int)tn);
+  hipLaunchKernelGGL((linear_f8_big_kernel<OUT, GROUPED>), dim3((unsigned)(tm * tn), 1, (unsigned)z), dim3(256), F8_BIG_LDS, st, a, (int)tm, (int)tn);
   return qbnn_check_launch_msg("qbnn_linear_f8");
 }
 
