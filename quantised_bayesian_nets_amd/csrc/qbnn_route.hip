@@ -10,6 +10,7 @@
 #include <stdio.h>
 #include <float.h>
 #include <math.h>
+#include <atomic>
 
 #include "../../include/qbnn.h"
 #include "qbnn_common.h"
@@ -26,12 +27,13 @@ static inline int route_fail(const char* fmt, long a = 0, long b = 0) {
 }
 
 constexpr int ROUTE_ROWS = 64;         // rows of a sample per workgroup = the unit of the counting sort
+constexpr int ROUTE_BLOCKS = 128;      // up to so many workgroups per sample, each sums the others' counts itself; beyond, a kernel between does
 
 struct RouteArgs {
   const void* logits; int64_t l_ss, l_rs;
   const float* bias;
   float* weights; int32_t* experts; int32_t* offsets; int32_t* rows; int32_t* counts;      // counts [S][blocks][E]
-  int S, T, E, k, groups, kept, sigmoid, renorm, blocks;
+  int S, T, E, k, groups, kept, sigmoid, renorm, blocks, bits;                             // bits: of an expert's index
   float scale;
 };
 
@@ -40,163 +42,438 @@ template <int T> __device__ __forceinline__ float route_lowest() {
   else if constexpr (T == QBNN_F16) return -65504.f;
   else return -FLT_MAX;
 }
-__device__ __forceinline__ double shfl_xor_f64(double v, int d) { return __shfl_xor(v, d); }
+__device__ __forceinline__ float route_exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896340736f); }      // off by at most (|v| + 2) 2^-23 of it
 
-template <int T, int CH> __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
-  __shared__ int hist[CH * 64];
-  __shared__ double keys[4][CH * 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int s = blockIdx.y, t0 = blockIdx.x * ROUTE_ROWS, t1 = min(a.T, t0 + ROUTE_ROWS);
-  for (int i = threadIdx.x; i < a.E; i += 256) hist[i] = 0;
-  __syncthreads();
-  const int per = a.E / a.groups;
-  const bool by_logit = !a.bias && a.groups == 1;             // both scores increase with the logit
-  for (int t = t0 + wave; t < t1; t += 4) {
-    const f8_type<T>* l = (const f8_type<T>*)a.logits + s * a.l_ss + t * a.l_rs;
-    float v[CH];
-    bool open[CH], nan = false;
-    float top = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int e = c * 64 + lane;
-      v[c] = e < a.E ? f8_load<T>(l[e]) : -INFINITY;
-      open[c] = v[c] > route_lowest<T>();                     // -inf, the type's lowest value and NaN are masked
-      nan |= v[c] != v[c];
-      if (open[c]) top = fmaxf(top, v[c]);
-    }
-    nan = __any(nan);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    double p[CH], sum = 0.;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      p[c] = !open[c] ? 0. : a.sigmoid ? 1. / (1. + exp(-(double)v[c])) : exp((double)v[c] - (double)top);
-      sum += p[c];
-    }
-    if (!a.sigmoid) {
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) sum += shfl_xor_f64(sum, d);
-#pragma unroll
-      for (int c = 0; c < CH; ++c) if (open[c]) p[c] /= sum;
-    }
-    double key[CH];
-    int idx[CH];
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int e = c * 64 + lane;
-      double q = by_logit ? (double)v[c] : p[c] + (a.bias && e < a.E ? (double)a.bias[e] : 0.);
-      key[c] = open[c] && q == q ? q : -INFINITY;
-      idx[c] = e < a.E ? e : 0x7fffffff;
-    }
-    if (a.groups > 1) {
-      // lane g sums group g's two largest keys (masked experts left out; a group of masked experts ranks last)
-#pragma unroll
-      for (int c = 0; c < CH; ++c) keys[wave][c * 64 + lane] = key[c];
-      __builtin_amdgcn_wave_barrier();
-      double a1 = -INFINITY, a2 = -INFINITY;
-      if (lane < a.groups)
-        for (int i = 0; i < per; ++i) {
-          const double q = keys[wave][lane * per + i];
-          if (q > a1) { a2 = a1; a1 = q; } else if (q > a2) a2 = q;
-        }
-      const double g = a1 == -INFINITY ? -INFINITY : a2 == -INFINITY ? a1 : a1 + a2;
-      int rank = 0;
-      for (int i = 0; i < a.groups; ++i) {
-        const double o = __shfl(g, i);
-        rank += o > g || (o == g && i < lane) ? 1 : 0;
+// ---- reductions over the L lanes (a power of two) of a row: each step's partner holds what the step before left in all lanes of its half ------------
+template <int CTRL> __device__ __forceinline__ uint32_t route_dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+template <int STEP> __device__ __forceinline__ uint32_t route_partner(uint32_t v) {
+  if constexpr (STEP == 1) return route_dpp<0xB1>(v);              // quad_perm 1 0 3 2
+  else if constexpr (STEP == 2) return route_dpp<0x4E>(v);         // quad_perm 2 3 0 1
+  else if constexpr (STEP == 4) return route_dpp<0x141>(v);        // row_half_mirror
+  else if constexpr (STEP == 8) return route_dpp<0x140>(v);        // row_mirror
+  else return (uint32_t)__shfl_xor((int)v, STEP);
+}
+template <int L, class F> __device__ __forceinline__ uint32_t route_reduce(uint32_t v, F f) {
+  if constexpr (L > 1) v = f(v, route_partner<1>(v));
+  if constexpr (L > 2) v = f(v, route_partner<2>(v));
+  if constexpr (L > 4) v = f(v, route_partner<4>(v));
+  if constexpr (L > 8) v = f(v, route_partner<8>(v));
+  if constexpr (L > 16) v = f(v, route_partner<16>(v));
+  if constexpr (L > 32) v = f(v, route_partner<32>(v));
+  return v;
+}
+template <int L> __device__ __forceinline__ uint32_t route_max(uint32_t v) { return route_reduce<L>(v, [](uint32_t a, uint32_t b) { return max(a, b); }); }
+template <int L> __device__ __forceinline__ float route_maxf(float v) {
+  return __uint_as_float(route_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+template <int L> __device__ __forceinline__ float route_sumf(float v) {
+  return __uint_as_float(route_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+// order-preserving bits of a float and back
+__device__ __forceinline__ uint32_t route_order(float v) { const uint32_t b = __float_as_uint(v); return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u); }
+__device__ __forceinline__ float route_value(uint32_t o) { return __uint_as_float(o ^ ((uint32_t)((int)~o >> 31) | 0x80000000u)); }
+
+// The group mask of a row whose keys lie in `keys` (LDS): lane q < rows x groups of the wave takes group q % groups of row q / groups and sums its two largest keys
+// (masked experts left out; a group of masked experts ranks last); ranks come from comparing with the row's other groups.  slack[row]: the score
+// of the last group kept minus the best one left out.  FLT: the keys' type.
+template <class FLT> __device__ __forceinline__ void route_groups(const RouteArgs& a, const FLT* keys, int rows, int pitch, FLT* score, uint32_t* stay, FLT* slack) {
+  const int lane = threadIdx.x & 63, per = a.E / a.groups;
+  for (int q0 = 0; q0 < rows * a.groups; q0 += 64) {
+    const int q = q0 + lane;
+    if (q < rows * a.groups) {
+      const int r = q / a.groups, g = q - r * a.groups;
+      const FLT* k = keys + r * pitch + g * per;
+      FLT a1 = -INFINITY, a2 = -INFINITY;
+      for (int i = 0; i < per; ++i) {
+        const FLT v = k[i];
+        if (v > a1) { a2 = a1; a1 = v; } else if (v > a2) a2 = v;
       }
-      const unsigned long long stay = __ballot(lane < a.groups && rank < a.kept);
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int e = c * 64 + lane;
-        if (e < a.E && !((stay >> (e / per)) & 1)) { key[c] = -INFINITY; idx[c] = 0x7fffffff; }
-      }
-      __builtin_amdgcn_wave_barrier();
-    }
-    int my_e = 0;
-    double my_p = 0.;
-    for (int j = 0; j < a.k; ++j) {
-      double b = key[0], bp = p[0];
-      int bi = idx[0];
-#pragma unroll
-      for (int c = 1; c < CH; ++c)
-        if (key[c] > b || (key[c] == b && idx[c] < bi)) { b = key[c]; bi = idx[c]; bp = p[c]; }
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const double ob = shfl_xor_f64(b, d), op = shfl_xor_f64(bp, d);
-        const int oi = __shfl_xor(bi, d);
-        if (ob > b || (ob == b && oi < bi)) { b = ob; bi = oi; bp = op; }
-      }
-#pragma unroll
-      for (int c = 0; c < CH; ++c) if (idx[c] == bi) { key[c] = -INFINITY; idx[c] = 0x7fffffff; }
-      if (lane == j) { my_e = bi; my_p = bp; }
-    }
-    double total = 0.;
-    if (a.renorm) {
-      total = lane < a.k ? my_p : 0.;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) total += shfl_xor_f64(total, d);
-    }
-    if (lane < a.k) {
-      const double w = a.renorm ? (total == 0. ? 0. : my_p / total) : my_p;
-      const int64_t at = ((int64_t)s * a.T + t) * a.k + lane;
-      a.weights[at] = nan ? NAN : (float)(w * (double)a.scale);
-      a.experts[at] = my_e;
-      atomicAdd(&hist[my_e], 1);                             // (a count: its value does not depend on the order)
+      score[q] = a1 == -INFINITY ? a1 : a2 == -INFINITY ? a1 : a1 + a2;
     }
   }
-  __syncthreads();
-  int32_t* out = a.counts + ((int64_t)s * a.blocks + blockIdx.x) * a.E;
-  for (int i = threadIdx.x; i < a.E; i += 256) out[i] = hist[i];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  for (int q0 = 0; q0 < rows * a.groups; q0 += 64) {
+    const int q = q0 + lane;
+    if (q < rows * a.groups) {
+      const int r = q / a.groups, g = q - r * a.groups;
+      const FLT mine = score[q];
+      int rank = 0;
+      FLT next = -INFINITY;                                     // the best score behind mine
+      for (int i = 0; i < a.groups; ++i) {
+        const FLT o = score[r * a.groups + i];
+        const bool ahead = o > mine || (o == mine && i < g);
+        rank += ahead ? 1 : 0;
+        if (!ahead && i != g && o > next) next = o;
+      }
+      stay[q] = rank < a.kept ? 1u : 0u;
+      if (rank == a.kept - 1) slack[r] = a.kept == a.groups ? (FLT)INFINITY : mine == next ? (FLT)0 : mine - next;
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
-// counts -> exclusive prefix over a sample's workgroups, per expert; offsets -> exclusive prefix over its experts
-__global__ __launch_bounds__(256) void route_scan_kernel(const RouteArgs a) {
-  __shared__ int total[1024];
-  const int s = blockIdx.x;
-  for (int e = threadIdx.x; e < a.E; e += 256) {
-    int run = 0;
-    for (int b = 0; b < a.blocks; ++b) {
-      int32_t* c = a.counts + ((int64_t)s * a.blocks + b) * a.E + e;
-      const int n = *c;
-      *c = run;
-      run += n;
+// ---- the order of the rows -----------------------------------------------------------------------------------------------------
+// A counting sort, stable: a workgroup's n choices in four quarters, one per wave; count[wave][E] holds each quarter's number of every expert and then the
+// position of its next one.  Within 64 choices a lane's rank is the number of lanes below it with the same expert, from one ballot per index bit.
+__device__ __forceinline__ int route_quarter(int n) { return ((n + 255) >> 8) << 6; }
+__device__ __forceinline__ void route_count(const uint32_t* choice, int* count, int n, int E) {      // count is 0
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, q = route_quarter(n);
+  for (int i = wave * q + lane; i < min(n, (wave + 1) * q); i += 64) atomicAdd(&count[wave * E + choice[i]], 1);      // (a number: no order)
+  __syncthreads();
+}
+// exclusive prefix over E values, four per thread and pass; at(e) reads, put(e, prefix) takes
+template <class At, class Put> __device__ __forceinline__ void route_prefix(int E, At at, Put put) {
+  __shared__ int sums[4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, e0 = threadIdx.x * 4;
+  int v[4], mine = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[i] = e0 + i < E ? at(e0 + i) : 0; mine += v[i]; }
+  int incl = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) { const int u = __shfl_up(incl, d); if (lane >= d) incl += u; }
+  if (lane == 63) sums[wave] = incl;
+  __syncthreads();
+  int run = incl - mine;
+  for (int w = 0; w < wave; ++w) run += sums[w];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (e0 + i < E) { put(e0 + i, run); run += v[i]; }
+}
+// count: each quarter's position of its next choice of e
+__device__ __forceinline__ void route_place(const RouteArgs& a, const uint32_t* choice, int* count, int n, int first) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, q = route_quarter(n);
+  int* mine = count + wave * a.E;
+  for (int i0 = wave * q; i0 < min(n, (wave + 1) * q); i0 += 64) {
+    const int i = i0 + lane;
+    const bool in = i < n;
+    const uint32_t e = in ? choice[i] : 0u;
+    unsigned long long same = __ballot(in);
+    for (int b = 0; b < a.bits; ++b) {
+      const unsigned long long ones = __ballot((e >> b) & 1);
+      same &= (e >> b) & 1 ? ones : ~ones;
     }
-    total[e] = run;
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    const int at = in ? mine[e] : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (in) {
+      a.rows[at + rank] = first + i;
+      if (rank == 0) mine[e] = at + __popcll(same);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+}
+// start(e): position of the workgroup's first choice of e -> the quarters' own positions
+template <class F> __device__ __forceinline__ void route_starts(int* count, int E, F start) {
+  for (int e = threadIdx.x; e < E; e += 256) {
+    int run = start(e);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) { const int c = count[w * E + e]; count[w * E + e] = run; run += c; }
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int run = s * a.T * a.k;
-    for (int e = 0; e < a.E; ++e) { a.offsets[s * a.E + e] = run; run += total[e]; }
-    if (s == a.S - 1) a.offsets[a.S * a.E] = run;
+}
+
+// L lanes per row, 16 neighbouring experts per lane.
+//
+// Fast pass: keys in fp32 as ordered integers, an expert's index (its complement) in their low bits, so that a round of the choice is one integer maximum and ties go
+// to the lowest index.  It decides where it provably can: logits of 16 bits compare exactly as they are; elsewhere each chosen key must lie above the next
+// one by more than the keys' error and the bits given up (and likewise the last group kept above the next).  The waves where one does not (a few
+// rows in a thousand, and rows with ties) do their rows again with 64-bit keys.
+// Bound: 16384 x 256 logits are 3 us of reading; a round costs 45 vector instructions for 64 / L rows.
+template <int L> __host__ __device__ constexpr int route_group_bytes(int groups) { return ((64 / L) * ((L * 16 + 2) * 8 + groups * 12 + 8) + 15) & ~15; }      // of a wave
+
+template <int T, int L> __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
+  constexpr int RPW = 64 / L;                                   // rows per wave
+  constexpr int PITCH = L * 16 + 2;
+  extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
+  __shared__ float row_top[ROUTE_ROWS], row_sum[ROUTE_ROWS];
+  // dynamic: choices and their scores [64][k], the quarters' counts [4][E], starts [E], and with groups each wave's keys, scores, masks
+  uint32_t* choice = (uint32_t*)dyn;
+  float* part = (float*)(choice + ROUTE_ROWS * a.k);
+  int* count = (int*)(part + ROUTE_ROWS * a.k);
+  int* start = count + 4 * a.E;
+  uint8_t* more = (uint8_t*)(start + a.E);
+  more += (-(uintptr_t)more) & 15;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / L, li = lane % L;
+  const int s = blockIdx.y, t0 = blockIdx.x * ROUTE_ROWS, rows = min(a.T - t0, ROUTE_ROWS);
+  const uint32_t low = (1u << a.bits) - 1;
+  const bool by_logit = !a.bias && a.groups == 1;               // both scores increase with the logit
+  const f8_type<T>* base = (const f8_type<T>*)a.logits + s * a.l_ss + t0 * a.l_rs;
+  for (int i = threadIdx.x; i < 4 * a.E; i += 256) count[i] = 0;
+
+  for (int r0 = wave * RPW; r0 < rows; r0 += 4 * RPW) {
+    const int r = r0 + sub, e0 = li * 16;
+    const bool valid = r < rows;
+    const f8_type<T>* l = base + (int64_t)min(r, rows - 1) * a.l_rs + e0;
+    float v[16];
+    if (e0 + 16 <= a.E) {
+      f8_type<T> raw[16];
+      __builtin_memcpy(raw, l, sizeof(raw));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = f8_load<T>(raw[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = e0 + i < a.E ? f8_load<T>(l[i]) : -INFINITY;
+    }
+    uint32_t open = 0;                                          // not masked: -inf, the type's lowest value and NaN are
+    bool nan = false;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      nan |= v[i] != v[i];
+      if (v[i] > route_lowest<T>()) { open |= 1u << i; top = fmaxf(top, v[i]); }
+    }
+    top = route_maxf<L>(top);
+    float sc[16], sum = 0.f, worst = 0.f;                       // scores; the largest error of one, in 2^-23
+    if (!by_logit || !a.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = a.sigmoid ? -v[i] : v[i] - top;
+        const float z = route_exp(x);
+        sc[i] = (open >> i) & 1 ? (a.sigmoid ? 1.f / (1.f + z) : z) : 0.f;
+        sum += sc[i];
+      }
+    }
+    if (!a.sigmoid) sum = route_sumf<L>(sum);
+    if (li == 0 && valid) {
+      row_top[r] = top;
+      row_sum[r] = sum;
+    }
+    if (route_max<L>(nan ? 1u : 0u) && li == 0 && valid) row_top[r] = NAN;
+
+    uint32_t w[16];
+    bool unsure = false;
+    if (by_logit) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float q = (open >> i) & 1 ? v[i] + 0.f : -INFINITY;      // (-0 ties with 0)
+        w[i] = e0 + i < a.E ? (route_order(q) & ~low) | (low - (uint32_t)(e0 + i)) : 0u;
+      }
+    } else {
+      const float over = a.sigmoid ? 1.f : 1.f / sum;
+      float key[16], large = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = a.sigmoid ? sc[i] : sc[i] * over;
+        const float q = (open >> i) & 1 ? p + (a.bias && e0 + i < a.E ? a.bias[e0 + i] : 0.f) : -INFINITY;
+        key[i] = q == q ? q : -INFINITY;
+        if (key[i] > -INFINITY) {
+          worst = fmaxf(worst, p * (fabsf(a.sigmoid ? v[i] : v[i] - top) + 32.f));
+          large = fmaxf(large, fabsf(key[i]));
+        }
+      }
+      large = route_maxf<L>(large);
+      worst = (route_maxf<L>(worst) + large) * 2.384185791015625e-7f;      // 2 x 2^-23: of two keys' difference
+      unsure = !(worst < INFINITY);
+      uint32_t in = 0xffffu;
+      if (a.groups > 1) {
+        float* keys = (float*)(more + (size_t)wave * route_group_bytes<L>(a.groups));
+        float* score = keys + RPW * PITCH;
+        uint32_t* stay = (uint32_t*)(score + RPW * a.groups);
+        float* slack = (float*)(stay + RPW * a.groups);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) keys[sub * PITCH + e0 + i] = key[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        route_groups<float>(a, keys, RPW, PITCH, score, stay, slack);
+        unsure |= !(slack[sub] > 2.f * worst + large * 4.8e-7f);
+        const int per = a.E / a.groups;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (e0 + i < a.E && !stay[sub * a.groups + (e0 + i) / per]) in &= ~(1u << i);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = e0 + i < a.E && ((in >> i) & 1) ? (route_order(key[i]) & ~low) | (low - (uint32_t)(e0 + i)) : 0u;
+    }
+    // k rounds, and one more to see that the last choice was none too close
+    const bool exact = by_logit && T != QBNN_F32;
+    uint32_t before = 0;
+    for (int j = 0; j < a.k + (exact ? 0 : 1); ++j) {
+      uint32_t m = w[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) m = max(m, w[i]);
+      m = route_max<L>(m);
+      if (j < a.k && li == 0 && valid) choice[r * a.k + j] = low - (m & low);
+      if (!exact && j > 0 && m != 0) {
+        if (by_logit) unsure |= ((before ^ m) & ~low) == 0;
+        else unsure |= !(route_value(before & ~low) - route_value(m | low) > worst);
+      }
+      before = m;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = w[i] == m ? 0u : w[i];
+    }
+    if (__any(unsure && valid)) {
+      double key[16], total = 0.;
+      int idx[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const double x = (double)v[i];
+        key[i] = !((open >> i) & 1) ? 0. : by_logit ? x : a.sigmoid ? 1. / (1. + exp(-x)) : exp(x - (double)top);
+        total += key[i];
+        idx[i] = e0 + i < a.E ? e0 + i : 0x7fffffff;
+      }
+      if (!by_logit && !a.sigmoid)
+#pragma unroll
+        for (int d = 1; d < L; d <<= 1) total += __shfl_xor(total, d);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        double q = by_logit || a.sigmoid ? key[i] : key[i] / total;
+        if (a.bias && e0 + i < a.E) q += (double)a.bias[e0 + i];
+        key[i] = ((open >> i) & 1) && q == q ? q : -INFINITY;
+      }
+      if (a.groups > 1) {
+        double* keys = (double*)(more + (size_t)wave * route_group_bytes<L>(a.groups));
+        double* score = keys + RPW * PITCH;
+        double* slack = score + RPW * a.groups;
+        uint32_t* stay = (uint32_t*)(slack + RPW);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) keys[sub * PITCH + e0 + i] = key[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        route_groups<double>(a, keys, RPW, PITCH, score, stay, slack);
+        const int per = a.E / a.groups;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (e0 + i < a.E && !stay[sub * a.groups + (e0 + i) / per]) { key[i] = -INFINITY; idx[i] = 0x7fffffff; }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+      for (int j = 0; j < a.k; ++j) {
+        double b = key[0];
+        int bi = idx[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i)
+          if (key[i] > b || (key[i] == b && idx[i] < bi)) { b = key[i]; bi = idx[i]; }
+#pragma unroll
+        for (int d = 1; d < L; d <<= 1) {
+          const double ob = __shfl_xor(b, d);
+          const int oi = __shfl_xor(bi, d);
+          if (ob > b || (ob == b && oi < bi)) { b = ob; bi = oi; }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) if (idx[i] == bi) { key[i] = -INFINITY; idx[i] = 0x7fffffff; }
+        if (li == 0 && valid) choice[r * a.k + j] = (uint32_t)bi;
+      }
+    }
   }
+  __syncthreads();
+
+  // weights: a thread per choice, scores taken again from the logits
+  const int n = rows * a.k;
+  const int64_t first = ((int64_t)s * a.T + t0) * a.k;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int r = i / a.k, e = (int)choice[i];
+    const float l = f8_load<T>(base[(int64_t)r * a.l_rs + e]), top = row_top[r];
+    float p = a.sigmoid ? 1.f / (1.f + route_exp(-l)) : route_exp(l - top) / row_sum[r];
+    if (!(l > route_lowest<T>())) p = 0.f;
+    if (top != top) p = NAN;
+    part[i] = p;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += 256) {
+    float p = part[i];
+    if (a.renorm) {
+      const int r = i / a.k;
+      float total = 0.f;
+      for (int j = 0; j < a.k; ++j) total += part[r * a.k + j];
+      p = total == 0.f ? 0.f : p / total;
+    }
+    a.weights[first + i] = p * a.scale;
+    a.experts[first + i] = (int32_t)choice[i];
+  }
+  route_count(choice, count, n, a.E);
+  auto total = [&](int e) { return count[e] + count[a.E + e] + count[2 * a.E + e] + count[3 * a.E + e]; };
+  if (a.blocks > 1) {
+    int32_t* out = a.counts + ((int64_t)s * (a.blocks + 1) + blockIdx.x) * a.E;
+    for (int e = threadIdx.x; e < a.E; e += 256) out[e] = total(e);
+    return;
+  }
+  const int all = s * a.T * a.k;
+  route_prefix(a.E, total, [&](int e, int before) { a.offsets[s * a.E + e] = start[e] = all + before; });
+  if (s == a.S - 1 && threadIdx.x == 0) a.offsets[a.S * a.E] = all + n;
+  __syncthreads();
+  route_starts(count, a.E, [&](int e) { return start[e]; });
+  route_place(a, choice, count, n, (int)first);
+}
+
+// counts [blocks + 1][E] of a sample: each workgroup's -> the workgroups' before it, and the sum in the last row.  16 experts per workgroup, 16 runs of rows.
+__global__ __launch_bounds__(256) void route_scan_kernel(const RouteArgs a) {
+  __shared__ int run[16][17];
+  const int e = blockIdx.x * 16 + (threadIdx.x & 15), r = threadIdx.x >> 4, per = (a.blocks + 15) / 16;
+  int32_t* c = a.counts + (int64_t)blockIdx.y * (a.blocks + 1) * a.E + e;
+  const int b0 = r * per, b1 = min(a.blocks, b0 + per);
+  int sum = 0;
+  if (e < a.E)
+    for (int b = b0; b < b1; ++b) sum += c[(int64_t)b * a.E];
+  run[r][threadIdx.x & 15] = sum;
+  __syncthreads();
+  if (e >= a.E) return;
+  int at = 0, all = 0;
+  for (int i = 0; i < 16; ++i) { const int v = run[i][threadIdx.x & 15]; at += i < r ? v : 0; all += v; }
+  for (int b = b0; b < b1; ++b) { const int v = c[(int64_t)b * a.E]; c[(int64_t)b * a.E] = at; at += v; }
+  if (r == 0) c[(int64_t)a.blocks * a.E] = all;
 }
 
 __global__ __launch_bounds__(256) void route_scatter_kernel(const RouteArgs a) {
-  extern __shared__ int32_t mine[];
-  const int s = blockIdx.y, t0 = blockIdx.x * ROUTE_ROWS, n = (min(a.T, t0 + ROUTE_ROWS) - t0) * a.k;
+  extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
+  uint32_t* choice = (uint32_t*)dyn;
+  int* count = (int*)(choice + ROUTE_ROWS * a.k);
+  int* before = count + 4 * a.E;                                // of the sample's workgroups before this one
+  int* sums = before + a.E;
+  const int s = blockIdx.y, blk = blockIdx.x, t0 = blk * ROUTE_ROWS, n = (min(a.T, t0 + ROUTE_ROWS) - t0) * a.k;
   const int64_t first = ((int64_t)s * a.T + t0) * a.k;
-  for (int i = threadIdx.x; i < n; i += 256) mine[i] = a.experts[first + i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const int e = mine[i];
-    int rank = 0;
-    for (int j = 0; j < i; ++j) rank += mine[j] == e ? 1 : 0;
-    a.rows[a.offsets[s * a.E + e] + a.counts[((int64_t)s * a.blocks + blockIdx.x) * a.E + e] + rank] = (int32_t)(first + i);
+  for (int i = threadIdx.x; i < 4 * a.E; i += 256) count[i] = 0;
+  for (int i = threadIdx.x; i < n; i += 256) choice[i] = (uint32_t)a.experts[first + i];
+  const int32_t* c = a.counts + (int64_t)s * (a.blocks + 1) * a.E;
+  for (int e = threadIdx.x; e < a.E; e += 256) {
+    if (a.blocks > ROUTE_BLOCKS) {
+      before[e] = c[(int64_t)blk * a.E + e];
+      sums[e] = c[(int64_t)a.blocks * a.E + e];
+    } else {
+      int lower = 0, all = 0;
+#pragma unroll 8
+      for (int b = 0; b < a.blocks; ++b) {
+        const int v = c[(int64_t)b * a.E + e];
+        lower += b < blk ? v : 0;
+        all += v;
+      }
+      before[e] = lower;
+      sums[e] = all;
+    }
   }
+  __syncthreads();
+  route_count(choice, count, n, a.E);
+  const int all = s * a.T * a.k;
+  route_prefix(a.E, [&](int e) { return sums[e]; }, [&](int e, int lower) {
+    before[e] += all + lower;
+    if (blk == 0) a.offsets[s * a.E + e] = all + lower;
+  });
+  if (blk == 0 && s == a.S - 1 && threadIdx.x == 0) a.offsets[a.S * a.E] = all + a.T * a.k;
+  __syncthreads();
+  route_starts(count, a.E, [&](int e) { return before[e]; });
+  route_place(a, choice, count, n, (int)first);
 }
 
+template <int T, int L> int launch_route_as(const RouteArgs& a, hipStream_t st) {
+  static std::atomic<uint64_t> attr{0};
+  const int waves = L < 4 ? L : 4;                              // 64 / L rows each: that many have rows
+  const int lds = ROUTE_ROWS * a.k * 8 + a.E * 20 + 16 + (a.groups > 1 ? waves * route_group_bytes<L>(a.groups) : 0);
+  if (int rc = qbnn_ensure_dyn_lds((const void*)route_kernel<T, L>, &attr, 128 * 1024)) return rc;
+  hipLaunchKernelGGL((route_kernel<T, L>), dim3((unsigned)a.blocks, (unsigned)a.S), dim3(256), lds, st, a);
+  return qbnn_check_launch_msg("qbnn_route_experts");
+}
 template <int T> int launch_route(const RouteArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)a.blocks, (unsigned)a.S);
-  if (a.E <= 64) hipLaunchKernelGGL((route_kernel<T, 1>), grid, dim3(256), 0, st, a);
-  else if (a.E <= 128) hipLaunchKernelGGL((route_kernel<T, 2>), grid, dim3(256), 0, st, a);
-  else if (a.E <= 256) hipLaunchKernelGGL((route_kernel<T, 4>), grid, dim3(256), 0, st, a);
-  else if (a.E <= 512) hipLaunchKernelGGL((route_kernel<T, 8>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((route_kernel<T, 16>), grid, dim3(256), 0, st, a);
-  if (int rc = qbnn_check_launch_msg("qbnn_route_experts")) return rc;
-  hipLaunchKernelGGL(route_scan_kernel, dim3((unsigned)a.S), dim3(256), 0, st, a);
-  if (int rc = qbnn_check_launch_msg("qbnn_route_experts (scan)")) return rc;
-  hipLaunchKernelGGL(route_scatter_kernel, grid, dim3(256), ROUTE_ROWS * a.k * sizeof(int32_t), st, a);
+  int rc;
+  if (a.E <= 16) rc = launch_route_as<T, 1>(a, st);
+  else if (a.E <= 32) rc = launch_route_as<T, 2>(a, st);
+  else if (a.E <= 64) rc = launch_route_as<T, 4>(a, st);
+  else if (a.E <= 128) rc = launch_route_as<T, 8>(a, st);
+  else if (a.E <= 256) rc = launch_route_as<T, 16>(a, st);
+  else if (a.E <= 512) rc = launch_route_as<T, 32>(a, st);
+  else rc = launch_route_as<T, 64>(a, st);
+  if (rc || a.blocks == 1) return rc;
+  if (a.blocks > ROUTE_BLOCKS) {
+    hipLaunchKernelGGL(route_scan_kernel, dim3((unsigned)((a.E + 15) / 16), (unsigned)a.S), dim3(256), 0, st, a);
+    if ((rc = qbnn_check_launch_msg("qbnn_route_experts (scan)"))) return rc;
+  }
+  hipLaunchKernelGGL(route_scatter_kernel, dim3((unsigned)a.blocks, (unsigned)a.S), dim3(256), ROUTE_ROWS * a.k * 4 + a.E * 24, st, a);
   return qbnn_check_launch_msg("qbnn_route_experts (order)");
 }
 
@@ -229,7 +506,7 @@ template <int T> __global__ __launch_bounds__(256) void combine_kernel(const flo
 }  // namespace
 
 QBNN_EXPORT int64_t qbnn_route_workspace_ints(int32_t S, int32_t T, int32_t E) {
-  return S <= 0 || T <= 0 || E <= 0 ? 0 : (int64_t)S * ((T + ROUTE_ROWS - 1) / ROUTE_ROWS) * E;
+  return S <= 0 || T <= 0 || E <= 0 ? 0 : (int64_t)S * ((T + ROUTE_ROWS - 1) / ROUTE_ROWS + 1) * E;
 }
 
 QBNN_EXPORT int qbnn_route_experts(const qbnn_route* r, void* stream) {
@@ -246,6 +523,7 @@ QBNN_EXPORT int qbnn_route_experts(const qbnn_route* r, void* stream) {
   a.weights = r->weights; a.experts = r->experts; a.offsets = r->offsets; a.rows = r->rows; a.counts = r->workspace;
   a.S = r->S; a.T = r->T; a.E = r->E; a.k = r->top_k; a.groups = r->groups; a.kept = r->top_groups; a.sigmoid = r->sigmoid; a.renorm = r->renormalize; a.scale = r->scale;
   a.blocks = (r->T + ROUTE_ROWS - 1) / ROUTE_ROWS;
+  for (a.bits = 0; (1 << a.bits) < r->E; ++a.bits) {}
   switch (r->type) {
     case QBNN_F32: return launch_route<QBNN_F32>(a, (hipStream_t)stream);
     case QBNN_BF16: return launch_route<QBNN_BF16>(a, (hipStream_t)stream);

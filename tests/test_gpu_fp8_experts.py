@@ -193,7 +193,7 @@ def route_check(logits, k, **kw):
     return r
 
 
-@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 8, 2), (5, 3, 3), (63, 60, 4), (64, 64, 6), (65, 65, 8), (300, 128, 1), (129, 130, 7), (1000, 256, 8), (77, 512, 16), (40, 1024, 32), (4097, 16, 2)])
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 8, 2), (5, 3, 3), (63, 60, 4), (64, 64, 6), (65, 65, 8), (300, 128, 1), (129, 130, 7), (1000, 256, 8), (77, 512, 16), (40, 1024, 32), (4097, 16, 2), (8300, 20, 3)])
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_router(T, E, k, dtype):
     for score, renorm in itertools.product(("softmax", "sigmoid"), (False, True)):
