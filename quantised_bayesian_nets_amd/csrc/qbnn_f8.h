@@ -65,51 +65,43 @@ __device__ __forceinline__ uint32_t f8_magnitude(float v) {
   const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
   return b < 0x7f800000u ? b : 0u;
 }
-// four values already scaled to [-448, 448] -> four e4m3 bytes; what is not finite becomes NaN (0x7f), set apart from the conversion's mode
+// four values already scaled to [-448, 448] -> four e4m3 bytes; the conversion makes a NaN of what is not finite
 __device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d) {
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
-  uint32_t u = (uint32_t)r;
-  if (!(fabsf(a) <= 448.f)) u = (u & 0xffffff00u) | 0x7fu;
-  if (!(fabsf(b) <= 448.f)) u = (u & 0xffff00ffu) | 0x7f00u;
-  if (!(fabsf(c) <= 448.f)) u = (u & 0xff00ffffu) | 0x7f0000u;
-  if (!(fabsf(d) <= 448.f)) u = (u & 0x00ffffffu) | 0x7f000000u;
-  return u;
+  const int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
 }
 
 // ---- matrix instruction --------------------------------------------------------------------------------------------------------
 // D[16 weight rows][16 activation rows] += (128 columns of both) with one power of two per operand row; lane l supplies row l & 15 of
 // both operands, 32 of the 128 columns -- any 32, as long as the four lane groups of both operands agree on them, since all 128 columns of a
-// row share its scale (byte 0 of ws / xs).  D: lane l holds weight rows 4 (l >> 4) .. + 3 of activation row l & 15.
+// row share its scale (a byte of ws / xs).  D: lane l holds weight rows 4 (l >> 4) .. + 3 of activation row l & 15.
 //
 // f8_mfma: the e4m3 instruction.  It adds the products of 8 neighbouring bytes after aligning them to the largest, what lies 2^-13 below it cut
 // off, and keeps fp32 from there on (probed): 1.3e-5 of the result's norm on normal data, an eightieth of half a step of fp16 and a
 // hundred-and-fiftieth of bf16's -- the form for results of 16 and 8 bits.
-// f8_mfma_exact: the operands widened to bf16 (exact) and multiplied by the bf16 instruction, whose sums are fp32 throughout, the block's
-// scale applied to its sum: half the matrix rate, the widening beside it on the vector unit; the form for fp32 results.
-__device__ __forceinline__ f8_v4f f8_mfma(f8_v8i w, f8_v8i x, f8_v4f acc, int ws, int xs) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc, 0, 0, 0, ws, 0, xs);
+// f8_mfma_exact: the operands widened to bf16 times their block's scale (both exact) and multiplied by the bf16 instruction, whose sums are fp32
+// throughout: half the matrix rate, the widening beside it on the vector unit; the form for fp32 results.
+template <int BYTE> __device__ __forceinline__ f8_v4f f8_mfma(f8_v8i w, f8_v8i x, f8_v4f acc, uint32_t ws, uint32_t xs) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc, 0, 0, BYTE, (int)ws, BYTE, (int)xs);
 }
 typedef __bf16 f8_v8b __attribute__((ext_vector_type(8)));
 typedef __bf16 f8_v2b __attribute__((ext_vector_type(2)));
 struct F8Wide { f8_v8b part[4]; };
-__device__ __forceinline__ F8Wide f8_widen(f8_v8i v) {
+// exponent: biased, in the lowest byte
+__device__ __forceinline__ F8Wide f8_widen(f8_v8i v, uint32_t exponent) {
+  const float s = __uint_as_float((exponent & 255) << 23);
   F8Wide o;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const f8_v2b a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * g], 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * g], 1.f, true);
-    const f8_v2b c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * g + 1], 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * g + 1], 1.f, true);
+    const f8_v2b a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * g], s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * g], s, true);
+    const f8_v2b c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * g + 1], s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * g + 1], s, true);
     o.part[g] = (f8_v8b){a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
   }
   return o;
 }
-__device__ __forceinline__ f8_v4f f8_mfma_exact(const F8Wide& w, const F8Wide& x, f8_v4f acc, int ws, int xs) {
-  f8_v4f c = {0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ f8_v4f f8_mfma_exact(const F8Wide& w, const F8Wide& x, f8_v4f acc) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.part[g], x.part[g], c, 0, 0, 0);
-  const int n = ws + xs - 254;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) acc[i] += __builtin_ldexpf(c[i], n);
+  for (int g = 0; g < 4; ++g) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.part[g], x.part[g], acc, 0, 0, 0);
   return acc;
 }
 

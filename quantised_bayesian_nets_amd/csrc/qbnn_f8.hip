@@ -31,7 +31,15 @@ struct QuantF8Args {
   const void* x; int64_t x_bs, x_rs;       // batch / row stride in elements; columns are contiguous
   uint8_t* q; uint8_t* e;                  // [batch][R][Kp], [batch][Rb][Sp]
   int R, K, Kb, Sp; int64_t blocks;        // blocks = batch * Rb * Kb
+  uint32_t kb_magic, r_magic; int kb_shift, r_shift;      // division by Kb and R: n * magic >> (32 + shift), n < 2^31 (rows form)
 };
+// n / d for n < 2^31: the smallest p with 2^p >= d gives an error below 1 / d
+static void f8_magic(uint32_t d, uint32_t& magic, int& shift) {
+  shift = 0;
+  while ((1u << shift) < d) ++shift;
+  magic = (uint32_t)((((uint64_t)1 << (31 + shift)) + d - 1) / d);
+}
+__device__ __forceinline__ uint32_t f8_divide(uint32_t n, uint32_t magic, int shift) { return (uint32_t)(((uint64_t)n * magic) >> (31 + shift)); }
 
 // 8 columns from `col` of a row of K (zeros behind the last); rows may start at any element's address
 template <int T> __device__ __forceinline__ void f8_load8(const f8_type<T>* row, int col, int K, float (&v)[8]) {
@@ -51,10 +59,9 @@ __device__ __forceinline__ uint32_t f8_max8(const float (&v)[8]) {
   for (int i = 0; i < 8; ++i) m = max(m, f8_magnitude(v[i]));
   return m;
 }
-__device__ __forceinline__ uint32_t f8_max16(uint32_t m) {      // over the 16 lanes of a row's block
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
-  return m;
+template <int CTRL> __device__ __forceinline__ uint32_t f8_max_dpp(uint32_t m) { return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, CTRL, 0xf, 0xf, true)); }
+__device__ __forceinline__ uint32_t f8_max16(uint32_t m) {      // over the 16 lanes of a row's block: quads, then halves and rows mirrored
+  return f8_max_dpp<0x140>(f8_max_dpp<0x141>(f8_max_dpp<0x4E>(f8_max_dpp<0xB1>(m))));
 }
 __device__ __forceinline__ f8_v2i f8_scale8(const float (&v)[8], float down) {
   return (f8_v2i){(int)f8_pack4(v[0] * down, v[1] * down, v[2] * down, v[3] * down), (int)f8_pack4(v[4] * down, v[5] * down, v[6] * down, v[7] * down)};
@@ -66,18 +73,35 @@ __device__ __forceinline__ void f8_put_exponent(uint8_t* row, int kb, int Kb, in
     for (int i = Kb; i < Sp; ++i) row[i] = 0;
 }
 
-template <int T> __global__ __launch_bounds__(256) void quantize_f8_rows_kernel(const QuantF8Args a) {
-  const int64_t b = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (b >= a.blocks) return;                                        // (all 16 lanes of a block)
-  const int64_t r = b / a.Kb;
-  const int kb = (int)(b - r * a.Kb), j = threadIdx.x & 15;
-  const int64_t bt = r / a.R;
-  const f8_type<T>* row = (const f8_type<T>*)a.x + bt * a.x_bs + (r - bt * a.R) * a.x_rs;
-  float v[8];
-  f8_load8<T>(row, kb * 128 + j * 8, a.K, v);
-  const int e = f8_exponent(f8_max16(f8_max8(v)));
-  *(f8_v2i*)(a.q + r * ((int64_t)a.Kb * 128) + kb * 128 + j * 8) = f8_scale8(v, f8_pow2(-e));
-  if (j == 0) f8_put_exponent(a.e + r * a.Sp, kb, a.Kb, a.Sp, e);
+// U blocks, 16 apart, in flight per 16 lanes (4 for large inputs, 1 where there are too few blocks to fill the card); TAIL: K is not a multiple of 8
+template <int T, int U, bool TAIL> __global__ __launch_bounds__(256) void quantize_f8_rows_kernel(const QuantF8Args a) {
+  const int j = threadIdx.x & 15;
+  const uint32_t b0 = blockIdx.x * (16 * U) + (threadIdx.x >> 4), blocks = (uint32_t)a.blocks;
+  float v[U][8];
+  uint32_t r[U];
+  int kb[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t b = min(b0 + 16 * u, blocks - 1);                // (past the last: done again, to the same bytes)
+    r[u] = f8_divide(b, a.kb_magic, a.kb_shift);
+    kb[u] = (int)(b - r[u] * (uint32_t)a.Kb);
+    const uint32_t bt = f8_divide(r[u], a.r_magic, a.r_shift);
+    const f8_type<T>* row = (const f8_type<T>*)a.x + bt * a.x_bs + (int64_t)(r[u] - bt * (uint32_t)a.R) * a.x_rs;
+    const int col = kb[u] * 128 + j * 8;
+    if constexpr (TAIL) f8_load8<T>(row, col, a.K, v[u]);
+    else {
+      f8_type<T> t[8] = {};
+      if (col < a.K) __builtin_memcpy(t, row + col, sizeof(t));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[u][i] = f8_load<T>(t[i]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int e = f8_exponent(f8_max16(f8_max8(v[u])));
+    *(f8_v2i*)(a.q + (int64_t)r[u] * ((int64_t)a.Kb * 128) + kb[u] * 128 + j * 8) = f8_scale8(v[u], f8_pow2(-e));
+    if (j == 0) f8_put_exponent(a.e + (int64_t)r[u] * a.Sp, kb[u], a.Kb, a.Sp, e);
+  }
 }
 
 template <int T> __global__ __launch_bounds__(256) void quantize_f8_blocks_kernel(const QuantF8Args a) {
@@ -114,11 +138,39 @@ template <int T> __global__ __launch_bounds__(256) void quantize_f8_blocks_kerne
   if (threadIdx.x == 0) f8_put_exponent(a.e + br * a.Sp, kb, a.Kb, a.Sp, e);
 }
 
-template <int T> int launch_quantize(const QuantF8Args& a, int block_rows, hipStream_t st) {
-  const int64_t grid = block_rows == 1 ? (a.blocks + 15) / 16 : a.blocks;
-  if (grid > 0x7fffffff) return f8_fail("qbnn_quantize_f8: too many blocks (%ld)", (long)a.blocks);
-  if (block_rows == 1) hipLaunchKernelGGL((quantize_f8_rows_kernel<T>), dim3((unsigned)grid), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((quantize_f8_blocks_kernel<T>), dim3((unsigned)grid), dim3(256), 0, st, a);
+template <int T> int launch_quantize_rows(QuantF8Args a, int64_t batch, hipStream_t st) {
+  if (a.x_bs == a.R * a.x_rs && batch * a.R < ((int64_t)1 << 31)) { a.R = (int)(batch * a.R); batch = 1; }      // one matrix
+  f8_magic((uint32_t)a.Kb, a.kb_magic, a.kb_shift);
+  // launches of fewer than 2^31 blocks and rows
+  const int64_t rows = batch * a.R, most = ((int64_t)1 << 30) / a.Kb;
+  const int64_t step = rows <= most ? rows : batch == 1 ? most : (most / a.R ? most / a.R * a.R : 0);
+  if (step == 0) return f8_fail("qbnn_quantize_f8: a matrix of %ld blocks in a batch", (long)((int64_t)a.R * a.Kb));
+  f8_magic((uint32_t)(batch == 1 ? (step < a.R ? step : a.R) : a.R), a.r_magic, a.r_shift);
+  for (int64_t r0 = 0; r0 < rows; r0 += step) {
+    QuantF8Args c = a;
+    const int64_t n = rows - r0 < step ? rows - r0 : step;
+    c.blocks = n * a.Kb;
+    c.x = (const char*)a.x + (batch == 1 ? r0 * a.x_rs : r0 / a.R * a.x_bs) * (int64_t)sizeof(f8_type<T>);
+    if (batch == 1) { c.R = (int)n; f8_magic((uint32_t)n, c.r_magic, c.r_shift); }
+    c.q = a.q + r0 * ((int64_t)a.Kb * 128);
+    c.e = a.e + r0 * a.Sp;
+    const bool many = c.blocks >= 65536;
+    const dim3 grid((unsigned)((c.blocks + (many ? 63 : 15)) / (many ? 64 : 16)));
+    if (a.K % 8) {
+      if (many) hipLaunchKernelGGL((quantize_f8_rows_kernel<T, 4, true>), grid, dim3(256), 0, st, c);
+      else hipLaunchKernelGGL((quantize_f8_rows_kernel<T, 1, true>), grid, dim3(256), 0, st, c);
+    } else {
+      if (many) hipLaunchKernelGGL((quantize_f8_rows_kernel<T, 4, false>), grid, dim3(256), 0, st, c);
+      else hipLaunchKernelGGL((quantize_f8_rows_kernel<T, 1, false>), grid, dim3(256), 0, st, c);
+    }
+    if (int rc = qbnn_check_launch_msg("qbnn_quantize_f8")) return rc;
+  }
+  return QBNN_OK;
+}
+template <int T> int launch_quantize(const QuantF8Args& a, int64_t batch, int block_rows, hipStream_t st) {
+  if (block_rows == 1) return launch_quantize_rows<T>(a, batch, st);
+  if (a.blocks > 0x7fffffff) return f8_fail("qbnn_quantize_f8: too many blocks (%ld)", (long)a.blocks);
+  hipLaunchKernelGGL((quantize_f8_blocks_kernel<T>), dim3((unsigned)a.blocks), dim3(256), 0, st, a);
   return qbnn_check_launch_msg("qbnn_quantize_f8");
 }
 
@@ -211,8 +263,9 @@ template <int OUT, bool GROUPED> __device__ __forceinline__ void f8_put4(const F
 }
 
 // Direct form: operands straight from memory into the matrix instruction's registers, the waves of a workgroup split the columns and
-// join their sums in LDS in a fixed order.  For few rows, where the weights are read once and nothing is used twice.
-template <int MT, int NT, int NW, int OUT, bool EXACT, bool GROUPED>
+// join their sums in LDS in a fixed order.  For few rows, where the weights are read once and nothing is used twice: what counts is bytes in flight, so a
+// wave asks for D blocks of columns (1, 2 or 4: one dword of exponents) before it multiplies the first.
+template <int MT, int NT, int NW, int D, int OUT, bool EXACT, bool GROUPED>
 __global__ __launch_bounds__(NW * 64) void linear_f8_direct_kernel(const F8Args a) {
   __shared__ __attribute__((aligned(16))) f8_v4f red[NW > 1 ? NW : 1][MT * NT * 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, h = lane >> 4;
@@ -223,51 +276,65 @@ __global__ __launch_bounds__(NW * 64) void linear_f8_direct_kernel(const F8Args 
   const uint8_t* xp[MT]; const uint8_t* xep[MT];
   const uint8_t* wp[NT]; const uint8_t* wep[NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int row = f8_x_row<GROUPED>(a, min(t.m0 + 16 * i + r16, t.m1 - 1));      // a row behind the last repeats it: its result is not stored
-    xp[i] = a.x + (int64_t)t.sample * a.x_ss + row * pitch + h * 16;
-    xep[i] = a.xe + (int64_t)t.sample * a.xe_ss + (int64_t)row * a.Sp;
-  }
-#pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int row = min(n0 + 16 * j + r16, a.N - 1);
     wp[j] = a.w + (int64_t)t.set * a.w_ss + row * pitch + h * 16;
     wep[j] = a.we + (int64_t)t.set * a.we_ss + (int64_t)(row >> 7) * a.Sp;
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int row = f8_x_row<GROUPED>(a, min(t.m0 + 16 * i + r16, t.m1 - 1));      // a row behind the last repeats it: its result is not stored
+    xp[i] = a.x + (int64_t)t.sample * a.x_ss + row * pitch + h * 16;
+    xep[i] = a.xe + (int64_t)t.sample * a.xe_ss + (int64_t)row * a.Sp;
   }
   f8_v4f acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = (f8_v4f){0.f, 0.f, 0.f, 0.f};
-  for (int kb = wave; kb < a.Kb; kb += NW) {
-    f8_v8i xf[MT], wf[NT];
-    int xs[MT], ws[NT];
+#pragma unroll 1
+  for (int k0 = wave * D; k0 < a.Kb; k0 += NW * D) {
+    f8_v8i xf[D][MT], wf[D][NT];
+    uint32_t xs[MT], ws[NT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      wf[j] = f8_join(*(const f8_v4i*)(wp[j] + kb * 128), *(const f8_v4i*)(wp[j] + kb * 128 + 64));
-      ws[j] = wep[j][kb];
+    for (int d = 0; d < D; ++d) {
+      const int at = min(k0 + d, a.Kb - 1) * 128;               // (past the last block: read again, not multiplied)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) wf[d][j] = f8_join(*(const f8_v4i*)(wp[j] + at), *(const f8_v4i*)(wp[j] + at + 64));
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      xf[i] = f8_join(*(const f8_v4i*)(xp[i] + kb * 128), *(const f8_v4i*)(xp[i] + kb * 128 + 64));
-      xs[i] = xep[i][kb];
+    for (int d = 0; d < D; ++d) {
+      const int at = min(k0 + d, a.Kb - 1) * 128;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xf[d][i] = f8_join(*(const f8_v4i*)(xp[i] + at), *(const f8_v4i*)(xp[i] + at + 64));
     }
-    if constexpr (EXACT) {
-      F8Wide xw[MT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) xw[i] = f8_widen(xf[i]);
+    for (int j = 0; j < NT; ++j) ws[j] = *(const uint32_t*)(wep[j] + (k0 & ~3)) >> ((k0 & 3) * 8);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const F8Wide ww = f8_widen(wf[j]);
+    for (int i = 0; i < MT; ++i) xs[i] = *(const uint32_t*)(xep[i] + (k0 & ~3)) >> ((k0 & 3) * 8);
+    auto multiply = [&](auto Dc) {
+      constexpr int d = decltype(Dc)::value;
+      if constexpr (EXACT) {
+        F8Wide xw[MT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i][j] = f8_mfma_exact(ww, xw[i], acc[i][j], ws[j], xs[i]);
+        for (int i = 0; i < MT; ++i) xw[i] = f8_widen(xf[d][i], xs[i] >> (8 * d));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const F8Wide ww = f8_widen(wf[d][j], ws[j] >> (8 * d));
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][j] = f8_mfma_exact(ww, xw[i], acc[i][j]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = f8_mfma<d>(wf[d][j], xf[d][i], acc[i][j], ws[j], xs[i]);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = f8_mfma(wf[j], xf[i], acc[i][j], ws[j], xs[i]);
-    }
+    };
+    multiply(std::integral_constant<int, 0>{});
+    if constexpr (D > 1) { if (k0 + 1 < a.Kb) multiply(std::integral_constant<int, 1>{}); }
+    if constexpr (D > 2) { if (k0 + 2 < a.Kb) multiply(std::integral_constant<int, 2>{}); }
+    if constexpr (D > 2) { if (k0 + 3 < a.Kb) multiply(std::integral_constant<int, 3>{}); }
   }
   if constexpr (OUT == QBNN_F8) {
     static_assert(NT == 8, "a block of an e4m3 result is 128 columns of a row");
@@ -327,9 +394,9 @@ __global__ __launch_bounds__(NW * 64) void linear_f8_direct_kernel(const F8Args 
   }
 }
 
-template <int MT, int NT, int NW, int OUT, bool EXACT, bool GROUPED> int launch_direct(const F8Args& a, int tiles, int z, hipStream_t st) {
+template <int MT, int NT, int NW, int D, int OUT, bool EXACT, bool GROUPED> int launch_direct(const F8Args& a, int tiles, int z, hipStream_t st) {
   if (tiles > 65535 || z > 65535) return f8_fail("qbnn_linear_f8: %ld row tiles x %ld samples do not fit a grid", tiles, z);
-  hipLaunchKernelGGL((linear_f8_direct_kernel<MT, NT, NW, OUT, EXACT, GROUPED>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)tiles, (unsigned)z),
+  hipLaunchKernelGGL((linear_f8_direct_kernel<MT, NT, NW, D, OUT, EXACT, GROUPED>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)tiles, (unsigned)z),
                      dim3(NW * 64), 0, st, a);
   return qbnn_check_launch_msg("qbnn_linear_f8");
 }
@@ -364,7 +431,7 @@ template <int TM, int TN, bool GROUPED> __device__ __forceinline__ bool f8_locat
 // Results of a wave's (32 G) x 128 tile from row m, weight row nw on, 32 rows at a time through `stage` (F8_STAGE bytes of LDS of this wave's own, no longer read
 // by anyone; put(i, st) writes rows 32 i .. + 31 there, F8_PITCH floats each): 16 lanes then write 128 neighbouring columns of a row.  Stored from the
 // accumulators' layout they were 32 bytes of each of 32 rows per instruction, and with the bounds unrolled 30 KiB of code: 27,000 cycles a tile, as much as 11 steps.
-constexpr int F8_PITCH = 132, F8_STAGE = 32 * F8_PITCH * 4;
+constexpr int F8_PITCH = 132, F8_STAGE = 32 * F8_PITCH * 4 + 128 * 8;
 __device__ __forceinline__ float f8_relu(float u) { return u < 0.f ? 0.f : u; }      // (a NaN stays one)
 template <int G, int OUT, bool GROUPED, bool WHOLE, class Put>
 __device__ __forceinline__ void f8_finish_as(const F8Args& a, const F8Tile& t, int m, int nw, uint8_t* stage, Put put) {
@@ -379,6 +446,16 @@ __device__ __forceinline__ void f8_finish_as(const F8Args& a, const F8Tile& t, i
       for (int c = 0; c < 8; ++c) b[c] = c < in ? bias[c] : 0.f;
   }
   float* st = (float*)stage;
+  // where the wave's rows go and their weights: fetched once, side by side (row by row in the loop below, two dependent loads were 1,500 cycles each time)
+  int* const to_row = (int*)(stage + 32 * F8_PITCH * 4);
+  float* const to_weight = (float*)(to_row + 32 * G);
+  const bool moved = GROUPED && OUT != QBNN_F8 && a.y_rows;
+  if (moved)
+    for (int r = lane; r < 32 * G; r += 64) {
+      const int to = a.y_rows[min(m + r, t.m1 - 1)];
+      to_row[r] = to;
+      to_weight[r] = a.scale[to];
+    }
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     put(i, st);
@@ -407,9 +484,9 @@ __device__ __forceinline__ void f8_finish_as(const F8Args& a, const F8Tile& t, i
           }
         } else if (row < t.m1) {
           int64_t to = row;
-          if (GROUPED && a.y_rows) {
-            to = a.y_rows[row];
-            const float s = a.scale[to];
+          if (moved) {
+            to = to_row[i * 32 + r];
+            const float s = to_weight[i * 32 + r];
 #pragma unroll
             for (int c = 0; c < 8; ++c) v[c] = s == 0.f ? 0.f : v[c] * s;
           }
@@ -593,31 +670,27 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
         ws.arrive();
       }
       const int byte = (kb & 1) * 8;
-      F8Wide xw[MI][2];
+      F8Wide xw[MI][2], ww[4][2];
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const Frag f = read_x(buf, i);
-        xw[i][0] = f8_widen(f.k[0]);
-        xw[i][1] = f8_widen(f.k[1]);
+        xw[i][0] = f8_widen(f.k[0], xs[i].d[0] >> byte);
+        xw[i][1] = f8_widen(f.k[1], xs[i].d[0] >> byte);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const Frag f = read_w(buf, j);
-        const F8Wide ww[2] = {f8_widen(f.k[0]), f8_widen(f.k[1])};
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          f8_v16f c;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) c[k] = 0.f;
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ww[s].part[g], xw[i][s].part[g], c, 0, 0, 0);
-          const int e = (int)((ws.d[0] >> byte) & 255) + (int)((xs[i].d[0] >> byte) & 255) - 254;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) acc[i][j][k] += __builtin_ldexpf(c[k], e);
-        }
+        ww[j][0] = f8_widen(f.k[0], ws.d[0] >> byte);
+        ww[j][1] = f8_widen(f.k[1], ws.d[0] >> byte);
       }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < MI; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ww[j][s].part[g], xw[i][s].part[g], acc[i][j], 0, 0, 0);
       if (kb & 1) {
 #pragma unroll
         for (int i = 0; i < MI; ++i) xs[i].down();
@@ -809,18 +882,23 @@ template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, 
   // offsets are 32 bits wide in the tiled form: of a gathered row's bytes from the first, of any row's exponents, of a weight row's in its tile
   const int64_t far = GROUPED ? (int64_t)(a.rows ? a.x_rows : rows) * a.Kb * 128 : (int64_t)rows * a.Sp;
   const bool near = far < ((int64_t)1 << 32) && a.Kb < (1 << 16);
-  if (per > 64 && near) {
+  const auto tiles = [&](int tm, int tn) { return (int64_t)z * ((rows + tm - 1) / tm + spare / 2) * ((a.N + tn - 1) / tn); };
+  if (per > 32 && near) {
     if constexpr (!EXACT) {
-      if (per >= 192) return launch_big<OUT, GROUPED>(a, rows, z, st);
+      if (per > 128 && tiles(256, 256) >= 192) return launch_big<OUT, GROUPED>(a, rows, z, st);
     }
-    return launch_tiled<2, 2, 2, OUT, EXACT, GROUPED>(a, rows, z, st);
+    if (per > 64 && tiles(128, 256) >= 384) return launch_tiled<2, 2, 2, OUT, EXACT, GROUPED>(a, rows, z, st);
+    return launch_tiled<1, 2, 1, OUT, EXACT, GROUPED>(a, rows, z, st);
   }
   if constexpr (OUT == QBNN_F8) {
-    if (per <= 16) return launch_direct<1, 8, 4, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
-    return launch_direct<2, 8, 4, OUT, EXACT, GROUPED>(a, (rows + 31) / 32 + spare, z, st);
+    if (per <= 16) return launch_direct<1, 8, 4, 2, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
+    return launch_direct<2, 8, 4, 1, OUT, EXACT, GROUPED>(a, (rows + 31) / 32 + spare, z, st);
   } else {
-    if (per <= 16) return launch_direct<1, 1, 8, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
-    return launch_direct<4, 4, 4, OUT, EXACT, GROUPED>(a, (rows + 63) / 64 + spare, z, st);
+    if (per <= 16) {
+      if (GROUPED) return launch_direct<1, 4, 4, 2, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
+      return launch_direct<1, 1, 8, 4, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
+    }
+    return launch_direct<2, 4, 4, 2, OUT, EXACT, GROUPED>(a, (rows + 31) / 32 + spare, z, st);
   }
 }
 template <bool GROUPED> int launch_linear_any(const F8Args& a, int rows, int z, int y_type, int exact, hipStream_t st) {
@@ -867,9 +945,9 @@ QBNN_EXPORT int qbnn_quantize_f8(const void* x, int32_t x_type, int64_t x_batch_
   a.R = R; a.K = K; a.Kb = (K + 127) / 128; a.Sp = (a.Kb + 3) / 4 * 4;
   a.blocks = batch * (block_rows == 1 ? R : (R + 127) / 128) * a.Kb;
   switch (x_type) {
-    case QBNN_F32: return launch_quantize<QBNN_F32>(a, block_rows, (hipStream_t)stream);
-    case QBNN_BF16: return launch_quantize<QBNN_BF16>(a, block_rows, (hipStream_t)stream);
-    default: return launch_quantize<QBNN_F16>(a, block_rows, (hipStream_t)stream);
+    case QBNN_F32: return launch_quantize<QBNN_F32>(a, batch, block_rows, (hipStream_t)stream);
+    case QBNN_BF16: return launch_quantize<QBNN_BF16>(a, batch, block_rows, (hipStream_t)stream);
+    default: return launch_quantize<QBNN_F16>(a, batch, block_rows, (hipStream_t)stream);
   }
 }
 
