@@ -415,17 +415,20 @@ template <int MI, int WM, int WN> struct F8Tiled {
 };
 typedef float f8_v16f __attribute__((ext_vector_type(16)));
 
-// Workgroups of one XCD (every eighth) take neighbouring tiles, in columns of 4 row tiles: what they read at a time shares its L2.  false: no tile.
-template <int TM, int TN, bool GROUPED> __device__ __forceinline__ bool f8_locate(const F8Args& a, int tiles_m, int tiles_n, F8Tile& t, int& n0) {
-  const int tm = GROUPED ? f8_count_tiles<TM>(a) : tiles_m, total = tm * tiles_n;
+// Workgroups of one XCD (every eighth) take neighbouring tiles, in columns of 4 row tiles, sample after sample: what they read at a time shares its L2.
+// false: no tile.
+template <int TM, int TN, bool GROUPED> __device__ __forceinline__ bool f8_locate(const F8Args& a, int tiles_m, int tiles_n, int samples, F8Tile& t, int& n0) {
+  const int tm = GROUPED ? f8_count_tiles<TM>(a) : tiles_m, each = tm * tiles_n, total = each * samples;
   const int p = blockIdx.x;
   if (p >= total) return false;
   const int per = total >> 3, rest = total & 7, xcd = p & 7;
-  const int q = xcd * per + min(xcd, rest) + (p >> 3);
+  int q = xcd * per + min(xcd, rest) + (p >> 3);
+  const int z = GROUPED ? 0 : q / each;
+  q -= z * each;
   const int band = q / (4 * tiles_n), in = q - band * (4 * tiles_n), rows = min(4, tm - band * 4);
   const int col = in / rows;
   n0 = col * TN;
-  return f8_find_tile<TM, GROUPED>(a, band * 4 + in - col * rows, blockIdx.z, t);
+  return f8_find_tile<TM, GROUPED>(a, band * 4 + in - col * rows, z, t);
 }
 
 // Results of a wave's (32 G) x 128 tile from row m, weight row nw on, 32 rows at a time through `stage` (F8_STAGE bytes of LDS of this wave's own, no longer read
@@ -460,7 +463,7 @@ __device__ __forceinline__ void f8_finish_as(const F8Args& a, const F8Tile& t, i
   for (int i = 0; i < G; ++i) {
     put(i, st);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // (the wave's own LDS: no barrier)
-    constexpr int AT_ONCE = WHOLE ? 4 : 1;
+    constexpr int AT_ONCE = WHOLE ? 4 : 2;
 #pragma unroll 1
     for (int p0 = 0; p0 < 8; p0 += AT_ONCE)
 #pragma unroll
@@ -491,9 +494,11 @@ __device__ __forceinline__ void f8_finish_as(const F8Args& a, const F8Tile& t, i
             for (int c = 0; c < 8; ++c) v[c] = s == 0.f ? 0.f : v[c] * s;
           }
           f8_type<OUT>* y = (f8_type<OUT>*)a.y + (int64_t)t.sample * a.y_ss + to * a.y_rs + nw + n;
-          if constexpr (!WHOLE) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) if (c < in) y[c] = f8_store<OUT>(v[c]);
+          if (!WHOLE && in < 8) {                               // the lane at the end: its values by way of the stage, one by one
+            *(f8_v4f*)(st + r * F8_PITCH + n) = (f8_v4f){v[0], v[1], v[2], v[3]};
+            *(f8_v4f*)(st + r * F8_PITCH + n + 4) = (f8_v4f){v[4], v[5], v[6], v[7]};
+#pragma unroll 1
+            for (int c = 0; c < in; ++c) y[c] = f8_store<OUT>(st[r * F8_PITCH + n + c]);
           } else if constexpr (OUT == QBNN_F32) {
             __builtin_memcpy(y, v, sizeof(v));
           } else {
@@ -533,7 +538,7 @@ struct F8Exponents {
 };
 
 template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED>
-__global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const F8Args a, int tiles_m, int tiles_n) {
+__global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const F8Args a, int tiles_m, int tiles_n, int samples) {
   using C = F8Tiled<MI, WM, WN>;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, h = lane >> 5;
@@ -541,7 +546,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
 
   F8Tile t;
   int n0;
-  if (!f8_locate<C::TM, C::TN, GROUPED>(a, tiles_m, tiles_n, t, n0)) return;
+  if (!f8_locate<C::TM, C::TN, GROUPED>(a, tiles_m, tiles_n, samples, t, n0)) return;
   const int64_t pitch = (int64_t)a.Kb * 128;
   const uint8_t* xg = a.x + (int64_t)t.sample * a.x_ss;
   const uint8_t* wg = a.w + (int64_t)t.set * a.w_ss + n0 * pitch;
@@ -719,9 +724,8 @@ template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED> int launch_
   static std::atomic<uint64_t> attr{0};
   if (int rc = qbnn_ensure_dyn_lds((const void*)linear_f8_tiled_kernel<MI, WM, WN, OUT, EXACT, GROUPED>, &attr, C::LDS)) return rc;
   const int64_t tm = (rows + C::TM - 1) / C::TM + (GROUPED ? a.groups : 0), tn = (a.N + C::TN - 1) / C::TN;
-  if (tm * tn > 0x7fffffff || z > 65535) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
-  hipLaunchKernelGGL((linear_f8_tiled_kernel<MI, WM, WN, OUT, EXACT, GROUPED>), dim3((unsigned)(tm * tn), 1, (unsigned)z), dim3(C::WAVES * 64), C::LDS, st, a,
-                     (int)tm, (int)tn);
+  if (tm * tn * z > 0x7fffffff) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
+  hipLaunchKernelGGL((linear_f8_tiled_kernel<MI, WM, WN, OUT, EXACT, GROUPED>), dim3((unsigned)(tm * tn * z)), dim3(C::WAVES * 64), C::LDS, st, a, (int)tm, (int)tn, z);
   return qbnn_check_launch_msg("qbnn_linear_f8");
 }
 
@@ -744,14 +748,14 @@ template <int B> __device__ __forceinline__ void f8_mfma_in_place(f8_v4f& acc, c
 constexpr int F8_BIG_LDS = 131072 + 2 * 2048;      // two steps of x and w, two sets of exponents (1 KiB of x, 256 bytes for each wave of w)
 
 template <int OUT, bool GROUPED>
-__global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, int tiles_m, int tiles_n) {
+__global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, int tiles_m, int tiles_n, int samples) {
   constexpr int W0 = 65536, E0 = 131072;             // x at 0 and 32768, w at W0 and W0 + 32768, exponents at E0 and E0 + 2048
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, h = lane >> 4;
   const int wm = wave >> 1, wn = wave & 1;
   F8Tile t;
   int n0;
-  if (!f8_locate<256, 256, GROUPED>(a, tiles_m, tiles_n, t, n0)) return;
+  if (!f8_locate<256, 256, GROUPED>(a, tiles_m, tiles_n, samples, t, n0)) return;
   const int64_t pitch = (int64_t)a.Kb * 128;
   const uint8_t* xg = a.x + (int64_t)t.sample * a.x_ss;
   const uint8_t* wg = a.w + (int64_t)t.set * a.w_ss + n0 * pitch;
@@ -870,8 +874,8 @@ template <int OUT, bool GROUPED> int launch_big(const F8Args& a, int rows, int z
   static std::atomic<uint64_t> attr{0};
   if (int rc = qbnn_ensure_dyn_lds((const void*)linear_f8_big_kernel<OUT, GROUPED>, &attr, F8_BIG_LDS)) return rc;
   const int64_t tm = (rows + 255) / 256 + (GROUPED ? a.groups : 0), tn = (a.N + 255) / 256;
-  if (tm * tn > 0x7fffffff || z > 65535) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
-  hipLaunchKernelGGL((linear_f8_big_kernel<OUT, GROUPED>), dim3((unsigned)(tm * tn), 1, (unsigned)z), dim3(256), F8_BIG_LDS, st, a, (int)tm, (int)tn);
+  if (tm * tn * z > 0x7fffffff) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
+  hipLaunchKernelGGL((linear_f8_big_kernel<OUT, GROUPED>), dim3((unsigned)(tm * tn * z)), dim3(256), F8_BIG_LDS, st, a, (int)tm, (int)tn, z);
   return qbnn_check_launch_msg("qbnn_linear_f8");
 }
 
