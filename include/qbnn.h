@@ -648,31 +648,21 @@ int qbnn_regression_metrics(const float* mean, const float* var, const float* ta
 int qbnn_quantize_f8(const void* x, int32_t x_type, int64_t x_batch_stride, int64_t x_row_stride, int64_t batch, int32_t R, int32_t K,
                      int32_t block_rows, uint8_t* q, uint8_t* exponents, void* stream);
 
-/* y[s][m][n] = act( sum_k x[s][m][k] w[s][n][k] + bias[s][n] ).  exact (fp32 and e4m3 results): products and sums in fp32, at half the
- * matrix rate; without it the e4m3 matrix instruction, which cuts the products of 8 neighbouring columns off 2^-13 below the largest of them
+/* y[s][m][n] = act( sum_k x[s][m][k] w[s][n][k] + bias[s][n] ).  For fp32 results products and sums in fp32 ("exact"), at half the
+ * matrix rate; for the others the e4m3 matrix instruction, which cuts the products of 8 neighbouring columns off 2^-13 below the largest of them
  * before it adds them, and sums in fp32 from there (1.3e-5 of the result's norm on normal data).  x: block_rows 1, w: block_rows 128.  Strides
  * per sample in bytes for the operands (0 = shared by the samples), in elements for the bias; y [n_samples][M][N] dense, or for QBNN_F8 in
  * the operand format (y_exp, block_rows 1).  Replaces the fp32 / int8 product of a stochastic Linear (bbb/linear.py:42-50). */
 typedef struct qbnn_f8_linear {
-  const uint8_t* x; const uint8_t* x_exp; int64_t x_ss, x_exp_ss;
+  const void* x_float; int64_t x_float_ss, x_float_rs;   /* != NULL: float rows (strides in elements) that are quantised into x / x_exp first */
+  uint8_t* x; uint8_t* x_exp; int64_t x_ss, x_exp_ss;
   const uint8_t* w; const uint8_t* w_exp; int64_t w_ss, w_exp_ss;
   const float* bias; int64_t bias_ss;
   void* y; uint8_t* y_exp;
-  int32_t M, N, K, n_samples, relu, y_type, exact;
+  int32_t M, N, K, n_samples, relu, y_type, x_type;
 } qbnn_f8_linear;
 
 int qbnn_linear_f8_mc(const qbnn_f8_linear* host_desc, void* stream);
-
-/* The same over ragged groups of rows: rows offsets[g] .. offsets[g + 1] - 1 (device, ascending, offsets[groups] <= M) take weight set and bias
- * g % w_groups (strides w_ss, w_exp_ss, bias_ss).  x_rows != NULL: row i reads x row (x_rows[i] / topk) % x_row_count.  y_rows != NULL: row i's
- * result goes to y row y_rows[i], times y_weights[y_rows[i]] (0 where that weight is 0).  Rows behind the last group are neither read nor written. */
-typedef struct qbnn_f8_routed {
-  const int32_t* offsets; int32_t groups, w_groups;
-  const int32_t* x_rows; int32_t topk, x_row_count;
-  const int32_t* y_rows; const float* y_weights;
-} qbnn_f8_routed;
-
-int qbnn_linear_f8_routed(const qbnn_f8_linear* host_desc, const qbnn_f8_routed* host_routed, void* stream);
 
 #define QBNN_ROUTE_MAX_EXPERTS 1024
 #define QBNN_ROUTE_MAX_CHOICES 32
@@ -694,8 +684,24 @@ typedef struct qbnn_route {
 int64_t qbnn_route_workspace_ints(int32_t S, int32_t T, int32_t E);
 int qbnn_route_experts(const qbnn_route* host_desc, void* stream);
 
-/* y[t][n] = sum_j o[t * top_k + j][n], in the order of j, rounded once to y_type. */
-int qbnn_combine_routed(const float* o, int32_t rows, int32_t top_k, int32_t N, void* y, int32_t y_type, void* stream);
+/* Two linear layers of E experts with a ReLU between, over the rows that the router sent to each:
+ *   y[s][t] = sum_j weights[s][t][j] ( relu(x[s][t] w_up[e]^T + b_up[e]) w_down[e]^T + b_down[e] ),  e = experts[s][t][j]
+ * offsets / rows / weights: of qbnn_route_experts with the same S, T, E, top_k.  x [S or 1][T][D] (x_rows = S T or T; float: quantised into x / x_exp
+ * first), w_up [S or 1][E][H][D], w_down [S or 1][E][N][H] (block_rows 128; strides per expert in bytes, up_sets / down_sets = E or S E), biases fp32 (strides per
+ * expert in elements).  Hidden rows are quantised in blocks of 128; exact: bit 0 the first product, bit 1 the second (see qbnn_f8_linear); a result whose weight
+ * is 0 is left out, whatever it is.  The weighted results are fp32 and summed in the order of j, rounded once to y_type (QBNN_F32 .. QBNN_F16).
+ * Workspaces: h [S T top_k][Hp], h_exp [S T top_k][Hs] (Hp, Hs of H columns), o fp32 [S T top_k][N]. */
+typedef struct qbnn_f8_experts {
+  const void* x_float; int64_t x_float_ss, x_float_rs;
+  uint8_t* x; uint8_t* x_exp;
+  const int32_t* offsets; const int32_t* rows; const float* weights;
+  const uint8_t* w_up; const uint8_t* up_exp; int64_t up_ss, up_exp_ss; const float* b_up; int64_t b_up_ss;
+  const uint8_t* w_down; const uint8_t* down_exp; int64_t down_ss, down_exp_ss; const float* b_down; int64_t b_down_ss;
+  uint8_t* h; uint8_t* h_exp; float* o; void* y;
+  int32_t S, T, E, top_k, x_rows, D, H, N, up_sets, down_sets, exact, x_type, y_type;
+} qbnn_f8_experts;
+
+int qbnn_experts_f8(const qbnn_f8_experts* host_desc, void* stream);
 
 const char* qbnn_last_error(void);
 int qbnn_version(void);

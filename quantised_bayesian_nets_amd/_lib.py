@@ -3,6 +3,7 @@
 The product path has NO CPU fallback: if the library is missing or a call fails, this raises."""
 import ctypes as C
 import os
+import struct
 
 from . import build as _build
 
@@ -108,26 +109,10 @@ class HeadCall(C.Structure):
                 ("probs", C.c_void_p), ("n_samples", C.c_int32), ("desc", C.POINTER(HeadDesc))]
 
 
-class F8Linear(C.Structure):
-    """qbnn_f8_linear (include/qbnn.h)."""
-    _fields_ = [("x", C.c_void_p), ("x_exp", C.c_void_p), ("x_ss", C.c_int64), ("x_exp_ss", C.c_int64),
-                ("w", C.c_void_p), ("w_exp", C.c_void_p), ("w_ss", C.c_int64), ("w_exp_ss", C.c_int64),
-                ("bias", C.c_void_p), ("bias_ss", C.c_int64), ("y", C.c_void_p), ("y_exp", C.c_void_p),
-                ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("n_samples", C.c_int32), ("relu", C.c_int32), ("y_type", C.c_int32), ("exact", C.c_int32)]
-
-
-class F8Routed(C.Structure):
-    """qbnn_f8_routed (include/qbnn.h)."""
-    _fields_ = [("offsets", C.c_void_p), ("groups", C.c_int32), ("w_groups", C.c_int32), ("x_rows", C.c_void_p), ("topk", C.c_int32),
-                ("x_row_count", C.c_int32), ("y_rows", C.c_void_p), ("y_weights", C.c_void_p)]
-
-
-class Route(C.Structure):
-    """qbnn_route (include/qbnn.h)."""
-    _fields_ = [("logits", C.c_void_p), ("logits_ss", C.c_int64), ("logits_rs", C.c_int64), ("bias", C.c_void_p), ("weights", C.c_void_p),
-                ("experts", C.c_void_p), ("offsets", C.c_void_p), ("rows", C.c_void_p), ("workspace", C.c_void_p),
-                ("S", C.c_int32), ("T", C.c_int32), ("E", C.c_int32), ("top_k", C.c_int32), ("groups", C.c_int32), ("top_groups", C.c_int32),
-                ("sigmoid", C.c_int32), ("renormalize", C.c_int32), ("type", C.c_int32), ("scale", C.c_float)]
+# Descriptors that a call fills field by field are packed at once (a ctypes field costs 0.1 us): the C structs' fields in order, native alignment.
+F8_LINEAR = struct.Struct("@Pqq PPqq PPqq Pq PP 7i")               # qbnn_f8_linear
+F8_EXPERTS = struct.Struct("@Pqq PP PPP PPqqPq PPqqPq PPPP 13i")   # qbnn_f8_experts
+ROUTE = struct.Struct("@Pqq P PPPPP 9i f")                         # qbnn_route
 
 
 EXPORTS = ["qbnn_mlp_bbb_f32_mc", "qbnn_mlp_bbb_f32_workspace_floats", "qbnn_packed_weight_bytes", "qbnn_pack_weights_host", "qbnn_sample_weights_i8", "qbnn_sample_weights_i8_multi", "qbnn_set_device_noise_source", "qbnn_conv2d_i8_mc", "qbnn_conv2d_i8_post_mc", "qbnn_conv_pool_drop_i8_mc", "qbnn_linear_i8_mc", "qbnn_im2col5x5_c1", "qbnn_conv_c1_pool_i8_mc",
@@ -136,7 +121,7 @@ EXPORTS = ["qbnn_mlp_bbb_f32_mc", "qbnn_mlp_bbb_f32_workspace_floats", "qbnn_pac
            "qbnn_dequant_softmax_mc", "qbnn_flatten_nchw_mc", "qbnn_flatten_nchw_rows_mc", "qbnn_add_relu_q_mc", "qbnn_sample_weights_f32", "qbnn_linear_f32_mc", "qbnn_head_i8_mc", "qbnn_reduce_moments", "qbnn_finalize_moments", "qbnn_classification_metrics", "qbnn_regression_metrics",
            "qbnn_conv2d_f32_mc", "qbnn_conv2d_f32_fused_mc", "qbnn_conv2d_f32_blocks", "qbnn_observe_partials_f32_mc", "qbnn_grid_to_i8_mc", "qbnn_fake_quant_ex_f32_mc", "qbnn_conv2d_q8_blocks", "qbnn_conv2d_q8_f32_mc", "qbnn_add_q8_blocks", "qbnn_add_q8_f32_mc", "qbnn_fake_quant_add_q8_mc", "qbnn_qat_weights_mc", "qbnn_sample_weights_f32_batch", "qbnn_affine_f32_mc", "qbnn_pool2d_f32_mc", "qbnn_flatten_nchw_f32_mc", "qbnn_softmax_f32_mc", "qbnn_observe_f32_mc", "qbnn_fake_quant_f32_mc", "qbnn_sample_weights_f32_strided", "qbnn_sample_weights_f32_ohwi",
            "qbnn_dropout_mask_f32_mc", "qbnn_dropout_f32_mc", "qbnn_conv2d_f32_drop_mc",
-           "qbnn_quantize_f8", "qbnn_linear_f8_mc", "qbnn_linear_f8_routed", "qbnn_route_workspace_ints", "qbnn_route_experts", "qbnn_combine_routed",
+           "qbnn_quantize_f8", "qbnn_linear_f8_mc", "qbnn_experts_f8", "qbnn_route_workspace_ints", "qbnn_route_experts",
            "qbnn_last_error", "qbnn_version"]
 
 
@@ -240,12 +225,11 @@ def lib():
         L.qbnn_dropout_f32_mc.argtypes = [vp, i64, vp, i32, i32, i32, f, vp, i64, i32, vp, i64, i32, vp]
         L.qbnn_conv2d_f32_drop_mc.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, f, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, vp]
         L.qbnn_quantize_f8.argtypes = [vp, i32, i64, i64, i64, i32, i32, i32, vp, vp, vp]
-        L.qbnn_linear_f8_mc.argtypes = [C.POINTER(F8Linear), vp]
-        L.qbnn_linear_f8_routed.argtypes = [C.POINTER(F8Linear), C.POINTER(F8Routed), vp]
+        L.qbnn_linear_f8_mc.argtypes = [C.c_char_p, vp]
+        L.qbnn_experts_f8.argtypes = [C.c_char_p, vp]
         L.qbnn_route_workspace_ints.argtypes = [i32, i32, i32]
         L.qbnn_route_workspace_ints.restype = i64
-        L.qbnn_route_experts.argtypes = [C.POINTER(Route), vp]
-        L.qbnn_combine_routed.argtypes = [vp, i32, i32, i32, vp, i32, vp]
+        L.qbnn_route_experts.argtypes = [C.c_char_p, vp]
         _LIB = L
     return _LIB
 

@@ -905,72 +905,140 @@ template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, 
     return launch_direct<2, 4, 4, 2, OUT, EXACT, GROUPED>(a, (rows + 31) / 32 + spare, z, st);
   }
 }
+// what the two entries ask for: every type for dense rows (fp32 exact), e4m3 and fp32 of either form for groups
 template <bool GROUPED> int launch_linear_any(const F8Args& a, int rows, int z, int y_type, int exact, hipStream_t st) {
   switch (y_type) {
-    case QBNN_F32: return exact ? launch_linear<QBNN_F32, true, GROUPED>(a, rows, z, st) : launch_linear<QBNN_F32, false, GROUPED>(a, rows, z, st);
-    case QBNN_BF16: return launch_linear<QBNN_BF16, false, GROUPED>(a, rows, z, st);
-    case QBNN_F16: return launch_linear<QBNN_F16, false, GROUPED>(a, rows, z, st);
-    default: return exact ? launch_linear<QBNN_F8, true, GROUPED>(a, rows, z, st) : launch_linear<QBNN_F8, false, GROUPED>(a, rows, z, st);
+    case QBNN_F32: if constexpr (!GROUPED) return launch_linear<QBNN_F32, true, GROUPED>(a, rows, z, st);
+      else return exact ? launch_linear<QBNN_F32, true, GROUPED>(a, rows, z, st) : launch_linear<QBNN_F32, false, GROUPED>(a, rows, z, st);
+    case QBNN_BF16: if constexpr (!GROUPED) return launch_linear<QBNN_BF16, false, GROUPED>(a, rows, z, st);
+    case QBNN_F16: if constexpr (!GROUPED) return launch_linear<QBNN_F16, false, GROUPED>(a, rows, z, st);
+    default:
+      if constexpr (GROUPED) { if (exact) return launch_linear<QBNN_F8, true, GROUPED>(a, rows, z, st); }
+      return launch_linear<QBNN_F8, false, GROUPED>(a, rows, z, st);
   }
 }
 
-int fill_args(F8Args& a, const qbnn_f8_linear* d) {
-  if (!d || !d->x || !d->x_exp || !d->w || !d->w_exp || !d->y || d->N <= 0 || d->K <= 0 || d->M < 0 || d->n_samples < 0 || d->y_type < QBNN_F32 || d->y_type > QBNN_F8 ||
-      (d->y_type == QBNN_F8 && !d->y_exp) || d->x_ss < 0 || d->w_ss < 0 ||
-      (d->exact && d->y_type != QBNN_F32 && d->y_type != QBNN_F8))
-    return f8_fail("qbnn_linear_f8: bad argument");
-  const uintptr_t low = (uintptr_t)d->x | (uintptr_t)d->w | (uintptr_t)d->x_ss | (uintptr_t)d->w_ss | (d->y_type == QBNN_F8 ? (uintptr_t)d->y : 0);
-  const uintptr_t low4 = (uintptr_t)d->x_exp | (uintptr_t)d->w_exp | (uintptr_t)d->x_exp_ss | (uintptr_t)d->w_exp_ss;
-  if ((low & 15) || (low4 & 3)) return f8_fail("qbnn_linear_f8: e4m3 operands start at multiples of 16 bytes, exponents of 4");
-  a = F8Args{};
-  a.Kb = (int)(((int64_t)d->K + 127) / 128);
+// ---- y[t] = sum over the row's top_k results, in the order of choice --------------------------------------------------------------
+// The results come in fp32: rounded to 16 bits first, each would cost as much as the one rounding of the sum does.
+template <int T> __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ o, f8_type<T>* __restrict__ y, int rows, int k, int N) {
+  const int n0 = (blockIdx.x * 256 + threadIdx.x) * 4;
+  const int64_t t = blockIdx.y + (int64_t)blockIdx.z * 32768;
+  if (n0 >= N || t >= rows) return;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  const bool whole = n0 + 4 <= N;
+  for (int j = 0; j < k; ++j) {
+    const float* r = o + (t * k + j) * N + n0;
+    float v[4];
+    if (whole) __builtin_memcpy(v, r, sizeof(v));
+    else
+      for (int i = 0; i < 4; ++i) v[i] = n0 + i < N ? r[i] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += v[i];
+  }
+  f8_type<T> v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = f8_store<T>(sum[i]);
+  f8_type<T>* out = y + t * N + n0;
+  if (whole) __builtin_memcpy(out, v, sizeof(v));
+  else
+    for (int i = 0; i < 4; ++i) if (n0 + i < N) out[i] = v[i];
+}
+
+int launch_combine(const float* o, int rows, int k, int N, void* y, int y_type, hipStream_t st) {
+  const dim3 grid((unsigned)((N + 1023) / 1024), (unsigned)(rows < 32768 ? rows : 32768), (unsigned)((rows + 32767) / 32768));
+  switch (y_type) {
+    case QBNN_F32: hipLaunchKernelGGL((combine_kernel<QBNN_F32>), grid, dim3(256), 0, st, o, (float*)y, rows, k, N); break;
+    case QBNN_BF16: hipLaunchKernelGGL((combine_kernel<QBNN_BF16>), grid, dim3(256), 0, st, o, (uint16_t*)y, rows, k, N); break;
+    default: hipLaunchKernelGGL((combine_kernel<QBNN_F16>), grid, dim3(256), 0, st, o, (_Float16*)y, rows, k, N); break;
+  }
+  return qbnn_check_launch_msg("qbnn_experts_f8 (sum)");
+}
+
+int quantize(const void* x, int x_type, int64_t bs, int64_t rs, int64_t batch, int R, int K, int block_rows, uint8_t* q, uint8_t* e, hipStream_t st) {
+  QuantF8Args a = {};
+  a.x = x; a.x_bs = bs; a.x_rs = rs; a.q = q; a.e = e;
+  a.R = R; a.K = K; a.Kb = (K + 127) / 128; a.Sp = (a.Kb + 3) / 4 * 4;
+  a.blocks = batch * (block_rows == 1 ? R : (R + 127) / 128) * a.Kb;
+  switch (x_type) {
+    case QBNN_F32: return launch_quantize<QBNN_F32>(a, batch, block_rows, st);
+    case QBNN_BF16: return launch_quantize<QBNN_BF16>(a, batch, block_rows, st);
+    default: return launch_quantize<QBNN_F16>(a, batch, block_rows, st);
+  }
+}
+bool aligned(const void* p, int64_t stride, int to) { return !(((uintptr_t)p | (uintptr_t)stride) & (to - 1)); }
+bool float_type(int t) { return t >= QBNN_F32 && t <= QBNN_F16; }
+void set_columns(F8Args& a, int K) {
+  a.Kb = (int)(((int64_t)K + 127) / 128);
   a.Sp = (a.Kb + 3) / 4 * 4;
-  a.x = d->x; a.xe = d->x_exp; a.x_ss = d->x_ss; a.xe_ss = d->x_exp_ss;
-  a.w = d->w; a.we = d->w_exp; a.w_ss = d->w_ss; a.we_ss = d->w_exp_ss;
-  a.bias = d->bias; a.bias_ss = d->bias_ss;
-  a.y = (uint8_t*)d->y; a.ye = d->y_exp;
-  a.M = d->M; a.N = d->N; a.relu = d->relu;
-  const int Nb = (int)(((int64_t)d->N + 127) / 128);
-  a.y_rs = d->y_type == QBNN_F8 ? Nb * 128 : d->N;
+}
+void set_result(F8Args& a, void* y, uint8_t* ye, int M, int N, int type) {
+  const int Nb = (int)(((int64_t)N + 127) / 128);
+  a.y = (uint8_t*)y; a.ye = ye; a.M = M; a.N = N;
+  a.y_rs = type == QBNN_F8 ? Nb * 128 : N;
   a.ye_rs = (Nb + 3) / 4 * 4;
-  a.y_ss = (int64_t)d->M * a.y_rs;
-  return QBNN_OK;
+  a.y_ss = (int64_t)M * a.y_rs;
 }
 
 }  // namespace
 
 QBNN_EXPORT int qbnn_quantize_f8(const void* x, int32_t x_type, int64_t x_batch_stride, int64_t x_row_stride, int64_t batch, int32_t R, int32_t K,
                                  int32_t block_rows, uint8_t* q, uint8_t* exponents, void* stream) {
-  if (x_type < QBNN_F32 || x_type > QBNN_F16 || batch < 0 || R < 0 || K <= 0 || (block_rows != 1 && block_rows != 128)) return f8_fail("qbnn_quantize_f8: bad argument");
+  if (!float_type(x_type) || batch < 0 || R < 0 || K <= 0 || (block_rows != 1 && block_rows != 128)) return f8_fail("qbnn_quantize_f8: bad argument");
   if (batch == 0 || R == 0) return QBNN_OK;
-  if (!x || !q || !exponents || ((uintptr_t)q & 15) || K > 0x7fffff00) return f8_fail("qbnn_quantize_f8: bad argument (q starts at a multiple of 16 bytes)");
-  QuantF8Args a;
-  a.x = x; a.x_bs = x_batch_stride; a.x_rs = x_row_stride; a.q = q; a.e = exponents;
-  a.R = R; a.K = K; a.Kb = (K + 127) / 128; a.Sp = (a.Kb + 3) / 4 * 4;
-  a.blocks = batch * (block_rows == 1 ? R : (R + 127) / 128) * a.Kb;
-  switch (x_type) {
-    case QBNN_F32: return launch_quantize<QBNN_F32>(a, batch, block_rows, (hipStream_t)stream);
-    case QBNN_BF16: return launch_quantize<QBNN_BF16>(a, batch, block_rows, (hipStream_t)stream);
-    default: return launch_quantize<QBNN_F16>(a, batch, block_rows, (hipStream_t)stream);
-  }
+  if (!x || !q || !exponents || !aligned(q, 0, 16) || K > 0x7fffff00) return f8_fail("qbnn_quantize_f8: bad argument (q starts at a multiple of 16 bytes)");
+  return quantize(x, x_type, x_batch_stride, x_row_stride, batch, R, K, block_rows, q, exponents, (hipStream_t)stream);
 }
 
-QBNN_EXPORT int qbnn_linear_f8_mc(const qbnn_f8_linear* host_desc, void* stream) {
-  F8Args a;
-  if (int rc = fill_args(a, host_desc)) return rc;
-  if (a.M == 0 || host_desc->n_samples == 0) return QBNN_OK;
-  return launch_linear_any<false>(a, a.M, host_desc->n_samples, host_desc->y_type, host_desc->exact, (hipStream_t)stream);
+QBNN_EXPORT int qbnn_linear_f8_mc(const qbnn_f8_linear* d, void* stream) {
+  if (!d || d->N <= 0 || d->K <= 0 || d->K > 0x7fffff00 || d->N > 0x7fffff00 || d->M < 0 || d->n_samples < 0 || d->y_type < QBNN_F32 || d->y_type > QBNN_F8 ||
+      (d->x_float && !float_type(d->x_type)))
+    return f8_fail("qbnn_linear_f8_mc: bad argument");
+  if (d->M == 0 || d->n_samples == 0) return QBNN_OK;
+  if (!d->x || !d->x_exp || !d->w || !d->w_exp || !d->y || (d->y_type == QBNN_F8 && !d->y_exp)) return f8_fail("qbnn_linear_f8_mc: bad argument");
+  if (!aligned(d->x, d->x_ss, 16) || !aligned(d->w, d->w_ss, 16) || !aligned(d->x_exp, d->x_exp_ss, 4) || !aligned(d->w_exp, d->w_exp_ss, 4) ||
+      (d->y_type == QBNN_F8 && !aligned(d->y, 0, 16)))
+    return f8_fail("qbnn_linear_f8_mc: e4m3 operands start at multiples of 16 bytes, exponents of 4");
+  if (d->x_float)
+    if (int rc = quantize(d->x_float, d->x_type, d->x_float_ss, d->x_float_rs, d->x_ss ? d->n_samples : 1, d->M, d->K, 1, d->x, d->x_exp, (hipStream_t)stream)) return rc;
+  F8Args a = {};
+  set_columns(a, d->K);
+  a.x = d->x; a.xe = d->x_exp; a.x_ss = d->x_ss; a.xe_ss = d->x_exp_ss;
+  a.w = d->w; a.we = d->w_exp; a.w_ss = d->w_ss; a.we_ss = d->w_exp_ss;
+  a.bias = d->bias; a.bias_ss = d->bias_ss; a.relu = d->relu;
+  set_result(a, d->y, d->y_exp, d->M, d->N, d->y_type);
+  return launch_linear_any<false>(a, a.M, d->n_samples, d->y_type, 0, (hipStream_t)stream);
 }
 
-QBNN_EXPORT int qbnn_linear_f8_routed(const qbnn_f8_linear* host_desc, const qbnn_f8_routed* r, void* stream) {
-  F8Args a;
-  if (int rc = fill_args(a, host_desc)) return rc;
-  if (!r || !r->offsets || r->groups <= 0 || r->w_groups <= 0 || (r->x_rows && (r->topk <= 0 || r->x_row_count <= 0)) || (r->y_rows && !r->y_weights) ||
-      (r->y_rows && host_desc->y_type == QBNN_F8))
-    return f8_fail("qbnn_linear_f8_routed: bad argument");
-  if (a.M == 0) return QBNN_OK;
-  a.offsets = r->offsets; a.groups = r->groups; a.w_groups = r->w_groups;
-  a.rows = r->x_rows; a.topk = r->topk; a.x_rows = r->x_row_count;
-  a.y_rows = r->y_rows; a.scale = r->y_weights;
-  return launch_linear_any<true>(a, a.M, 1, host_desc->y_type, host_desc->exact, (hipStream_t)stream);
+QBNN_EXPORT int qbnn_experts_f8(const qbnn_f8_experts* d, void* stream) {
+  if (!d || d->S < 0 || d->T < 0 || d->E <= 0 || d->top_k <= 0 || d->D <= 0 || d->H <= 0 || d->N <= 0 || d->D > 0x7fffff00 || d->H > 0x7fffff00 || d->N > 0x7fffff00 ||
+      !float_type(d->y_type) || (d->x_float && !float_type(d->x_type)) || (d->up_sets != d->E && d->up_sets != d->S * d->E) ||
+      (d->down_sets != d->E && d->down_sets != d->S * d->E) || (int64_t)d->S * d->T * d->top_k > 0x7fffffff || (int64_t)d->S * d->E > 0x7fffffff)
+    return f8_fail("qbnn_experts_f8: bad argument");
+  const int rows = d->S * d->T * d->top_k;
+  if (rows == 0) return QBNN_OK;
+  if (!d->x || !d->x_exp || !d->offsets || !d->rows || !d->weights || !d->w_up || !d->up_exp || !d->w_down || !d->down_exp || !d->h || !d->h_exp || !d->o || !d->y ||
+      (d->x_rows != d->T && d->x_rows != d->S * d->T))
+    return f8_fail("qbnn_experts_f8: bad argument");
+  if (!aligned(d->x, 0, 16) || !aligned(d->w_up, d->up_ss, 16) || !aligned(d->w_down, d->down_ss, 16) || !aligned(d->h, 0, 16) || !aligned(d->x_exp, 0, 4) ||
+      !aligned(d->up_exp, d->up_exp_ss, 4) || !aligned(d->down_exp, d->down_exp_ss, 4) || !aligned(d->h_exp, 0, 4))
+    return f8_fail("qbnn_experts_f8: e4m3 operands start at multiples of 16 bytes, exponents of 4");
+  hipStream_t st = (hipStream_t)stream;
+  if (d->x_float)
+    if (int rc = quantize(d->x_float, d->x_type, d->x_float_ss, d->x_float_rs, d->x_rows / d->T, d->T, d->D, 1, d->x, d->x_exp, st)) return rc;
+  F8Args a = {};
+  a.offsets = d->offsets; a.groups = d->S * d->E;
+  set_columns(a, d->D);
+  a.x = d->x; a.xe = d->x_exp; a.rows = d->rows; a.topk = d->top_k; a.x_rows = d->x_rows;
+  a.w = d->w_up; a.we = d->up_exp; a.w_ss = d->up_ss; a.we_ss = d->up_exp_ss; a.w_groups = d->up_sets;
+  a.bias = d->b_up; a.bias_ss = d->b_up_ss; a.relu = 1;
+  set_result(a, d->h, d->h_exp, rows, d->H, QBNN_F8);
+  if (int rc = launch_linear_any<true>(a, rows, 1, QBNN_F8, d->exact & 1, st)) return rc;
+  set_columns(a, d->H);
+  a.x = d->h; a.xe = d->h_exp; a.rows = nullptr;
+  a.w = d->w_down; a.we = d->down_exp; a.w_ss = d->down_ss; a.we_ss = d->down_exp_ss; a.w_groups = d->down_sets;
+  a.bias = d->b_down; a.bias_ss = d->b_down_ss; a.relu = 0;
+  a.y_rows = d->rows; a.scale = d->weights;
+  set_result(a, d->o, nullptr, rows, d->N, QBNN_F32);
+  if (int rc = launch_linear_any<true>(a, rows, 1, QBNN_F32, d->exact >> 1 & 1, st)) return rc;
+  return launch_combine(d->o, d->S * d->T, d->top_k, d->N, d->y, d->y_type, st);
 }

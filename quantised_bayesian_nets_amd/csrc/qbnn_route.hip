@@ -1,4 +1,4 @@
-// libqbnn_hip.so: the router of a layer of experts and the sum of the experts' results.
+// libqbnn_hip.so: the router of a layer of experts.
 //   scores    s = softmax(l) or sigmoid(l) over a row's E logits;  key = s + bias (what is compared), weight = s (what is multiplied)
 //   groups    E / groups neighbouring experts each; a group counts its two largest keys, the best `top_groups` groups stay
 //   choice    the top_k largest keys, ties to the lowest index; weights optionally divided by their sum, times `scale`
@@ -477,32 +477,6 @@ template <int T> int launch_route(const RouteArgs& a, hipStream_t st) {
   return qbnn_check_launch_msg("qbnn_route_experts (order)");
 }
 
-// ---- y[t] = sum over the row's top_k results, in the order of choice --------------------------------------------------------------
-// The results come in fp32: rounded to 16 bits first, each would cost as much as the one rounding of the sum does.
-template <int T> __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ o, f8_type<T>* __restrict__ y, int rows, int k, int N) {
-  const int n0 = (blockIdx.x * 256 + threadIdx.x) * 4;
-  const int64_t t = blockIdx.y + (int64_t)blockIdx.z * 32768;
-  if (n0 >= N || t >= rows) return;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  const bool whole = n0 + 4 <= N;
-  for (int j = 0; j < k; ++j) {
-    const float* r = o + (t * k + j) * N + n0;
-    float v[4];
-    if (whole) __builtin_memcpy(v, r, sizeof(v));
-    else
-      for (int i = 0; i < 4; ++i) v[i] = n0 + i < N ? r[i] : 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] += v[i];
-  }
-  f8_type<T> v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = f8_store<T>(sum[i]);
-  f8_type<T>* out = y + t * N + n0;
-  if (whole) __builtin_memcpy(out, v, sizeof(v));
-  else
-    for (int i = 0; i < 4; ++i) if (n0 + i < N) out[i] = v[i];
-}
-
 }  // namespace
 
 QBNN_EXPORT int64_t qbnn_route_workspace_ints(int32_t S, int32_t T, int32_t E) {
@@ -529,17 +503,4 @@ QBNN_EXPORT int qbnn_route_experts(const qbnn_route* r, void* stream) {
     case QBNN_BF16: return launch_route<QBNN_BF16>(a, (hipStream_t)stream);
     default: return launch_route<QBNN_F16>(a, (hipStream_t)stream);
   }
-}
-
-QBNN_EXPORT int qbnn_combine_routed(const float* o, int32_t rows, int32_t top_k, int32_t N, void* y, int32_t y_type, void* stream) {
-  if (rows < 0 || top_k <= 0 || N <= 0 || y_type < QBNN_F32 || y_type > QBNN_F16) return route_fail("qbnn_combine_routed: bad argument");
-  if (rows == 0) return QBNN_OK;
-  if (!o || !y) return route_fail("qbnn_combine_routed: bad argument");
-  const dim3 grid((unsigned)((N + 1023) / 1024), (unsigned)(rows < 32768 ? rows : 32768), (unsigned)((rows + 32767) / 32768));
-  switch (y_type) {
-    case QBNN_F32: hipLaunchKernelGGL((combine_kernel<QBNN_F32>), grid, dim3(256), 0, (hipStream_t)stream, o, (float*)y, rows, top_k, N); break;
-    case QBNN_BF16: hipLaunchKernelGGL((combine_kernel<QBNN_BF16>), grid, dim3(256), 0, (hipStream_t)stream, o, (uint16_t*)y, rows, top_k, N); break;
-    default: hipLaunchKernelGGL((combine_kernel<QBNN_F16>), grid, dim3(256), 0, (hipStream_t)stream, o, (_Float16*)y, rows, top_k, N); break;
-  }
-  return qbnn_check_launch_msg("qbnn_combine_routed");
 }

@@ -2,13 +2,10 @@
 
 Beside the ensembles here, which evaluate every member on every row: k of E are evaluated, each row by its own choice, and their results are summed
 with the router's weights.  Experts are two linear layers with a ReLU between, in 8-bit floating point (fp8.py)."""
-import ctypes as C
-
 import torch
 
 from . import _lib
-from .fp8 import BLOCK, FLOAT_TYPES, F8Tensor, _F8, _bias, _evaluates, _float, _on, _operand, padded_columns
-from .layers import timed
+from .fp8 import BLOCK, FLOAT_TYPES, F8Tensor, _bias, _device, _float, _launch, _room, _rows, padded_columns
 
 MAX_EXPERTS, MAX_CHOICES = 1024, 32      # include/qbnn.h: QBNN_ROUTE_MAX_EXPERTS, QBNN_ROUTE_MAX_CHOICES
 
@@ -47,25 +44,23 @@ def route_experts(logits, top_k, score="softmax", bias=None, groups=1, top_group
     if S * T * top_k >= 1 << 31 or S > 65535:
         raise ValueError("too many rows for one call")
     bias = _bias(bias, ((E,),), "[E]")
-    dev = _evaluates(logits, bias)
+    dev = _device(logits, bias)
     if logits.stride(-1) != 1 and E > 1:
         logits = logits.contiguous()
-    lead = (S, T) if logits.dim() == 3 else (T,)
-    weights = torch.empty((*lead, top_k), dtype=torch.float32, device=dev)
-    experts = torch.empty((*lead, top_k), dtype=torch.int32, device=dev)
-    rows = torch.empty(S * T * top_k, dtype=torch.int32, device=dev)
-    if rows.numel() == 0:
-        return Routing(weights, experts, torch.zeros(S * E + 1, dtype=torch.int32, device=dev), rows, E)
-    offsets = torch.empty(S * E + 1, dtype=torch.int32, device=dev)
+    lead = (*logits.shape[:-1], top_k)
+    weights = torch.empty(lead, dtype=torch.float32, device=dev)
+    experts = torch.empty(lead, dtype=torch.int32, device=dev)
+    n = S * T * top_k
+    if n == 0:
+        return Routing(weights, experts, torch.zeros(S * E + 1, dtype=torch.int32, device=dev), torch.empty(0, dtype=torch.int32, device=dev), E)
     L = _lib.lib()
-    ws = torch.empty(int(L.qbnn_route_workspace_ints(S, T, E)), dtype=torch.int32, device=dev)
-    d = _lib.Route()
-    d.logits, d.logits_ss, d.logits_rs, d.type = logits.data_ptr(), (logits.stride(0) if logits.dim() == 3 else 0), logits.stride(-2), FLOAT_TYPES[logits.dtype]
-    d.bias = None if bias is None else bias.data_ptr()
-    d.weights, d.experts, d.offsets, d.rows, d.workspace = weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(), rows.data_ptr(), ws.data_ptr()
-    d.S, d.T, d.E, d.top_k, d.groups, d.top_groups, d.sigmoid, d.renormalize, d.scale = S, T, E, top_k, groups, top_groups, int(score == "sigmoid"), int(bool(renormalize)), scale
-    with _on(dev), timed("route_experts"):
-        _lib.check(L.qbnn_route_experts(C.byref(d), _lib.current_stream()))
+    plan = torch.empty(S * E + 1 + n + L.qbnn_route_workspace_ints(S, T, E), dtype=torch.int32, device=dev)      # offsets, rows, workspace
+    offsets, rows = plan[:S * E + 1], plan[S * E + 1:S * E + 1 + n]
+    at = plan.data_ptr()
+    _launch("route_experts", dev, L.qbnn_route_experts, _lib.ROUTE.pack(
+        logits.data_ptr(), logits.stride(0) if len(lead) == 3 else 0, logits.stride(-2), 0 if bias is None else bias.data_ptr(),
+        weights.data_ptr(), experts.data_ptr(), at, at + 4 * (S * E + 1), at + 4 * (S * E + 1 + n),
+        S, T, E, top_k, groups, top_groups, score == "sigmoid", bool(renormalize), FLOAT_TYPES[logits.dtype], scale))
     return Routing(weights, experts, offsets, rows, E)
 
 
@@ -89,8 +84,8 @@ def experts_fp8(x, routing, w_up, w_down, b_up=None, b_down=None, out_dtype=None
         out_dtype = out_dtype or _float(x, "x").dtype
     if out_dtype not in FLOAT_TYPES:
         raise TypeError("out_dtype is float32, bfloat16 or float16")
-    lead, k, E = routing.experts.shape[:-1], routing.experts.shape[-1], routing.n_experts
-    S, T = (lead if len(lead) == 2 else (1, lead[0]))
+    (*lead, k), E = routing.experts.shape, routing.n_experts
+    S, T = lead if len(lead) == 2 else (1, lead[0])
     xs = x.shape
     H, D = w_up.shape[-2:]
     N = w_down.shape[-2]
@@ -98,42 +93,32 @@ def experts_fp8(x, routing, w_up, w_down, b_up=None, b_down=None, out_dtype=None
         raise ValueError("x is [%d or 1, %d, %d] for this routing and w_up" % (S, T, D))
     if w_down.shape[-1] != H or H < 1 or N < 1:
         raise ValueError("w_up [.., H, D] and w_down [.., N, H] do not fit: %s and %s" % (w_up.shape, w_down.shape))
-    own = []
     for w in (w_up, w_down):
-        if tuple(w.shape[:-2]) not in ((E,), (1, E), (S, E)):
+        if w.shape[:-2] not in ((E,), (1, E), (S, E)):
             raise ValueError("the routing has %d experts and %d samples" % (E, S))
-        own.append(len(w.shape) == 4 and w.shape[0] == S)
-    b_up = _bias(b_up, ((*w_up.shape[:-2], H),), "like w_up without its columns")
-    b_down = _bias(b_down, ((*w_down.shape[:-2], N),), "like w_down without its columns")
-    dev = _evaluates(x.data if isinstance(x, F8Tensor) else x, routing.weights, w_up.data, w_down.data, b_up, b_down)
+    b_up = _bias(b_up, (w_up.shape[:-1],), "like w_up without its columns")
+    b_down = _bias(b_down, (w_down.shape[:-1],), "like w_down without its columns")
+    held = isinstance(x, F8Tensor)
+    dev = _device(x.data if held else x, routing.weights, w_up.data, w_down.data, b_up, b_down)
     y = torch.empty((*lead, N), dtype=out_dtype, device=dev)
     R = S * T * k
     if R == 0:
         return y
-    with _on(dev):
-        x = _operand(x)
-        L, st = _lib.lib(), _lib.current_stream()
-        hp, sp = padded_columns(H)
-        h = torch.empty((R, hp), dtype=torch.float8_e4m3fn, device=dev)
-        he = torch.empty((R, sp), dtype=torch.uint8, device=dev)
-        o = torch.empty((R, N), dtype=torch.float32, device=dev)
-        for first, w, b, per_sample in ((True, w_up, b_up, own[0]), (False, w_down, b_down, own[1])):
-            d, r = _lib.F8Linear(), _lib.F8Routed()
-            d.w, d.w_exp, d.w_ss, d.w_exp_ss = w.data.data_ptr(), w.exponent.data_ptr(), w.data.stride(-3), w.exponent.stride(-3)
-            if b is not None:
-                d.bias, d.bias_ss = b.data_ptr(), b.stride(-2)
-            r.offsets, r.groups, r.w_groups = routing.offsets.data_ptr(), S * E, (S * E if per_sample else E)
-            d.M, d.n_samples = R, 1
-            if first:
-                d.x, d.x_exp, d.y, d.y_exp = x.data.data_ptr(), x.exponent.data_ptr(), h.data_ptr(), he.data_ptr()
-                d.N, d.K, d.relu, d.y_type, d.exact = H, D, 1, _F8, int(out_dtype != torch.bfloat16)
-                r.x_rows, r.topk, r.x_row_count = routing.rows.data_ptr(), k, x.data.shape[:-1].numel()
-            else:
-                d.x, d.x_exp, d.y = h.data_ptr(), he.data_ptr(), o.data_ptr()
-                d.N, d.K, d.relu, d.y_type, d.exact = N, H, 0, 0, int(out_dtype == torch.float32)
-                r.y_rows, r.y_weights = routing.rows.data_ptr(), routing.weights.data_ptr()
-            with timed("linear_f8_routed"):
-                _lib.check(L.qbnn_linear_f8_routed(C.byref(d), C.byref(r), st))
-        with timed("combine_routed"):
-            _lib.check(L.qbnn_combine_routed(_lib.ptr(o), S * T, k, N, _lib.ptr(y), FLOAT_TYPES[out_dtype], st))
+    (dp, ds), (hp, hs) = padded_columns(D), padded_columns(H)
+    x_rows = T * (xs[0] if len(xs) == 3 else 1)
+    xf = xf_ss = xf_rs = x_type = 0
+    if held:
+        xq, xe = x.data.data_ptr(), x.exponent.data_ptr()
+        room, (h, he, o) = _room(dev, R * hp, R * hs, 4 * R * N)
+    else:
+        x = _rows(x)
+        xf, xf_ss, xf_rs, x_type = x.data_ptr(), (x.stride(0) if len(xs) == 3 else 0), x.stride(-2), FLOAT_TYPES[x.dtype]
+        room, (xq, xe, h, he, o) = _room(dev, x_rows * dp, x_rows * ds, R * hp, R * hs, 4 * R * N)
+    up, ue, down, de = w_up.data, w_up.exponent, w_down.data, w_down.exponent
+    _launch("experts_f8", dev, _lib.lib().qbnn_experts_f8, _lib.F8_EXPERTS.pack(
+        xf, xf_ss, xf_rs, xq, xe, routing.offsets.data_ptr(), routing.rows.data_ptr(), routing.weights.data_ptr(),
+        up.data_ptr(), ue.data_ptr(), H * dp, -(-H // BLOCK) * ds, 0 if b_up is None else b_up.data_ptr(), H,
+        down.data_ptr(), de.data_ptr(), N * hp, -(-N // BLOCK) * hs, 0 if b_down is None else b_down.data_ptr(), N,
+        h, he, o, y.data_ptr(), S, T, E, k, x_rows, D, H, N, w_up.shape[:-2].numel(), w_down.shape[:-2].numel(),
+        0 if out_dtype == torch.bfloat16 else 1 if out_dtype == torch.float16 else 3, x_type, FLOAT_TYPES[out_dtype]))
     return y

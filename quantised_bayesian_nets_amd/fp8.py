@@ -5,15 +5,10 @@ The int8 layers (layers.py) carry one calibrated scale per tensor; a block of 12
 few large weights (mu + sigma eps has no bound) do not cost the others their precision.  As everywhere here the S Monte-Carlo samples of a
 layer run in one launch, there is no CPU path, and nothing is differentiated: the engine evaluates.
 """
-import contextlib
-import ctypes as C
-
 import torch
-import torch.nn.functional as F
 
-from . import _lib
-from .layers import _MC, timed
-from . import models_f32
+from . import _lib, layers, models_f32
+from .layers import _MC
 
 FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # include/qbnn.h: QBNN_F32, QBNN_BF16, QBNN_F16
 _F8 = 3                                                                    # QBNN_F8
@@ -34,7 +29,8 @@ class F8Tensor:
     __slots__ = ("data", "exponent", "columns", "block_rows")
 
     def __init__(self, data, exponent, columns, block_rows):
-        shape, kp, sp = data.shape, *padded_columns(columns)
+        shape = data.shape
+        kp, sp = padded_columns(columns)
         if block_rows != 1 and block_rows != BLOCK:
             raise ValueError("block_rows is 1 or 128")
         if data.dtype != torch.float8_e4m3fn or exponent.dtype != torch.uint8:
@@ -47,7 +43,7 @@ class F8Tensor:
 
     @property
     def shape(self):
-        return (*self.data.shape[:-1], self.columns)
+        return torch.Size((*self.data.shape[:-1], self.columns))
 
     @property
     def device(self):
@@ -64,13 +60,14 @@ class F8Tensor:
         return (self.data.to(torch.float32) * scale)[..., :self.columns].to(dtype)
 
 
-def _evaluates(*tensors):
-    """Refuses what the engine would silently get wrong: tensors off the GPU, on several devices, or waiting for a gradient."""
+def _device(*tensors):
+    """The device of a call's tensors (None entries left out).  Refuses what the engine would silently get wrong: tensors off the GPU, on several devices, or
+    waiting for a gradient."""
     dev = None
     for t in tensors:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise RuntimeError("qbnn layers run on an MI355X only (no CPU fallback)")
         if dev is None:
             dev = t.device
@@ -81,9 +78,24 @@ def _evaluates(*tensors):
     return dev
 
 
-def _on(dev):
-    """The device current for a launch: a call's tensors decide, not the caller's current device."""
-    return contextlib.nullcontext() if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _launch(key, dev, fn, *args):
+    """fn(*args, stream) on the current stream of `dev`: a call's tensors decide the device, not the caller's current one."""
+    if dev.index == torch.cuda.current_device() and layers.PROFILE is None:
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)))
+        return
+    with torch.cuda.device(dev), layers.timed(key):
+        _lib.check(fn(*args, _lib.current_stream()))
+
+
+def _room(dev, *sizes):
+    """One allocation for a call's workspaces (bytes): its tensor and each one's address, at multiples of 256."""
+    at, places = 0, []
+    for n in sizes:
+        places.append(at)
+        at += (n + 255) & ~255
+    t = torch.empty(at, dtype=torch.uint8, device=dev)
+    base = t.data_ptr()
+    return t, [base + p for p in places]
 
 
 def _float(t, name):
@@ -100,28 +112,26 @@ def quantize_fp8(x, block_rows=1):
         raise ValueError("x is [..., R, K] with K >= 1")
     if block_rows != 1 and block_rows != BLOCK:
         raise ValueError("block_rows is 1 or 128")
-    dev = _evaluates(x)
+    dev = _device(x)
     lead, (R, K) = x.shape[:-2], x.shape[-2:]
-    if x.stride(-1) != 1 and K > 1 or x.dim() > 3:
-        x = x.contiguous()
+    x = _rows(x)
     kp, sp = padded_columns(K)
     q = torch.empty((*lead, R, kp), dtype=torch.float8_e4m3fn, device=dev)
     e = torch.empty((*lead, -(-R // block_rows), sp), dtype=torch.uint8, device=dev)
-    batch = lead.numel()
-    bs, rs = (x.stride(0) if x.dim() == 3 else R * K), x.stride(-2)
-    with _on(dev), timed("quantize_f8"):
-        _lib.check(_lib.lib().qbnn_quantize_f8(_lib.ptr(x), FLOAT_TYPES[x.dtype], bs, rs, batch, R, K, block_rows, _lib.ptr(q), _lib.ptr(e), _lib.current_stream()))
+    _launch("quantize_f8", dev, _lib.lib().qbnn_quantize_f8, x.data_ptr(), FLOAT_TYPES[x.dtype], (x.stride(0) if x.dim() == 3 else R * K), x.stride(-2), lead.numel(),
+            R, K, block_rows, q.data_ptr(), e.data_ptr())
     return F8Tensor(q, e, K, block_rows)
 
 
-def _operand(x):
-    return x if isinstance(x, F8Tensor) else quantize_fp8(x)
+def _rows(x):
+    """x as the quantiser reads it: at most three dimensions with strides of their own, columns side by side (a copy where they are not)."""
+    return x.contiguous() if x.stride(-1) != 1 and x.shape[-1] > 1 or x.dim() > 3 else x
 
 
 def _bias(bias, shapes, what):
     if bias is None:
         return None
-    if bias.dtype != torch.float32 or tuple(bias.shape) not in shapes:
+    if bias.dtype != torch.float32 or bias.shape not in shapes:
         raise ValueError("bias is float32 %s" % what)
     return bias.contiguous()
 
@@ -155,32 +165,30 @@ def linear_fp8(x, w, bias=None, relu=False, out_dtype=None):
     if out_dtype not in FLOAT_TYPES and out_dtype != torch.float8_e4m3fn:
         raise TypeError("out_dtype is float32, bfloat16, float16 or float8_e4m3fn")
     bias = _bias(bias, ((N,), (S, N)), "[N] or [S, N]")
-    dev = _evaluates(x.data if isinstance(x, F8Tensor) else x, w.data, bias)
-    with _on(dev):
-        x = _operand(x)
-        lead = (S, B) if len(xs) == 3 or len(ws) == 3 else (B,)
-        ye = None
-        if out_dtype == torch.float8_e4m3fn:
-            np_, sp = padded_columns(N)
-            y = torch.empty((*lead, np_), dtype=out_dtype, device=dev)
-            ye = torch.empty((*lead, sp), dtype=torch.uint8, device=dev)
+    held = isinstance(x, F8Tensor)
+    dev = _device(x.data if held else x, w.data, bias)
+    lead = (S, B) if len(xs) == 3 or len(ws) == 3 else (B,)
+    ye = None
+    if out_dtype == torch.float8_e4m3fn:
+        np_, sp = padded_columns(N)
+        y = torch.empty((*lead, np_), dtype=out_dtype, device=dev)
+        ye = torch.empty((*lead, sp), dtype=torch.uint8, device=dev)
+    else:
+        y = torch.empty((*lead, N), dtype=out_dtype, device=dev)
+    if S * B:
+        kp, sp = padded_columns(K)
+        xf = xf_ss = xf_rs = x_type = 0
+        if held:
+            xq, xe = x.data.data_ptr(), x.exponent.data_ptr()
         else:
-            y = torch.empty((*lead, N), dtype=out_dtype, device=dev)
-        if S * B == 0:
-            return y if ye is None else F8Tensor(y, ye, N, 1)
-        d = _lib.F8Linear()
-        d.x, d.x_exp, d.w, d.w_exp = x.data.data_ptr(), x.exponent.data_ptr(), w.data.data_ptr(), w.exponent.data_ptr()
-        if sx > 1:
-            d.x_ss, d.x_exp_ss = x.data.stride(0), x.exponent.stride(0)
-        if sw > 1:
-            d.w_ss, d.w_exp_ss = w.data.stride(0), w.exponent.stride(0)
-        if bias is not None:
-            d.bias, d.bias_ss = bias.data_ptr(), (N if bias.dim() == 2 and S > 1 else 0)
-        d.y, d.y_exp = y.data_ptr(), (None if ye is None else ye.data_ptr())
-        d.M, d.N, d.K, d.n_samples, d.relu = B, N, K, S, int(bool(relu))
-        d.y_type, d.exact = FLOAT_TYPES.get(out_dtype, _F8), int(out_dtype == torch.float32)
-        with timed("linear_f8"):
-            _lib.check(_lib.lib().qbnn_linear_f8_mc(C.byref(d), _lib.current_stream()))
+            x = _rows(x)
+            xf, xf_ss, xf_rs, x_type = x.data_ptr(), (x.stride(0) if len(xs) == 3 else 0), x.stride(-2), FLOAT_TYPES[x.dtype]
+            room, (xq, xe) = _room(dev, sx * B * kp, sx * B * sp)
+        _launch("linear_f8", dev, _lib.lib().qbnn_linear_f8_mc, _lib.F8_LINEAR.pack(
+            xf, xf_ss, xf_rs, xq, xe, (B * kp if sx > 1 else 0), (B * sp if sx > 1 else 0),
+            w.data.data_ptr(), w.exponent.data_ptr(), (N * kp if sw > 1 else 0), (-(-N // BLOCK) * sp if sw > 1 else 0),
+            0 if bias is None else bias.data_ptr(), N if bias is not None and bias.dim() == 2 and S > 1 else 0,
+            y.data_ptr(), 0 if ye is None else ye.data_ptr(), B, N, K, S, bool(relu), FLOAT_TYPES.get(out_dtype, _F8), x_type))
     return y if ye is None else F8Tensor(y, ye, N, 1)
 
 

@@ -73,16 +73,34 @@ def test_experts_refuse():
 
 def test_c_entries_refuse():
     """Argument errors come back as codes with a text, before any launch."""
-    import ctypes as C
     L = _lib.lib()
     assert L.qbnn_quantize_f8(None, 0, 0, 0, 1, 1, 1, 1, None, None, None) == -1
     assert L.qbnn_quantize_f8(None, 5, 0, 0, 0, 1, 1, 1, None, None, None) == -1
     assert L.qbnn_quantize_f8(None, 0, 0, 0, 0, 1, 1, 1, None, None, None) == 0
-    assert L.qbnn_linear_f8_mc(C.byref(_lib.F8Linear()), None) == -1 and b"qbnn_linear_f8" in L.qbnn_last_error()
-    d = _lib.F8Linear()
-    d.x, d.x_exp, d.w, d.w_exp, d.y, d.M, d.N, d.K, d.n_samples = 1032, 1024, 1024, 1024, 1024, 1, 1, 1, 1
-    assert L.qbnn_linear_f8_mc(C.byref(d), None) == -1 and b"multiples of 16" in L.qbnn_last_error()
-    assert L.qbnn_linear_f8_routed(C.byref(d), C.byref(_lib.F8Routed()), None) == -1
-    assert L.qbnn_route_experts(C.byref(_lib.Route()), None) == -1
-    assert L.qbnn_combine_routed(None, 1, 1, 1, None, 7, None) == -1
+    linear, experts, route = _lib.F8_LINEAR, _lib.F8_EXPERTS, _lib.ROUTE
+    assert L.qbnn_linear_f8_mc(bytes(linear.size), None) == -1 and b"qbnn_linear_f8" in L.qbnn_last_error()
+    p = [0, 0, 0, 1032, 1024, 0, 0, 1024, 1024, 0, 0, 0, 0, 1024, 0]
+    assert L.qbnn_linear_f8_mc(linear.pack(*p, 1, 1, 1, 1, 0, 0, 0), None) == -1 and b"multiples of 16" in L.qbnn_last_error()
+    assert L.qbnn_linear_f8_mc(linear.pack(*p, 1, 1, 1, 1, 0, 4, 0), None) == -1 and b"bad argument" in L.qbnn_last_error()
+    assert L.qbnn_linear_f8_mc(linear.pack(*p, 0, 1, 1, 1, 0, 0, 0), None) == 0
+    assert L.qbnn_experts_f8(bytes(experts.size), None) == -1
+    assert L.qbnn_experts_f8(experts.pack(*[0] * 24, 1, 0, 2, 1, 1, 1, 1, 1, 2, 2, 0, 0, 0), None) == 0          # no rows
+    assert L.qbnn_experts_f8(experts.pack(*[0] * 24, 1, 1, 2, 1, 1, 1, 1, 1, 2, 2, 0, 0, 0), None) == -1         # no tensors
+    assert L.qbnn_route_experts(bytes(route.size), None) == -1
+    assert L.qbnn_route_experts(route.pack(*[1024] * 9, 1, 1, 4, 5, 1, 1, 0, 0, 0, 1.0), None) == -1             # more choices than experts
     assert L.qbnn_route_workspace_ints(0, 5, 5) == 0
+
+
+def test_descriptors_match_the_header(tmp_path):
+    """The packed descriptors are the C structs: sizes (up to the last field) and the offsets of the fields at their ends, by a C compiler."""
+    import os
+    import shutil
+    import subprocess
+    if not shutil.which("gcc"):
+        pytest.skip("no C compiler")
+    src, exe = tmp_path / "t.c", tmp_path / "t"
+    src.write_text('#include "qbnn.h"\n#include <stdio.h>\nint main(void) { printf("%zu %zu %zu %zu %zu %zu\\n", offsetof(qbnn_f8_linear, x_type) + 4, offsetof(qbnn_f8_linear, M), '
+                   'offsetof(qbnn_f8_experts, y_type) + 4, offsetof(qbnn_f8_experts, S), offsetof(qbnn_route, scale) + 4, offsetof(qbnn_route, S)); return 0; }\n')
+    subprocess.check_call(["gcc", "-I", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include"), str(src), "-o", str(exe)])
+    linear, experts, route = _lib.F8_LINEAR.size, _lib.F8_EXPERTS.size, _lib.ROUTE.size
+    assert [int(v) for v in subprocess.check_output([str(exe)]).split()] == [linear, linear - 28, experts, experts - 52, route, route - 40]
