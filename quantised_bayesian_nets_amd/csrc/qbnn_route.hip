@@ -3,8 +3,8 @@
 //   groups    E / groups neighbouring experts each; a group counts its two largest keys, the best `top_groups` groups stay
 //   choice    the top_k largest keys, ties to the lowest index; weights optionally divided by their sum, times `scale`
 //   order     the (row, choice) pairs of a sample sorted by expert, stable: what the experts' products walk
-// Keys are compared as 64-bit values: two experts whose scores differ only behind fp32's last place are still told apart, so the choice
-// does not depend on the order in which a row's sum was taken.
+// The choice is that of 64-bit keys: two experts whose scores differ only behind fp32's last place are still told apart, so it does not depend on
+// the order in which a row's sum was taken.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -73,41 +73,39 @@ template <int L> __device__ __forceinline__ float route_sumf(float v) {
 __device__ __forceinline__ uint32_t route_order(float v) { const uint32_t b = __float_as_uint(v); return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u); }
 __device__ __forceinline__ float route_value(uint32_t o) { return __uint_as_float(o ^ ((uint32_t)((int)~o >> 31) | 0x80000000u)); }
 
-// The group mask of a row whose keys lie in `keys` (LDS): lane q < rows x groups of the wave takes group q % groups of row q / groups and sums its two largest keys
-// (masked experts left out; a group of masked experts ranks last); ranks come from comparing with the row's other groups.  slack[row]: the score
-// of the last group kept minus the best one left out.  FLT: the keys' type.
-template <class FLT> __device__ __forceinline__ void route_groups(const RouteArgs& a, const FLT* keys, int rows, int pitch, FLT* score, uint32_t* stay, FLT* slack) {
-  const int lane = threadIdx.x & 63, per = a.E / a.groups;
-  for (int q0 = 0; q0 < rows * a.groups; q0 += 64) {
-    const int q = q0 + lane;
-    if (q < rows * a.groups) {
-      const int r = q / a.groups, g = q - r * a.groups;
-      const FLT* k = keys + r * pitch + g * per;
-      FLT a1 = -INFINITY, a2 = -INFINITY;
-      for (int i = 0; i < per; ++i) {
-        const FLT v = k[i];
-        if (v > a1) { a2 = a1; a1 = v; } else if (v > a2) a2 = v;
-      }
-      score[q] = a1 == -INFINITY ? a1 : a2 == -INFINITY ? a1 : a1 + a2;
+// What a group of keys counts: its two largest summed, masked ones left out; a group of masked keys ranks last.
+template <class FLT> __device__ __forceinline__ FLT route_score(FLT a1, FLT a2) { return a1 == -INFINITY ? a1 : a2 == -INFINITY ? a1 : a1 + a2; }
+
+// score[row][group] of the wave's rows from their keys in LDS, a lane per (row, group)
+template <class FLT> __device__ __forceinline__ void route_group_scores(const RouteArgs& a, const FLT* keys, int rows, int pitch, FLT* score) {
+  const int per = a.E / a.groups;
+  for (int q = threadIdx.x & 63; q < rows * a.groups; q += 64) {
+    const int r = q / a.groups, g = q - r * a.groups;
+    const FLT* k = keys + r * pitch + g * per;
+    FLT a1 = -INFINITY, a2 = -INFINITY;
+    for (int i = 0; i < per; ++i) {
+      const FLT v = k[i];
+      if (v > a1) { a2 = a1; a1 = v; } else if (v > a2) a2 = v;
     }
+    score[q] = route_score(a1, a2);
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  for (int q0 = 0; q0 < rows * a.groups; q0 += 64) {
-    const int q = q0 + lane;
-    if (q < rows * a.groups) {
-      const int r = q / a.groups, g = q - r * a.groups;
-      const FLT mine = score[q];
-      int rank = 0;
-      FLT next = -INFINITY;                                     // the best score behind mine
-      for (int i = 0; i < a.groups; ++i) {
-        const FLT o = score[r * a.groups + i];
-        const bool ahead = o > mine || (o == mine && i < g);
-        rank += ahead ? 1 : 0;
-        if (!ahead && i != g && o > next) next = o;
-      }
-      stay[q] = rank < a.kept ? 1u : 0u;
-      if (rank == a.kept - 1) slack[r] = a.kept == a.groups ? (FLT)INFINITY : mine == next ? (FLT)0 : mine - next;
+}
+// Which groups stay, by comparing each with its row's others; slack[row]: the score of the last group kept minus the best one left out.
+template <class FLT> __device__ __forceinline__ void route_keep_groups(const RouteArgs& a, int rows, const FLT* score, uint32_t* stay, FLT* slack) {
+  for (int q = threadIdx.x & 63; q < rows * a.groups; q += 64) {
+    const int r = q / a.groups, g = q - r * a.groups;
+    const FLT mine = score[q];
+    int rank = 0;
+    FLT next = -INFINITY;                                       // the best score behind mine
+    for (int i = 0; i < a.groups; ++i) {
+      const FLT o = score[r * a.groups + i];
+      const bool ahead = o > mine || (o == mine && i < g);
+      rank += ahead ? 1 : 0;
+      if (!ahead && i != g && o > next) next = o;
     }
+    stay[q] = rank < a.kept ? 1u : 0u;
+    if (rank == a.kept - 1) slack[r] = a.kept == a.groups ? (FLT)INFINITY : mine == next ? (FLT)0 : mine - next;
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
@@ -172,33 +170,112 @@ template <class F> __device__ __forceinline__ void route_starts(int* count, int 
   __syncthreads();
 }
 
+// LDS of a wave for its rows' groups: fp32 keys [64 / L][L 16 + 2] where a group is no power of two, scores, masks and slack of 64 / L rows; 64-bit ones of one row
+template <int L> __host__ __device__ constexpr int route_group_bytes(int groups) {
+  const int fast = (64 / L) * ((L * 16 + 2 + 2 * groups) * 4 + 4), exact = ((L < 4 ? 64 : L * 16) + 1) * 8 + groups * 12;
+  return ((fast > exact ? fast : exact) + 15) & ~15;
+}
+
+// One row by a whole wave with 64-bit keys, NP experts per lane.
+template <int T, int NP> __device__ __forceinline__ void route_exact_row(const RouteArgs& a, const f8_type<T>* l, bool by_logit, uint8_t* more, uint32_t* choice) {
+  const int lane = threadIdx.x & 63;
+  double key[NP], top = -INFINITY, total = 0.;
+  int idx[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    idx[i] = i * 64 + lane < a.E ? i * 64 + lane : 0x7fffffff;
+    const float v = i * 64 + lane < a.E ? f8_load<T>(l[i * 64 + lane]) : -INFINITY;
+    key[i] = v > route_lowest<T>() ? (double)v : -INFINITY;     // (false for NaN)
+    top = fmax(top, key[i]);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = fmax(top, __shfl_xor(top, d));
+  if (!by_logit) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const bool open = key[i] > -INFINITY;
+      key[i] = !open ? -1. : a.sigmoid ? 1. / (1. + exp(-key[i])) : exp(key[i] - top);
+      total += open ? key[i] : 0.;
+    }
+    if (!a.sigmoid)
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      double q = a.sigmoid ? key[i] : key[i] / total;
+      if (a.bias && i * 64 + lane < a.E) q += (double)a.bias[i * 64 + lane];
+      key[i] = key[i] >= 0. && q == q ? q : -INFINITY;
+    }
+    if (a.groups > 1) {
+      double* keys = (double*)more;
+      double* score = keys + NP * 64;
+      double* slack = score + a.groups;
+      uint32_t* stay = (uint32_t*)(slack + 1);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) if (i * 64 + lane < a.E) keys[i * 64 + lane] = key[i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      route_group_scores<double>(a, keys, 1, 0, score);
+      route_keep_groups<double>(a, 1, score, stay, slack);
+      const int per = a.E / a.groups;
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        if (idx[i] < a.E && !stay[idx[i] / per]) { key[i] = -INFINITY; idx[i] = 0x7fffffff; }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  }
+  for (int j = 0; j < a.k; ++j) {
+    double b = key[0];
+    int bi = idx[0];
+#pragma unroll
+    for (int i = 1; i < NP; ++i)
+      if (key[i] > b || (key[i] == b && idx[i] < bi)) { b = key[i]; bi = idx[i]; }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const double ob = __shfl_xor(b, d);
+      const int oi = __shfl_xor(bi, d);
+      if (ob > b || (ob == b && oi < bi)) { b = ob; bi = oi; }
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) if (idx[i] == bi) { key[i] = -INFINITY; idx[i] = 0x7fffffff; }
+    if (lane == 0) choice[j] = (uint32_t)bi;
+  }
+}
+
 // L lanes per row, 16 neighbouring experts per lane.
 //
-// Fast pass: keys in fp32 as ordered integers, an expert's index (its complement) in their low bits, so that a round of the choice is one integer maximum and ties go
-// to the lowest index.  It decides where it provably can: logits of 16 bits compare exactly as they are; elsewhere each chosen key must lie above the next
-// one by more than the keys' error and the bits given up (and likewise the last group kept above the next).  The waves where one does not (a few
-// rows in a thousand, and rows with ties) do their rows again with 64-bit keys.
-// Bound: 16384 x 256 logits are 3 us of reading; a round costs 45 vector instructions for 64 / L rows.
-template <int L> __host__ __device__ constexpr int route_group_bytes(int groups) { return ((64 / L) * ((L * 16 + 2) * 8 + groups * 12 + 8) + 15) & ~15; }      // of a wave
+// Fast pass: keys in fp32 as ordered integers whose low bits say which expert they are (its complement: ties go to the lowest index), so that a round of the
+// choice is one integer maximum.  Logits of 16 bits compare exactly as they are and carry the whole index; other keys give up only 4 bits, for the place
+// in their lane, and the choice must be proved: each chosen key has to lie above the next one by more than the keys' error and the bits given up (and
+// likewise the last group kept above the next), and one lane alone may hold it.  Rows without that proof (1 in 1000 of 256 random fp32 logits, and rows with ties)
+// are listed and done again, a whole wave each, with 64-bit keys.  Masked experts are the integers below all keys, lowest index first.
+// A key that was chosen is not taken out: the next round looks for the largest below it, as the smallest unsigned m - 1 - w (what lies above wraps).
+// Bound: a round is 24 + 12 instructions for 64 / L rows; 32768 x 256 logits are 5 us of reading.
+constexpr uint32_t ROUTE_MASKED = 0x00800000u;                  // the order of the lowest finite float: masked experts lie below
 
 template <int T, int L> __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
   constexpr int RPW = 64 / L;                                   // rows per wave
   constexpr int PITCH = L * 16 + 2;
+  constexpr int NP = L < 4 ? 1 : L / 4;                         // experts per lane where a wave does one row
   extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
   __shared__ float row_top[ROUTE_ROWS], row_sum[ROUTE_ROWS];
+  __shared__ int again[ROUTE_ROWS], n_again;
   // dynamic: choices and their scores [64][k], the quarters' counts [4][E], starts [E], and with groups each wave's keys, scores, masks
   uint32_t* choice = (uint32_t*)dyn;
   float* part = (float*)(choice + ROUTE_ROWS * a.k);
   int* count = (int*)(part + ROUTE_ROWS * a.k);
   int* start = count + 4 * a.E;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / L, li = lane % L;
   uint8_t* more = (uint8_t*)(start + a.E);
   more += (-(uintptr_t)more) & 15;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / L, li = lane % L;
+  more += (size_t)wave * route_group_bytes<L>(a.groups);
   const int s = blockIdx.y, t0 = blockIdx.x * ROUTE_ROWS, rows = min(a.T - t0, ROUTE_ROWS);
-  const uint32_t low = (1u << a.bits) - 1;
   const bool by_logit = !a.bias && a.groups == 1;               // both scores increase with the logit
+  const bool exact = by_logit && T != QBNN_F32;
+  const uint32_t low = exact ? (1u << a.bits) - 1 : 15u;
   const f8_type<T>* base = (const f8_type<T>*)a.logits + s * a.l_ss + t0 * a.l_rs;
   for (int i = threadIdx.x; i < 4 * a.E; i += 256) count[i] = 0;
+  if (threadIdx.x == 0) n_again = 0;
+  __syncthreads();
 
   for (int r0 = wave * RPW; r0 < rows; r0 += 4 * RPW) {
     const int r = r0 + sub, e0 = li * 16;
@@ -214,145 +291,140 @@ template <int T, int L> __global__ __launch_bounds__(256) void route_kernel(cons
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = e0 + i < a.E ? f8_load<T>(l[i]) : -INFINITY;
     }
-    uint32_t open = 0;                                          // not masked: -inf, the type's lowest value and NaN are
     bool nan = false;
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       nan |= v[i] != v[i];
-      if (v[i] > route_lowest<T>()) { open |= 1u << i; top = fmaxf(top, v[i]); }
+      v[i] = v[i] > route_lowest<T>() ? v[i] : -INFINITY;       // masked: -inf, the type's lowest value and NaN
+      top = fmaxf(top, v[i]);
     }
     top = route_maxf<L>(top);
-    float sc[16], sum = 0.f, worst = 0.f;                       // scores; the largest error of one, in 2^-23
-    if (!by_logit || !a.sigmoid) {
+    uint32_t w[16];
+    bool unsure = false;
+    float sum = 0.f, worst = 0.f;                               // worst: the error of two keys' difference
+    if (by_logit) {
+      if (!a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += v[i] > -INFINITY ? route_exp(v[i] - top) : 0.f;
+        sum = route_sumf<L>(sum);
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float x = a.sigmoid ? -v[i] : v[i] - top;
-        const float z = route_exp(x);
-        sc[i] = (open >> i) & 1 ? (a.sigmoid ? 1.f / (1.f + z) : z) : 0.f;
-        sum += sc[i];
+        const uint32_t place = exact ? low - (uint32_t)(e0 + i) : 15u - i;
+        w[i] = v[i] > -INFINITY ? (route_order(v[i] + 0.f) & ~low) | place : e0 + i < a.E ? (uint32_t)(a.E - e0 - i) : 0u;      // (-0 ties with 0)
+      }
+    } else {
+      // p off by at most p (|x| + c) 2^-23.  Sigmoid: 1 + z, its reciprocal and exp's (|x| + 2): c = 5, 8 taken.  Softmax: exp's |x| + 3, the sum's: 15 + 6
+      // additions (11) and its terms' own (sum p |x| <= ln E < 7, and 3): c = 26, 32 taken.  Adding the bias: half a step of the key.
+      float key[16], large = 0.f;
+      const float c = a.sigmoid ? 8.f : 32.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float z = route_exp(a.sigmoid ? -v[i] : v[i] - top);
+        key[i] = v[i] > -INFINITY ? (a.sigmoid ? __builtin_amdgcn_rcpf(1.f + z) : z) : 0.f;
+        sum += key[i];
+      }
+      if (!a.sigmoid) sum = route_sumf<L>(sum);
+      const float over = a.sigmoid ? 1.f : __builtin_amdgcn_rcpf(sum);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = key[i] * over;
+        const float q = p + (a.bias && e0 + i < a.E ? a.bias[e0 + i] : 0.f);
+        key[i] = v[i] > -INFINITY && q == q ? q : -INFINITY;
+        const float off = p * (fabsf(a.sigmoid ? v[i] : v[i] - top) + c);
+        worst = key[i] > -INFINITY ? fmaxf(worst, off) : worst;
+        large = key[i] > -INFINITY ? fmaxf(large, fabsf(key[i])) : large;
+      }
+      large = route_maxf<L>(large);
+      worst = (route_maxf<L>(worst) + large) * 2.384185791015625e-7f;
+      unsure = !(worst < INFINITY);
+      uint32_t in = 0xffffu;
+      if (a.groups > 1) {
+        const int per = a.E / a.groups;
+        float* score = (float*)more;                            // [RPW][groups]
+        uint32_t* stay = (uint32_t*)(score + RPW * a.groups);
+        float* slack = (float*)(stay + RPW * a.groups);
+        if ((per & (per - 1)) == 0) {                           // a lane holds whole groups, or a group whole lanes: in registers
+          float a1 = -INFINITY, a2 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            a2 = __builtin_amdgcn_fmed3f(a1, a2, key[i]);
+            a1 = fmaxf(a1, key[i]);
+            if (per < 16 && ((i + 1) & (per - 1)) == 0) {
+              if (e0 + i < a.E) score[sub * a.groups + (e0 + i) / (unsigned)per] = route_score(a1, a2);
+              a1 = a2 = -INFINITY;
+            }
+          }
+          auto join = [&](uint32_t p1, uint32_t p2) {
+            const float b1 = __uint_as_float(p1), b2 = __uint_as_float(p2);
+            a2 = fmaxf(fminf(a1, b1), fmaxf(a2, b2));
+            a1 = fmaxf(a1, b1);
+          };
+          if (L > 1 && per > 16) join(route_partner<1>(__float_as_uint(a1)), route_partner<1>(__float_as_uint(a2)));
+          if (L > 2 && per > 32) join(route_partner<2>(__float_as_uint(a1)), route_partner<2>(__float_as_uint(a2)));
+          if (L > 4 && per > 64) join(route_partner<4>(__float_as_uint(a1)), route_partner<4>(__float_as_uint(a2)));
+          if (L > 8 && per > 128) join(route_partner<8>(__float_as_uint(a1)), route_partner<8>(__float_as_uint(a2)));
+          if (L > 16 && per > 256) join(route_partner<16>(__float_as_uint(a1)), route_partner<16>(__float_as_uint(a2)));
+          if (per >= 16 && (e0 & (per - 1)) == 0 && e0 < a.E) score[sub * a.groups + e0 / (unsigned)per] = route_score(a1, a2);
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        } else {
+          float* keys = slack + RPW;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) keys[sub * PITCH + e0 + i] = key[i];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          route_group_scores<float>(a, keys, RPW, PITCH, score);
+        }
+        route_keep_groups<float>(a, RPW, score, stay, slack);
+        unsure |= !(slack[sub] > 2.f * worst + large * 4.8e-7f);
+        if (per >= 16 && (per & (per - 1)) == 0) in = e0 < a.E && stay[sub * a.groups + e0 / (unsigned)per] ? 0xffffu : 0u;
+        else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (e0 + i < a.E && !stay[sub * a.groups + (e0 + i) / (unsigned)per]) in &= ~(1u << i);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t order = key[i] > -INFINITY ? (route_order(key[i]) & ~15u) | (15u - i) : (uint32_t)(a.E - e0 - i);
+        w[i] = e0 + i < a.E && ((in >> i) & 1) ? order : 0u;
       }
     }
-    if (!a.sigmoid) sum = route_sumf<L>(sum);
     if (li == 0 && valid) {
       row_top[r] = top;
       row_sum[r] = sum;
     }
     if (route_max<L>(nan ? 1u : 0u) && li == 0 && valid) row_top[r] = NAN;
 
-    uint32_t w[16];
-    bool unsure = false;
-    if (by_logit) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float q = (open >> i) & 1 ? v[i] + 0.f : -INFINITY;      // (-0 ties with 0)
-        w[i] = e0 + i < a.E ? (route_order(q) & ~low) | (low - (uint32_t)(e0 + i)) : 0u;
-      }
-    } else {
-      const float over = a.sigmoid ? 1.f : 1.f / sum;
-      float key[16], large = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = a.sigmoid ? sc[i] : sc[i] * over;
-        const float q = (open >> i) & 1 ? p + (a.bias && e0 + i < a.E ? a.bias[e0 + i] : 0.f) : -INFINITY;
-        key[i] = q == q ? q : -INFINITY;
-        if (key[i] > -INFINITY) {
-          worst = fmaxf(worst, p * (fabsf(a.sigmoid ? v[i] : v[i] - top) + 32.f));
-          large = fmaxf(large, fabsf(key[i]));
-        }
-      }
-      large = route_maxf<L>(large);
-      worst = (route_maxf<L>(worst) + large) * 2.384185791015625e-7f;      // 2 x 2^-23: of two keys' difference
-      unsure = !(worst < INFINITY);
-      uint32_t in = 0xffffu;
-      if (a.groups > 1) {
-        float* keys = (float*)(more + (size_t)wave * route_group_bytes<L>(a.groups));
-        float* score = keys + RPW * PITCH;
-        uint32_t* stay = (uint32_t*)(score + RPW * a.groups);
-        float* slack = (float*)(stay + RPW * a.groups);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) keys[sub * PITCH + e0 + i] = key[i];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        route_groups<float>(a, keys, RPW, PITCH, score, stay, slack);
-        unsure |= !(slack[sub] > 2.f * worst + large * 4.8e-7f);
-        const int per = a.E / a.groups;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (e0 + i < a.E && !stay[sub * a.groups + (e0 + i) / per]) in &= ~(1u << i);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = e0 + i < a.E && ((in >> i) & 1) ? (route_order(key[i]) & ~low) | (low - (uint32_t)(e0 + i)) : 0u;
-    }
     // k rounds, and one more to see that the last choice was none too close
-    const bool exact = by_logit && T != QBNN_F32;
     uint32_t before = 0;
     for (int j = 0; j < a.k + (exact ? 0 : 1); ++j) {
-      uint32_t m = w[0];
+      const uint32_t c = before - 1;
+      uint32_t near = 0xffffffffu;
 #pragma unroll
-      for (int i = 1; i < 16; ++i) m = max(m, w[i]);
-      m = route_max<L>(m);
-      if (j < a.k && li == 0 && valid) choice[r * a.k + j] = low - (m & low);
-      if (!exact && j > 0 && m != 0) {
-        if (by_logit) unsure |= ((before ^ m) & ~low) == 0;
-        else unsure |= !(route_value(before & ~low) - route_value(m | low) > worst);
+      for (int i = 0; i < 16; ++i) near = min(near, c - w[i]);
+      const uint32_t mine = near <= c ? c - near : 0u;          // the lane's largest below `before`; 0: none
+      const uint32_t m = route_max<L>(mine);
+      if (j < a.k) {
+        const bool own = mine == m;
+        if (own && valid) choice[r * a.k + j] = m < ROUTE_MASKED ? a.E - m : exact ? low - (m & low) : e0 + 15u - (m & 15u);
+        if (!exact && L > 1) {
+          const unsigned long long owners = __ballot(own);
+          if (__popcll(owners) != RPW) unsure |= __popcll((owners >> (sub * L % 64)) & (L < 64 ? (1ull << (L % 64)) - 1 : ~0ull)) > 1;
+        }
+      }
+      if (!exact && j > 0 && m >= ROUTE_MASKED) {
+        if (by_logit) unsure |= ((before ^ m) & ~15u) == 0;
+        else unsure |= !(route_value(before & ~15u) - route_value(m | 15u) > worst);
       }
       before = m;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = w[i] == m ? 0u : w[i];
     }
-    if (__any(unsure && valid)) {
-      double key[16], total = 0.;
-      int idx[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const double x = (double)v[i];
-        key[i] = !((open >> i) & 1) ? 0. : by_logit ? x : a.sigmoid ? 1. / (1. + exp(-x)) : exp(x - (double)top);
-        total += key[i];
-        idx[i] = e0 + i < a.E ? e0 + i : 0x7fffffff;
-      }
-      if (!by_logit && !a.sigmoid)
-#pragma unroll
-        for (int d = 1; d < L; d <<= 1) total += __shfl_xor(total, d);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        double q = by_logit || a.sigmoid ? key[i] : key[i] / total;
-        if (a.bias && e0 + i < a.E) q += (double)a.bias[e0 + i];
-        key[i] = ((open >> i) & 1) && q == q ? q : -INFINITY;
-      }
-      if (a.groups > 1) {
-        double* keys = (double*)(more + (size_t)wave * route_group_bytes<L>(a.groups));
-        double* score = keys + RPW * PITCH;
-        double* slack = score + RPW * a.groups;
-        uint32_t* stay = (uint32_t*)(slack + RPW);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) keys[sub * PITCH + e0 + i] = key[i];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        route_groups<double>(a, keys, RPW, PITCH, score, stay, slack);
-        const int per = a.E / a.groups;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (e0 + i < a.E && !stay[sub * a.groups + (e0 + i) / per]) { key[i] = -INFINITY; idx[i] = 0x7fffffff; }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      }
-      for (int j = 0; j < a.k; ++j) {
-        double b = key[0];
-        int bi = idx[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i)
-          if (key[i] > b || (key[i] == b && idx[i] < bi)) { b = key[i]; bi = idx[i]; }
-#pragma unroll
-        for (int d = 1; d < L; d <<= 1) {
-          const double ob = __shfl_xor(b, d);
-          const int oi = __shfl_xor(bi, d);
-          if (ob > b || (ob == b && oi < bi)) { b = ob; bi = oi; }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) if (idx[i] == bi) { key[i] = -INFINITY; idx[i] = 0x7fffffff; }
-        if (li == 0 && valid) choice[r * a.k + j] = (uint32_t)bi;
-      }
-    }
+    if (unsure && li == 0 && valid) again[atomicAdd(&n_again, 1)] = r;      // (their order does not matter)
   }
+  __syncthreads();
+  for (int i = wave; i < n_again; i += 4)
+    route_exact_row<T, NP>(a, base + (int64_t)again[i] * a.l_rs, by_logit, more, choice + again[i] * a.k);
   __syncthreads();
 
   // weights: a thread per choice, scores taken again from the logits
@@ -393,22 +465,26 @@ template <int T, int L> __global__ __launch_bounds__(256) void route_kernel(cons
   route_place(a, choice, count, n, (int)first);
 }
 
-// counts [blocks + 1][E] of a sample: each workgroup's -> the workgroups' before it, and the sum in the last row.  16 experts per workgroup, 16 runs of rows.
+// counts [blocks + 1][E] of a sample: each workgroup's -> the workgroups' before it, and the sum in the last row.  4 experts per workgroup, 64 runs of rows (16 and 16
+// took 13 us for 512 x 256: their loads waited for one another).
 __global__ __launch_bounds__(256) void route_scan_kernel(const RouteArgs a) {
-  __shared__ int run[16][17];
-  const int e = blockIdx.x * 16 + (threadIdx.x & 15), r = threadIdx.x >> 4, per = (a.blocks + 15) / 16;
+  __shared__ int sums[4][4];
+  const int col = threadIdx.x & 3, r = threadIdx.x >> 2, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, e = blockIdx.x * 4 + col, per = (a.blocks + 63) / 64;
   int32_t* c = a.counts + (int64_t)blockIdx.y * (a.blocks + 1) * a.E + e;
-  const int b0 = r * per, b1 = min(a.blocks, b0 + per);
+  const int b0 = r * per, b1 = e < a.E ? min(a.blocks, b0 + per) : 0;
   int sum = 0;
-  if (e < a.E)
-    for (int b = b0; b < b1; ++b) sum += c[(int64_t)b * a.E];
-  run[r][threadIdx.x & 15] = sum;
+#pragma unroll 8
+  for (int b = b0; b < b1; ++b) sum += c[(int64_t)b * a.E];
+  int incl = sum;
+#pragma unroll
+  for (int d = 4; d < 64; d <<= 1) { const int u = __shfl_up(incl, d); if (lane >= d) incl += u; }
+  if (lane >= 60) sums[wave][col] = incl;
   __syncthreads();
-  if (e >= a.E) return;
-  int at = 0, all = 0;
-  for (int i = 0; i < 16; ++i) { const int v = run[i][threadIdx.x & 15]; at += i < r ? v : 0; all += v; }
+  int at = incl - sum;
+  for (int i = 0; i < wave; ++i) at += sums[i][col];
+  if (r == 63 && e < a.E) c[(int64_t)a.blocks * a.E] = at + sum;
+#pragma unroll 8
   for (int b = b0; b < b1; ++b) { const int v = c[(int64_t)b * a.E]; c[(int64_t)b * a.E] = at; at += v; }
-  if (r == 0) c[(int64_t)a.blocks * a.E] = all;
 }
 
 __global__ __launch_bounds__(256) void route_scatter_kernel(const RouteArgs a) {
@@ -453,8 +529,7 @@ __global__ __launch_bounds__(256) void route_scatter_kernel(const RouteArgs a) {
 
 template <int T, int L> int launch_route_as(const RouteArgs& a, hipStream_t st) {
   static std::atomic<uint64_t> attr{0};
-  const int waves = L < 4 ? L : 4;                              // 64 / L rows each: that many have rows
-  const int lds = ROUTE_ROWS * a.k * 8 + a.E * 20 + 16 + (a.groups > 1 ? waves * route_group_bytes<L>(a.groups) : 0);
+  const int lds = ROUTE_ROWS * a.k * 8 + a.E * 20 + 16 + (a.groups > 1 ? 4 * route_group_bytes<L>(a.groups) : 0);
   if (int rc = qbnn_ensure_dyn_lds((const void*)route_kernel<T, L>, &attr, 128 * 1024)) return rc;
   hipLaunchKernelGGL((route_kernel<T, L>), dim3((unsigned)a.blocks, (unsigned)a.S), dim3(256), lds, st, a);
   return qbnn_check_launch_msg("qbnn_route_experts");
@@ -470,7 +545,7 @@ template <int T> int launch_route(const RouteArgs& a, hipStream_t st) {
   else rc = launch_route_as<T, 64>(a, st);
   if (rc || a.blocks == 1) return rc;
   if (a.blocks > ROUTE_BLOCKS) {
-    hipLaunchKernelGGL(route_scan_kernel, dim3((unsigned)((a.E + 15) / 16), (unsigned)a.S), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(route_scan_kernel, dim3((unsigned)((a.E + 3) / 4), (unsigned)a.S), dim3(256), 0, st, a);
     if ((rc = qbnn_check_launch_msg("qbnn_route_experts (scan)"))) return rc;
   }
   hipLaunchKernelGGL(route_scatter_kernel, dim3((unsigned)a.blocks, (unsigned)a.S), dim3(256), ROUTE_ROWS * a.k * 4 + a.E * 24, st, a);
