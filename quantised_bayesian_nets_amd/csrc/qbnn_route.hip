@@ -76,18 +76,27 @@ __device__ __forceinline__ float route_value(uint32_t o) { return __uint_as_floa
 // What a group of keys counts: its two largest summed, masked ones left out; a group of masked keys ranks last.
 template <class FLT> __device__ __forceinline__ FLT route_score(FLT a1, FLT a2) { return a1 == -INFINITY ? a1 : a2 == -INFINITY ? a1 : a1 + a2; }
 
-// score[row][group] of the wave's rows from their keys in LDS, a lane per (row, group)
+// score[row][group] of the wave's rows from their keys in LDS, 2^parts lanes per (row, group)
 template <class FLT> __device__ __forceinline__ void route_group_scores(const RouteArgs& a, const FLT* keys, int rows, int pitch, FLT* score) {
-  const int per = a.E / a.groups;
-  for (int q = threadIdx.x & 63; q < rows * a.groups; q += 64) {
+  const int per = a.E / a.groups, lane = threadIdx.x & 63;
+  int parts = 0;
+  while ((rows * a.groups << (parts + 1)) <= 64) ++parts;
+  for (int q = lane >> parts; q < rows * a.groups; q += 64 >> parts) {
     const int r = q / a.groups, g = q - r * a.groups;
     const FLT* k = keys + r * pitch + g * per;
     FLT a1 = -INFINITY, a2 = -INFINITY;
-    for (int i = 0; i < per; ++i) {
+#pragma unroll 4
+    for (int i = lane & ((1 << parts) - 1); i < per; i += 1 << parts) {
       const FLT v = k[i];
-      if (v > a1) { a2 = a1; a1 = v; } else if (v > a2) a2 = v;
+      a2 = fmax(a2, fmin(a1, v));
+      a1 = fmax(a1, v);
     }
-    score[q] = route_score(a1, a2);
+    for (int d = 0; d < parts; ++d) {
+      const FLT b1 = __shfl_xor(a1, 1 << d), b2 = __shfl_xor(a2, 1 << d);
+      a2 = fmax(fmin(a1, b1), fmax(a2, b2));
+      a1 = fmax(a1, b1);
+    }
+    if ((lane & ((1 << parts) - 1)) == 0) score[q] = route_score(a1, a2);
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
@@ -98,6 +107,7 @@ template <class FLT> __device__ __forceinline__ void route_keep_groups(const Rou
     const FLT mine = score[q];
     int rank = 0;
     FLT next = -INFINITY;                                       // the best score behind mine
+#pragma unroll 4
     for (int i = 0; i < a.groups; ++i) {
       const FLT o = score[r * a.groups + i];
       const bool ahead = o > mine || (o == mine && i < g);
@@ -121,7 +131,7 @@ __device__ __forceinline__ void route_count(const uint32_t* choice, int* count, 
 }
 // exclusive prefix over E values, four per thread and pass; at(e) reads, put(e, prefix) takes
 template <class At, class Put> __device__ __forceinline__ void route_prefix(int E, At at, Put put) {
-  __shared__ int sums[4];
+  __shared__ int sums[8];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, e0 = threadIdx.x * 4;
   int v[4], mine = 0;
 #pragma unroll
@@ -162,7 +172,7 @@ __device__ __forceinline__ void route_place(const RouteArgs& a, const uint32_t* 
 }
 // start(e): position of the workgroup's first choice of e -> the quarters' own positions
 template <class F> __device__ __forceinline__ void route_starts(int* count, int E, F start) {
-  for (int e = threadIdx.x; e < E; e += 256) {
+  for (int e = threadIdx.x; e < E; e += blockDim.x) {
     int run = start(e);
 #pragma unroll
     for (int w = 0; w < 4; ++w) { const int c = count[w * E + e]; count[w * E + e] = run; run += c; }
@@ -170,58 +180,63 @@ template <class F> __device__ __forceinline__ void route_starts(int* count, int 
   __syncthreads();
 }
 
-// LDS of a wave for its rows' groups: fp32 keys [64 / L][L 16 + 2] where a group is no power of two, scores, masks and slack of 64 / L rows; 64-bit ones of one row
-template <int L> __host__ __device__ constexpr int route_group_bytes(int groups) {
-  const int fast = (64 / L) * ((L * 16 + 2 + 2 * groups) * 4 + 4), exact = ((L < 4 ? 64 : L * 16) + 1) * 8 + groups * 12;
+__host__ __device__ __forceinline__ bool route_whole(const RouteArgs& a) { const int per = a.E / a.groups; return per >= 16 && (per & (per - 1)) == 0; }
+// LDS of a wave: for its rows' groups fp32 keys [64 / L][L 16 + 2] where a group is not whole lanes, scores, masks and slack of 64 / L rows; or 64-bit ones of one row
+template <int L> __host__ __device__ constexpr int route_wave_bytes(int groups, bool whole) {
+  const int fast = groups > 1 ? (64 / L) * (((whole ? 0 : L * 16 + 2) + 2 * groups) * 4 + 4) : 0, exact = (L * 16 + 1) * 8 + groups * 12;
   return ((fast > exact ? fast : exact) + 15) & ~15;
 }
 
-// One row by a whole wave with 64-bit keys, NP experts per lane.
-template <int T, int NP> __device__ __forceinline__ void route_exact_row(const RouteArgs& a, const f8_type<T>* l, bool by_logit, uint8_t* more, uint32_t* choice) {
-  const int lane = threadIdx.x & 63;
-  double key[NP], top = -INFINITY, total = 0.;
-  int idx[NP];
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    idx[i] = i * 64 + lane < a.E ? i * 64 + lane : 0x7fffffff;
-    const float v = i * 64 + lane < a.E ? f8_load<T>(l[i * 64 + lane]) : -INFINITY;
-    key[i] = v > route_lowest<T>() ? (double)v : -INFINITY;     // (false for NaN)
-    top = fmax(top, key[i]);
+// One step of a choice over a wave: the larger key, and of equal ones the lower index
+template <int STEP> __device__ __forceinline__ void route_join(double& b, int& bi) {
+  const double ob = __hiloint2double((int)route_partner<STEP>((uint32_t)__double2hiint(b)), (int)route_partner<STEP>((uint32_t)__double2loint(b)));
+  const int oi = (int)route_partner<STEP>((uint32_t)bi);
+  if (ob > b || (ob == b && oi < bi)) { b = ob; bi = oi; }
+}
+
+// One row by a whole wave with 64-bit keys, NP experts per lane.  They are made one by one, through LDS: NP exponentials at once would halve the waves of the fast pass.
+template <int T, int NP> __device__ __forceinline__ void route_exact_row(const RouteArgs& a, const f8_type<T>* l, bool by_logit, double* keys, double* score, uint32_t* choice) {
+  const int lane = threadIdx.x & 63, per = a.E / a.groups;
+  double* slack = score + a.groups;
+  uint32_t* stay = (uint32_t*)(slack + 1);
+  double top = -INFINITY, total = 0.;
+#pragma unroll 1
+  for (int e = lane; e < a.E; e += 64) {
+    const float v = f8_load<T>(l[e]);
+    keys[e] = v > route_lowest<T>() ? (double)v : -INFINITY;    // (false for NaN)
+    top = fmax(top, keys[e]);
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = fmax(top, __shfl_xor(top, d));
   if (!by_logit) {
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const bool open = key[i] > -INFINITY;
-      key[i] = !open ? -1. : a.sigmoid ? 1. / (1. + exp(-key[i])) : exp(key[i] - top);
-      total += open ? key[i] : 0.;
+#pragma unroll 1
+    for (int e = lane; e < a.E; e += 64) {
+      const double x = keys[e], z = exp(a.sigmoid ? -x : x - top), p = a.sigmoid ? 1. / (1. + z) : z;
+      keys[e] = x > -INFINITY ? p : -1.;
+      total += x > -INFINITY ? p : 0.;
     }
-    if (!a.sigmoid)
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      double q = a.sigmoid ? key[i] : key[i] / total;
-      if (a.bias && i * 64 + lane < a.E) q += (double)a.bias[i * 64 + lane];
-      key[i] = key[i] >= 0. && q == q ? q : -INFINITY;
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+    total = a.sigmoid ? 1. : 1. / total;
+#pragma unroll 1
+    for (int e = lane; e < a.E; e += 64) {
+      const double p = keys[e], q = p * total + (a.bias ? (double)a.bias[e] : 0.);
+      keys[e] = p >= 0. && q == q ? q : -INFINITY;
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (a.groups > 1) {
-      double* keys = (double*)more;
-      double* score = keys + NP * 64;
-      double* slack = score + a.groups;
-      uint32_t* stay = (uint32_t*)(slack + 1);
-#pragma unroll
-      for (int i = 0; i < NP; ++i) if (i * 64 + lane < a.E) keys[i * 64 + lane] = key[i];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       route_group_scores<double>(a, keys, 1, 0, score);
       route_keep_groups<double>(a, 1, score, stay, slack);
-      const int per = a.E / a.groups;
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        if (idx[i] < a.E && !stay[idx[i] / per]) { key[i] = -INFINITY; idx[i] = 0x7fffffff; }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
+  }
+  double key[NP];
+  int idx[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int e = i * 64 + lane;
+    const bool in = e < a.E && (a.groups == 1 || stay[e / per]);
+    key[i] = in ? keys[e] : -INFINITY;
+    idx[i] = in ? e : 0x7fffffff;
   }
   for (int j = 0; j < a.k; ++j) {
     double b = key[0];
@@ -229,16 +244,17 @@ template <int T, int NP> __device__ __forceinline__ void route_exact_row(const R
 #pragma unroll
     for (int i = 1; i < NP; ++i)
       if (key[i] > b || (key[i] == b && idx[i] < bi)) { b = key[i]; bi = idx[i]; }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double ob = __shfl_xor(b, d);
-      const int oi = __shfl_xor(bi, d);
-      if (ob > b || (ob == b && oi < bi)) { b = ob; bi = oi; }
-    }
+    route_join<1>(b, bi);
+    route_join<2>(b, bi);
+    route_join<4>(b, bi);
+    route_join<8>(b, bi);
+    route_join<16>(b, bi);
+    route_join<32>(b, bi);
 #pragma unroll
     for (int i = 0; i < NP; ++i) if (idx[i] == bi) { key[i] = -INFINITY; idx[i] = 0x7fffffff; }
     if (lane == 0) choice[j] = (uint32_t)bi;
   }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 // L lanes per row, 16 neighbouring experts per lane.
@@ -252,13 +268,20 @@ template <int T, int NP> __device__ __forceinline__ void route_exact_row(const R
 // Bound: a round is 24 + 12 instructions for 64 / L rows; 32768 x 256 logits are 5 us of reading.
 constexpr uint32_t ROUTE_MASKED = 0x00800000u;                  // the order of the lowest finite float: masked experts lie below
 
-template <int T, int L> __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
-  constexpr int RPW = 64 / L;                                   // rows per wave
-  constexpr int PITCH = L * 16 + 2;
+// Waves of a workgroup: 64 rows are 64 L / 64 of them, done in turn by 4 where that is all and by 8 where there are more
+constexpr int route_waves(int L) { return L < 8 ? 4 : 8; }
+
+// KEY: what is compared
+enum { KEY_LOGIT, KEY_SIGMOID, KEY_SOFTMAX };
+
+template <int T, int L, int KEY> __global__ __launch_bounds__(route_waves(L) * 64, L >= 8 ? 4 : 2) void route_kernel(const RouteArgs a) {
+  constexpr int RPW = 64 / L, NW = route_waves(L);              // rows per wave, waves
   constexpr int NP = L < 4 ? 1 : L / 4;                         // experts per lane where a wave does one row
+  constexpr int PITCH = L * 16 + 2;
   extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
   __shared__ float row_top[ROUTE_ROWS], row_sum[ROUTE_ROWS];
   __shared__ int again[ROUTE_ROWS], n_again;
+  __shared__ __attribute__((aligned(16))) float bias[KEY == KEY_LOGIT ? 1 : L * 16];
   // dynamic: choices and their scores [64][k], the quarters' counts [4][E], starts [E], and with groups each wave's keys, scores, masks
   uint32_t* choice = (uint32_t*)dyn;
   float* part = (float*)(choice + ROUTE_ROWS * a.k);
@@ -267,94 +290,98 @@ template <int T, int L> __global__ __launch_bounds__(256) void route_kernel(cons
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / L, li = lane % L;
   uint8_t* more = (uint8_t*)(start + a.E);
   more += (-(uintptr_t)more) & 15;
-  more += (size_t)wave * route_group_bytes<L>(a.groups);
+
   const int s = blockIdx.y, t0 = blockIdx.x * ROUTE_ROWS, rows = min(a.T - t0, ROUTE_ROWS);
-  const bool by_logit = !a.bias && a.groups == 1;               // both scores increase with the logit
-  const bool exact = by_logit && T != QBNN_F32;
+  constexpr bool exact = KEY == KEY_LOGIT && T != QBNN_F32;
   const uint32_t low = exact ? (1u << a.bits) - 1 : 15u;
   const f8_type<T>* base = (const f8_type<T>*)a.logits + s * a.l_ss + t0 * a.l_rs;
-  for (int i = threadIdx.x; i < 4 * a.E; i += 256) count[i] = 0;
+  for (int i = threadIdx.x; i < 4 * a.E; i += NW * 64) count[i] = 0;
+  if constexpr (KEY != KEY_LOGIT)                               // (each lane's 16 straight from memory: 16 loads of 16 lines each, by every wave)
+    for (int i = threadIdx.x; i < L * 16; i += NW * 64) {
+      const float b = a.bias && i < a.E ? a.bias[i] : 0.f;
+      bias[i] = b == b ? b : -INFINITY;
+    }
   if (threadIdx.x == 0) n_again = 0;
   __syncthreads();
 
-  for (int r0 = wave * RPW; r0 < rows; r0 += 4 * RPW) {
-    const int r = r0 + sub, e0 = li * 16;
+  int e0 = li * 16;
+  const int per = KEY == KEY_LOGIT ? a.E : a.E / a.groups, g0 = e0 / per, p0 = e0 - g0 * per;      // the lane's first group, and the place in it
+  const bool whole = route_whole(a);                            // a group is whole lanes (and a power of two of them): its two largest without LDS
+  more += (size_t)wave * route_wave_bytes<L>(a.groups, whole);
+  for (int r0 = wave * RPW; r0 < rows; r0 += NW * RPW) {
+    asm volatile("" : "+v"(e0));                                // (or 16 of everything that depends on it alone are kept over the loop: 50 registers)
+    const int r = r0 + sub;
     const bool valid = r < rows;
-    const f8_type<T>* l = base + (int64_t)min(r, rows - 1) * a.l_rs + e0;
+    const f8_type<T>* l = base + (int64_t)min(r, rows - 1) * a.l_rs;
+    f8_type<T> raw[16];
+    if (e0 + 16 <= a.E) __builtin_memcpy(raw, l + e0, sizeof(raw));
+    else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) raw[i] = l[min(e0 + i, a.E - 1)];
+    }
     float v[16];
-    if (e0 + 16 <= a.E) {
-      f8_type<T> raw[16];
-      __builtin_memcpy(raw, l, sizeof(raw));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = f8_load<T>(raw[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = e0 + i < a.E ? f8_load<T>(l[i]) : -INFINITY;
-    }
+    for (int i = 0; i < 16; ++i) v[i] = e0 + i < a.E ? f8_load<T>(raw[i]) : -INFINITY;
     bool nan = false;
-    float top = -INFINITY;
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      nan |= v[i] != v[i];
-      v[i] = v[i] > route_lowest<T>() ? v[i] : -INFINITY;       // masked: -inf, the type's lowest value and NaN
-      top = fmaxf(top, v[i]);
+    for (int i = 0; i < 16; ++i) nan |= v[i] != v[i];
+    if (!a.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, v[i] > route_lowest<T>() ? v[i] : -INFINITY);
+      top = route_maxf<L>(top);
     }
-    top = route_maxf<L>(top);
     uint32_t w[16];
     bool unsure = false;
-    float sum = 0.f, worst = 0.f;                               // worst: the error of two keys' difference
-    if (by_logit) {
+    float worst = 0.f;                                          // two scores' errors
+    if constexpr (KEY == KEY_LOGIT) {
       if (!a.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum += v[i] > -INFINITY ? route_exp(v[i] - top) : 0.f;
+        for (int i = 0; i < 16; ++i) sum += v[i] > route_lowest<T>() ? route_exp(v[i] - top) : 0.f;
         sum = route_sumf<L>(sum);
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t place = exact ? low - (uint32_t)(e0 + i) : 15u - i;
-        w[i] = v[i] > -INFINITY ? (route_order(v[i] + 0.f) & ~low) | place : e0 + i < a.E ? (uint32_t)(a.E - e0 - i) : 0u;      // (-0 ties with 0)
+      for (int i = 0; i < 16; ++i) {                            // (-0 ties with 0)
+        const uint32_t order = (route_order(v[i] + 0.f) & ~low) | (exact ? low - (uint32_t)(e0 + i) : 15u - i);
+        w[i] = v[i] > route_lowest<T>() ? order : (uint32_t)max(a.E - e0 - i, 0);
       }
     } else {
-      // p off by at most p (|x| + c) 2^-23.  Sigmoid: 1 + z, its reciprocal and exp's (|x| + 2): c = 5, 8 taken.  Softmax: exp's |x| + 3, the sum's: 15 + 6
-      // additions (11) and its terms' own (sum p |x| <= ln E < 7, and 3): c = 26, 32 taken.  Adding the bias: half a step of the key.
-      float key[16], large = 0.f;
-      const float c = a.sigmoid ? 8.f : 32.f;
+      // exp is off by (|x| + 2) 2^-23 of it.  Sigmoid: p (1 - p) |x| < 0.23, p (1 - p) <= 1/4, 1 + z half a step, its reciprocal one: 2.3 2^-23, 3 taken.
+      // Softmax, x = v - top <= 0 off by half a step, p <= 1 / sum: a term by (1.5 |x| + 2), e^x |x| < 0.37; the sum by 15 + 6 additions (10.5) and its terms'
+      // own (sum p |x| <= ln E < 7: 12.5); the reciprocal and the product 1.5: 27.1 2^-23 / sum, 32 taken.
+      constexpr bool SIG = KEY == KEY_SIGMOID;
+      float key[16];
+      if constexpr (SIG) {
+        worst = 2 * 3 * 1.1920929e-7f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float z = route_exp(a.sigmoid ? -v[i] : v[i] - top);
-        key[i] = v[i] > -INFINITY ? (a.sigmoid ? __builtin_amdgcn_rcpf(1.f + z) : z) : 0.f;
-        sum += key[i];
-      }
-      if (!a.sigmoid) sum = route_sumf<L>(sum);
-      const float over = a.sigmoid ? 1.f : __builtin_amdgcn_rcpf(sum);
+        for (int i = 0; i < 16; ++i) key[i] = v[i] > route_lowest<T>() ? __builtin_amdgcn_rcpf(1.f + route_exp(-v[i])) + bias[e0 + i] : -INFINITY;
+      } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = key[i] * over;
-        const float q = p + (a.bias && e0 + i < a.E ? a.bias[e0 + i] : 0.f);
-        key[i] = v[i] > -INFINITY && q == q ? q : -INFINITY;
-        const float off = p * (fabsf(a.sigmoid ? v[i] : v[i] - top) + c);
-        worst = key[i] > -INFINITY ? fmaxf(worst, off) : worst;
-        large = key[i] > -INFINITY ? fmaxf(large, fabsf(key[i])) : large;
+        for (int i = 0; i < 16; ++i) {
+          key[i] = v[i] > route_lowest<T>() ? route_exp(v[i] - top) : 0.f;
+          sum += key[i];
+        }
+        sum = route_sumf<L>(sum);
+        const float over = __builtin_amdgcn_rcpf(sum);
+        worst = 2 * 32 * 1.1920929e-7f * over;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float q = key[i] * over + bias[e0 + i];
+          key[i] = v[i] > route_lowest<T>() && q == q ? q : -INFINITY;
+        }
       }
-      large = route_maxf<L>(large);
-      worst = (route_maxf<L>(worst) + large) * 2.384185791015625e-7f;
-      unsure = !(worst < INFINITY);
       uint32_t in = 0xffffu;
       if (a.groups > 1) {
-        const int per = a.E / a.groups;
         float* score = (float*)more;                            // [RPW][groups]
         uint32_t* stay = (uint32_t*)(score + RPW * a.groups);
         float* slack = (float*)(stay + RPW * a.groups);
-        if ((per & (per - 1)) == 0) {                           // a lane holds whole groups, or a group whole lanes: in registers
+        float large = 0.f;                                      // the largest key that counts
+        if (whole) {
           float a1 = -INFINITY, a2 = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             a2 = __builtin_amdgcn_fmed3f(a1, a2, key[i]);
             a1 = fmaxf(a1, key[i]);
-            if (per < 16 && ((i + 1) & (per - 1)) == 0) {
-              if (e0 + i < a.E) score[sub * a.groups + (e0 + i) / (unsigned)per] = route_score(a1, a2);
-              a1 = a2 = -INFINITY;
-            }
           }
           auto join = [&](uint32_t p1, uint32_t p2) {
             const float b1 = __uint_as_float(p1), b2 = __uint_as_float(p2);
@@ -366,29 +393,37 @@ template <int T, int L> __global__ __launch_bounds__(256) void route_kernel(cons
           if (L > 4 && per > 64) join(route_partner<4>(__float_as_uint(a1)), route_partner<4>(__float_as_uint(a2)));
           if (L > 8 && per > 128) join(route_partner<8>(__float_as_uint(a1)), route_partner<8>(__float_as_uint(a2)));
           if (L > 16 && per > 256) join(route_partner<16>(__float_as_uint(a1)), route_partner<16>(__float_as_uint(a2)));
-          if (per >= 16 && (e0 & (per - 1)) == 0 && e0 < a.E) score[sub * a.groups + e0 / (unsigned)per] = route_score(a1, a2);
+          large = fmaxf(a1 > -INFINITY ? fabsf(a1) : 0.f, a2 > -INFINITY ? fabsf(a2) : 0.f);
+          if (p0 == 0 && e0 < a.E) score[sub * a.groups + g0] = route_score(a1, a2);
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         } else {
           float* keys = slack + RPW;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) keys[sub * PITCH + e0 + i] = key[i];
+          for (int i = 0; i < 16; ++i) {
+            keys[sub * PITCH + e0 + i] = e0 + i < a.E ? key[i] : -INFINITY;
+            large = e0 + i < a.E && key[i] > -INFINITY ? fmaxf(large, fabsf(key[i])) : large;
+          }
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           route_group_scores<float>(a, keys, RPW, PITCH, score);
         }
         route_keep_groups<float>(a, RPW, score, stay, slack);
-        unsure |= !(slack[sub] > 2.f * worst + large * 4.8e-7f);
-        if (per >= 16 && (per & (per - 1)) == 0) in = e0 < a.E && stay[sub * a.groups + e0 / (unsigned)per] ? 0xffffu : 0u;
+        // sums of two keys each (score and bias), and the sums' rounding
+        unsure |= !(slack[sub] > 2.f * worst + route_maxf<L>(large) * 9.6e-7f);
+        if (whole) in = e0 < a.E && stay[sub * a.groups + g0] ? 0xffffu : 0u;
         else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (e0 + i < a.E && !stay[sub * a.groups + (e0 + i) / (unsigned)per]) in &= ~(1u << i);
+          for (int i = 0, g = g0, p = p0; i < 16; ++i) {
+            in ^= (stay[sub * a.groups + min(g, a.groups - 1)] ^ 1u) << i;
+            g += p + 1 == per ? 1 : 0;
+            p = p + 1 == per ? 0 : p + 1;
+          }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const uint32_t order = key[i] > -INFINITY ? (route_order(key[i]) & ~15u) | (15u - i) : (uint32_t)(a.E - e0 - i);
-        w[i] = e0 + i < a.E && ((in >> i) & 1) ? order : 0u;
+        const uint32_t order = (route_order(key[i]) & ~15u) | (15u - i);
+        w[i] = (key[i] > -INFINITY ? order : (uint32_t)max(a.E - e0 - i, 0)) & (uint32_t)((int)(in << (31 - i)) >> 31);
       }
     }
     if (li == 0 && valid) {
@@ -399,6 +434,7 @@ template <int T, int L> __global__ __launch_bounds__(256) void route_kernel(cons
 
     // k rounds, and one more to see that the last choice was none too close
     uint32_t before = 0;
+    float above = 0.f;
     for (int j = 0; j < a.k + (exact ? 0 : 1); ++j) {
       const uint32_t c = before - 1;
       uint32_t near = 0xffffffffu;
@@ -414,23 +450,28 @@ template <int T, int L> __global__ __launch_bounds__(256) void route_kernel(cons
           if (__popcll(owners) != RPW) unsure |= __popcll((owners >> (sub * L % 64)) & (L < 64 ? (1ull << (L % 64)) - 1 : ~0ull)) > 1;
         }
       }
-      if (!exact && j > 0 && m >= ROUTE_MASKED) {
-        if (by_logit) unsure |= ((before ^ m) & ~15u) == 0;
-        else unsure |= !(route_value(before & ~15u) - route_value(m | 15u) > worst);
+      if constexpr (KEY == KEY_LOGIT) {
+        if (!exact && j > 0 && m >= ROUTE_MASKED) unsure |= ((before ^ m) & ~15u) == 0;
+      } else {                                                  // each key gave up 15 last places at most and its bias half of one: 16 2^-23 of it
+        const float at = route_value(m);
+        if (j > 0 && m >= ROUTE_MASKED) unsure |= !(above - at > __builtin_fmaf(fmaxf(fabsf(above), fabsf(at)), 32 * 1.1920929e-7f, worst));
+        above = at;
       }
       before = m;
     }
     if (unsure && li == 0 && valid) again[atomicAdd(&n_again, 1)] = r;      // (their order does not matter)
   }
   __syncthreads();
-  for (int i = wave; i < n_again; i += 4)
-    route_exact_row<T, NP>(a, base + (int64_t)again[i] * a.l_rs, by_logit, more, choice + again[i] * a.k);
-  __syncthreads();
+  if constexpr (!exact) {
+    for (int i = wave; i < n_again; i += NW)
+      route_exact_row<T, NP>(a, base + (int64_t)again[i] * a.l_rs, KEY == KEY_LOGIT, (double*)more, (double*)more + L * 16, choice + again[i] * a.k);
+    __syncthreads();
+  }
 
   // weights: a thread per choice, scores taken again from the logits
   const int n = rows * a.k;
   const int64_t first = ((int64_t)s * a.T + t0) * a.k;
-  for (int i = threadIdx.x; i < n; i += 256) {
+  for (int i = threadIdx.x; i < n; i += NW * 64) {
     const int r = i / a.k, e = (int)choice[i];
     const float l = f8_load<T>(base[(int64_t)r * a.l_rs + e]), top = row_top[r];
     float p = a.sigmoid ? 1.f / (1.f + route_exp(-l)) : route_exp(l - top) / row_sum[r];
@@ -439,7 +480,7 @@ template <int T, int L> __global__ __launch_bounds__(256) void route_kernel(cons
     part[i] = p;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += 256) {
+  for (int i = threadIdx.x; i < n; i += NW * 64) {
     float p = part[i];
     if (a.renorm) {
       const int r = i / a.k;
@@ -454,7 +495,7 @@ template <int T, int L> __global__ __launch_bounds__(256) void route_kernel(cons
   auto total = [&](int e) { return count[e] + count[a.E + e] + count[2 * a.E + e] + count[3 * a.E + e]; };
   if (a.blocks > 1) {
     int32_t* out = a.counts + ((int64_t)s * (a.blocks + 1) + blockIdx.x) * a.E;
-    for (int e = threadIdx.x; e < a.E; e += 256) out[e] = total(e);
+    for (int e = threadIdx.x; e < a.E; e += NW * 64) out[e] = total(e);
     return;
   }
   const int all = s * a.T * a.k;
@@ -527,12 +568,16 @@ __global__ __launch_bounds__(256) void route_scatter_kernel(const RouteArgs a) {
   route_place(a, choice, count, n, (int)first);
 }
 
-template <int T, int L> int launch_route_as(const RouteArgs& a, hipStream_t st) {
+template <int T, int L, int KEY> int launch_route_by(const RouteArgs& a, hipStream_t st) {
   static std::atomic<uint64_t> attr{0};
-  const int lds = ROUTE_ROWS * a.k * 8 + a.E * 20 + 16 + (a.groups > 1 ? 4 * route_group_bytes<L>(a.groups) : 0);
-  if (int rc = qbnn_ensure_dyn_lds((const void*)route_kernel<T, L>, &attr, 128 * 1024)) return rc;
-  hipLaunchKernelGGL((route_kernel<T, L>), dim3((unsigned)a.blocks, (unsigned)a.S), dim3(256), lds, st, a);
+  const int lds = ROUTE_ROWS * a.k * 8 + a.E * 20 + 16 + (KEY == KEY_LOGIT && T != QBNN_F32 ? 0 : route_waves(L) * route_wave_bytes<L>(a.groups, route_whole(a)));
+  if (int rc = qbnn_ensure_dyn_lds((const void*)route_kernel<T, L, KEY>, &attr, 128 * 1024)) return rc;
+  hipLaunchKernelGGL((route_kernel<T, L, KEY>), dim3((unsigned)a.blocks, (unsigned)a.S), dim3(route_waves(L) * 64), lds, st, a);
   return qbnn_check_launch_msg("qbnn_route_experts");
+}
+template <int T, int L> int launch_route_as(const RouteArgs& a, hipStream_t st) {
+  if (!a.bias && a.groups == 1) return launch_route_by<T, L, KEY_LOGIT>(a, st);      // both scores increase with the logit
+  return a.sigmoid ? launch_route_by<T, L, KEY_SIGMOID>(a, st) : launch_route_by<T, L, KEY_SOFTMAX>(a, st);
 }
 template <int T> int launch_route(const RouteArgs& a, hipStream_t st) {
   int rc;
