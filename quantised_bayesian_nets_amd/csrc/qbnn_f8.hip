@@ -41,6 +41,9 @@ static void f8_magic(uint32_t d, uint32_t& magic, int& shift) {
 }
 __device__ __forceinline__ uint32_t f8_divide(uint32_t n, uint32_t magic, int shift) { return (uint32_t)(((uint64_t)n * magic) >> (31 + shift)); }
 
+// A 16-bit result with block exponents, as the experts' sums take it: fp16 of v 2^-e, e the block's exponent as of e4m3 (so at most 448; inf and NaN stay)
+constexpr int F8_HALF = 4;
+
 // 8 columns from `col` of a row of K (zeros behind the last); rows may start at any element's address
 template <int T> __device__ __forceinline__ void f8_load8(const f8_type<T>* row, int col, int K, float (&v)[8]) {
   if (col + 8 <= K) {
@@ -493,18 +496,31 @@ __device__ __forceinline__ void f8_finish_as(const F8Args& a, const F8Tile& t, i
 #pragma unroll
             for (int c = 0; c < 8; ++c) v[c] = s == 0.f ? 0.f : v[c] * s;
           }
-          f8_type<OUT>* y = (f8_type<OUT>*)a.y + (int64_t)t.sample * a.y_ss + to * a.y_rs + nw + n;
+          if constexpr (OUT == F8_HALF) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) if (!WHOLE && c >= in) v[c] = 0.f;
+            const int e = f8_exponent(f8_max16(f8_max8(v)));
+            const float down = f8_pow2(-e);
+            f8_v4i o;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[c] = f8_store2<QBNN_F16>(v[2 * c] * down, v[2 * c + 1] * down);
+            *(f8_v4i*)(a.y + (to * a.y_rs + nw + n) * 2) = o;
+            if (n == 0) a.ye[to * a.ye_rs + (nw >> 7)] = (uint8_t)(e + 127);
+            continue;
+          }
+          typedef f8_type<OUT == F8_HALF ? QBNN_F16 : OUT> Out;
+          Out* y = (Out*)a.y + (int64_t)t.sample * a.y_ss + to * a.y_rs + nw + n;
           if (!WHOLE && in < 8) {                               // the lane at the end: its values by way of the stage, one by one
             *(f8_v4f*)(st + r * F8_PITCH + n) = (f8_v4f){v[0], v[1], v[2], v[3]};
             *(f8_v4f*)(st + r * F8_PITCH + n + 4) = (f8_v4f){v[4], v[5], v[6], v[7]};
 #pragma unroll 1
-            for (int c = 0; c < in; ++c) y[c] = f8_store<OUT>(st[r * F8_PITCH + n + c]);
+            for (int c = 0; c < in; ++c) y[c] = f8_store<OUT == F8_HALF ? QBNN_F16 : OUT>(st[r * F8_PITCH + n + c]);
           } else if constexpr (OUT == QBNN_F32) {
             __builtin_memcpy(y, v, sizeof(v));
           } else {
             f8_v4i o;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) o[c] = f8_store2<OUT>(v[2 * c], v[2 * c + 1]);
+            for (int c = 0; c < 4; ++c) o[c] = f8_store2<OUT == F8_HALF ? QBNN_F16 : OUT>(v[2 * c], v[2 * c + 1]);
             __builtin_memcpy(y, &o, sizeof(o));
           }
         }
@@ -879,22 +895,26 @@ template <int OUT, bool GROUPED> int launch_big(const F8Args& a, int rows, int z
   return qbnn_check_launch_msg("qbnn_linear_f8");
 }
 
-// rows: the rows of one sample, or all routed rows
+// Whether the products go through LDS tiles.  rows: the rows of one sample, or all routed rows.  Offsets are 32 bits wide there: of a gathered row's bytes from the
+// first, of any row's exponents, of a weight row's in its tile.
+template <bool GROUPED> int f8_rows_each(const F8Args& a, int rows) { return GROUPED ? (rows + a.groups - 1) / a.groups : rows; }
+template <bool GROUPED> bool f8_tiled(const F8Args& a, int rows) {
+  const int64_t far = GROUPED ? (int64_t)(a.rows ? a.x_rows : rows) * a.Kb * 128 : (int64_t)rows * a.Sp;
+  return f8_rows_each<GROUPED>(a, rows) > 32 && far < ((int64_t)1 << 32) && a.Kb < (1 << 16);
+}
 template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, int rows, int z, hipStream_t st) {
   const int spare = GROUPED ? a.groups : 0;        // each group may end inside a tile
-  const int per = GROUPED ? (rows + a.groups - 1) / a.groups : rows;
-  // offsets are 32 bits wide in the tiled form: of a gathered row's bytes from the first, of any row's exponents, of a weight row's in its tile
-  const int64_t far = GROUPED ? (int64_t)(a.rows ? a.x_rows : rows) * a.Kb * 128 : (int64_t)rows * a.Sp;
-  const bool near = far < ((int64_t)1 << 32) && a.Kb < (1 << 16);
+  const int per = f8_rows_each<GROUPED>(a, rows);
   const auto tiles = [&](int tm, int tn) { return (int64_t)z * ((rows + tm - 1) / tm + spare / 2) * ((a.N + tn - 1) / tn); };
-  if (per > 32 && near) {
+  if (f8_tiled<GROUPED>(a, rows)) {
     if constexpr (!EXACT) {
       if (per > 128 && tiles(256, 256) >= 192) return launch_big<OUT, GROUPED>(a, rows, z, st);
     }
     if (per > 64 && tiles(128, 256) >= 384) return launch_tiled<2, 2, 2, OUT, EXACT, GROUPED>(a, rows, z, st);
     return launch_tiled<1, 2, 1, OUT, EXACT, GROUPED>(a, rows, z, st);
   }
-  if constexpr (OUT == QBNN_F8) {
+  if constexpr (OUT == F8_HALF) return f8_fail("qbnn_experts_f8: no direct form of this result");
+  else if constexpr (OUT == QBNN_F8) {
     if (per <= 16) return launch_direct<1, 8, 4, 2, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
     return launch_direct<2, 8, 4, 1, OUT, EXACT, GROUPED>(a, (rows + 31) / 32 + spare, z, st);
   } else {
@@ -905,13 +925,14 @@ template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, 
     return launch_direct<2, 4, 4, 2, OUT, EXACT, GROUPED>(a, (rows + 31) / 32 + spare, z, st);
   }
 }
-// what the two entries ask for: every type for dense rows (fp32 exact), e4m3 and fp32 of either form for groups
+// what the two entries ask for: every type for dense rows (fp32 exact), e4m3 and fp32 of either form and halves for groups
 template <bool GROUPED> int launch_linear_any(const F8Args& a, int rows, int z, int y_type, int exact, hipStream_t st) {
   switch (y_type) {
     case QBNN_F32: if constexpr (!GROUPED) return launch_linear<QBNN_F32, true, GROUPED>(a, rows, z, st);
       else return exact ? launch_linear<QBNN_F32, true, GROUPED>(a, rows, z, st) : launch_linear<QBNN_F32, false, GROUPED>(a, rows, z, st);
     case QBNN_BF16: if constexpr (!GROUPED) return launch_linear<QBNN_BF16, false, GROUPED>(a, rows, z, st);
     case QBNN_F16: if constexpr (!GROUPED) return launch_linear<QBNN_F16, false, GROUPED>(a, rows, z, st);
+    case F8_HALF: if constexpr (GROUPED) return launch_linear<F8_HALF, false, GROUPED>(a, rows, z, st);
     default:
       if constexpr (GROUPED) { if (exact) return launch_linear<QBNN_F8, true, GROUPED>(a, rows, z, st); }
       return launch_linear<QBNN_F8, false, GROUPED>(a, rows, z, st);
@@ -919,38 +940,52 @@ template <bool GROUPED> int launch_linear_any(const F8Args& a, int rows, int z, 
 }
 
 // ---- y[t] = sum over the row's top_k results, in the order of choice --------------------------------------------------------------
-// The results come in fp32: rounded to 16 bits first, each would cost as much as the one rounding of the sum does.
-template <int T> __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ o, f8_type<T>* __restrict__ y, int rows, int k, int N) {
-  const int n0 = (blockIdx.x * 256 + threadIdx.x) * 4;
+// The results come in fp32: rounded to the 16 bits of y first, each would cost as much as the one rounding of the sum does.  For a bf16 y, halves with block exponents
+// cost 2^-11 of each term beside the sum's 2^-8 and are half of the bytes, which bound this kernel (32768 x 4096: 115 us from fp32).
+constexpr int COMBINE_COLUMNS = 8;
+template <int T, bool HALF> __global__ __launch_bounds__(256) void combine_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__ oe, f8_type<T>* __restrict__ y, int rows, int k, int N) {
+  const int n0 = (blockIdx.x * 256 + threadIdx.x) * COMBINE_COLUMNS;
   const int64_t t = blockIdx.y + (int64_t)blockIdx.z * 32768;
   if (n0 >= N || t >= rows) return;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  const bool whole = n0 + 4 <= N;
+  const int Nb = (N + 127) >> 7;
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const bool whole = n0 + 8 <= N;
+#pragma unroll 4
   for (int j = 0; j < k; ++j) {
-    const float* r = o + (t * k + j) * N + n0;
-    float v[4];
-    if (whole) __builtin_memcpy(v, r, sizeof(v));
-    else
-      for (int i = 0; i < 4; ++i) v[i] = n0 + i < N ? r[i] : 0.f;
+    const int64_t r = t * k + j;
+    if constexpr (HALF) {                                       // (rows are padded to whole blocks)
+      const f8_v4i p = *(const f8_v4i*)(o + (r * (Nb * 128) + n0) * 2);
+      const float up = f8_pow2((int)oe[r * Nb + (n0 >> 7)] - 127);
+      _Float16 h[8];
+      __builtin_memcpy(h, &p, sizeof(h));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] += v[i];
+      for (int i = 0; i < 8; ++i) sum[i] += (float)h[i] * up;
+    } else {
+      const float* p = (const float*)o + r * N + n0;
+      float v[8];
+      if (whole) __builtin_memcpy(v, p, sizeof(v));
+      else
+        for (int i = 0; i < 8; ++i) v[i] = n0 + i < N ? p[i] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += v[i];
+    }
   }
-  f8_type<T> v[4];
+  f8_type<T> v[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = f8_store<T>(sum[i]);
+  for (int i = 0; i < 8; ++i) v[i] = f8_store<T>(sum[i]);
   f8_type<T>* out = y + t * N + n0;
   if (whole) __builtin_memcpy(out, v, sizeof(v));
   else
-    for (int i = 0; i < 4; ++i) if (n0 + i < N) out[i] = v[i];
+    for (int i = 0; i < 8; ++i) if (n0 + i < N) out[i] = v[i];
 }
 
-int launch_combine(const float* o, int rows, int k, int N, void* y, int y_type, hipStream_t st) {
-  const dim3 grid((unsigned)((N + 1023) / 1024), (unsigned)(rows < 32768 ? rows : 32768), (unsigned)((rows + 32767) / 32768));
-  switch (y_type) {
-    case QBNN_F32: hipLaunchKernelGGL((combine_kernel<QBNN_F32>), grid, dim3(256), 0, st, o, (float*)y, rows, k, N); break;
-    case QBNN_BF16: hipLaunchKernelGGL((combine_kernel<QBNN_BF16>), grid, dim3(256), 0, st, o, (uint16_t*)y, rows, k, N); break;
-    default: hipLaunchKernelGGL((combine_kernel<QBNN_F16>), grid, dim3(256), 0, st, o, (_Float16*)y, rows, k, N); break;
-  }
+int launch_combine(const void* o, const uint8_t* oe, int rows, int k, int N, void* y, int y_type, hipStream_t st) {
+  const dim3 grid((unsigned)((N + 256 * COMBINE_COLUMNS - 1) / (256 * COMBINE_COLUMNS)), (unsigned)(rows < 32768 ? rows : 32768), (unsigned)((rows + 32767) / 32768));
+  const uint8_t* in = (const uint8_t*)o;
+  if (oe) hipLaunchKernelGGL((combine_kernel<QBNN_BF16, true>), grid, dim3(256), 0, st, in, oe, (uint16_t*)y, rows, k, N);
+  else if (y_type == QBNN_F32) hipLaunchKernelGGL((combine_kernel<QBNN_F32, false>), grid, dim3(256), 0, st, in, oe, (float*)y, rows, k, N);
+  else if (y_type == QBNN_BF16) hipLaunchKernelGGL((combine_kernel<QBNN_BF16, false>), grid, dim3(256), 0, st, in, oe, (uint16_t*)y, rows, k, N);
+  else hipLaunchKernelGGL((combine_kernel<QBNN_F16, false>), grid, dim3(256), 0, st, in, oe, (_Float16*)y, rows, k, N);
   return qbnn_check_launch_msg("qbnn_experts_f8 (sum)");
 }
 
@@ -1020,7 +1055,7 @@ QBNN_EXPORT int qbnn_experts_f8(const qbnn_f8_experts* d, void* stream) {
       (d->x_rows != d->T && d->x_rows != d->S * d->T))
     return f8_fail("qbnn_experts_f8: bad argument");
   if (!aligned(d->x, 0, 16) || !aligned(d->w_up, d->up_ss, 16) || !aligned(d->w_down, d->down_ss, 16) || !aligned(d->h, 0, 16) || !aligned(d->x_exp, 0, 4) ||
-      !aligned(d->up_exp, d->up_exp_ss, 4) || !aligned(d->down_exp, d->down_exp_ss, 4) || !aligned(d->h_exp, 0, 4))
+      !aligned(d->up_exp, d->up_exp_ss, 4) || !aligned(d->down_exp, d->down_exp_ss, 4) || !aligned(d->h_exp, 0, 4) || !aligned(d->o, 0, 16))
     return f8_fail("qbnn_experts_f8: e4m3 operands start at multiples of 16 bytes, exponents of 4");
   hipStream_t st = (hipStream_t)stream;
   if (d->x_float)
@@ -1038,7 +1073,14 @@ QBNN_EXPORT int qbnn_experts_f8(const qbnn_f8_experts* d, void* stream) {
   a.w = d->w_down; a.we = d->down_exp; a.w_ss = d->down_ss; a.we_ss = d->down_exp_ss; a.w_groups = d->down_sets;
   a.bias = d->b_down; a.bias_ss = d->b_down_ss; a.relu = 0;
   a.y_rows = d->rows; a.scale = d->weights;
+  // halves where the result is bf16, behind tiles; they take R Nb 257 bytes of the R N 4
+  const bool half = d->y_type == QBNN_BF16 && !(d->exact & 2) && d->N >= 128 && f8_tiled<true>(a, rows);
   set_result(a, d->o, nullptr, rows, d->N, QBNN_F32);
-  if (int rc = launch_linear_any<true>(a, rows, 1, QBNN_F32, d->exact >> 1 & 1, st)) return rc;
-  return launch_combine(d->o, d->S * d->T, d->top_k, d->N, d->y, d->y_type, st);
+  if (half) {
+    const int Nb = (d->N + 127) / 128;
+    a.y_rs = Nb * 128; a.ye_rs = Nb;
+    a.ye = (uint8_t*)d->o + (int64_t)rows * a.y_rs * 2;
+  }
+  if (int rc = launch_linear_any<true>(a, rows, 1, half ? F8_HALF : QBNN_F32, d->exact >> 1 & 1, st)) return rc;
+  return launch_combine(d->o, half ? a.ye : nullptr, d->S * d->T, d->top_k, d->N, d->y, d->y_type, st);
 }

@@ -120,4 +120,8 @@ def experts(x, weights, chosen, up, down, b_up, b_down, dtype):
             size[s, t] += np.abs(o * w)
             part = np.abs(w) * (product_bound(hq, d, bd, exact=dtype == "float32") + swing @ np.abs(d).T)
             bound[s, t] += part + 3 * FP32 * np.abs(o * w)          # the weight's own error and its product
+            if dtype == "bfloat16":
+                # may be held as halves of v 2^-e, |v 2^-e| <= 448 and 2^e <= the block's largest / 224: half a step of v 2^-e, or of the subnormals (2^-25) below 2^-14
+                blocks = np.pad(np.abs(np.nan_to_num(o * w, posinf=0, neginf=0)), ((0, 0), (0, -N % 128))).reshape(len(w), -1, 128).max(2)
+                bound[s, t] += HALF_STEP["float16"] * np.abs(o * w) + np.repeat(blocks, 128, 1)[:, :N] * 2.0 ** -25 / 224
     return y, bound * (1 + HALF_STEP[dtype]) + k * 2 * FP32 * size + rounding(y, dtype)

@@ -312,6 +312,29 @@ def test_experts_masked_choice_adds_nothing():
     assert torch.equal(y, z) and torch.isfinite(y).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [20, 200])
+def test_experts_large_and_infinite_results(T, dtype):
+    """Results far outside of 16-bit floats' range, tiny ones in the same row, and one infinite column: it stays the only one."""
+    E, D, H, N, k = 3, 128, 256, 400, 2
+    x, l = rnd(40, T, D), rnd(41, T, E)
+    up, down = rnd(42, E, H, D, by=D ** -0.5), rnd(43, E, N, H, by=2.0 ** 30)
+    down[:, 128:256] *= 2.0 ** -60
+    bd = torch.zeros(E, N)
+    bd[:, 300] = float("inf")
+    up, down = (q.quantize_fp8(w.to(DEV), 128) for w in (up, down))
+    r = q.route_experts(l.to(DEV), k)
+    y = q.experts_fp8(x.to(DEV).to(dtype), r, up, down, None, bd.to(DEV))
+    uv, dv = held(up), held(down)
+    xv = orc.quantised(f64(x.to(dtype)), 1)[None]
+    finite = bd.clone()
+    finite[:, 300] = 0
+    want, bound = orc.experts(xv, f64(r.weights)[None], r.experts.cpu().numpy()[None], lambda s, e: uv[e], lambda s, e: dv[e], None, lambda s, e: f64(finite)[e], NAME[dtype])
+    keep = torch.arange(N) != 300
+    assert torch.isinf(y[:, 300]).all() and float(y[:, keep].abs().max()) > 1e8 and float(y[:, 128:256].abs().max()) < 1e-6
+    check(y[:, keep.to(DEV)], want[0][:, keep], bound[0][:, keep])
+
+
 def test_experts_empty():
     r = q.route_experts(torch.zeros(2, 0, 4, device=DEV), 2)
     w = q.quantize_fp8(torch.randn(4, 64, 64, device=DEV), 128)
