@@ -56,10 +56,16 @@ template <int T> __device__ __forceinline__ void f8_load8(const f8_type<T>* row,
     for (int i = 0; i < 8; ++i) v[i] = col + i < K ? f8_load<T>(row[col + i]) : 0.f;
   }
 }
-__device__ __forceinline__ uint32_t f8_max8(const float (&v)[8]) {
-  uint32_t m = 0;
+__device__ __forceinline__ uint32_t f8_max8(const float (&v)[8]) {      // of what is finite; a maximum passes NaN over, only infinities need a second look
+  float f = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, f8_magnitude(v[i]));
+  for (int i = 0; i < 8; ++i) f = fmaxf(f, fabsf(v[i]));
+  uint32_t m = __float_as_uint(f);
+  if (m == 0x7f800000u) {
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, f8_magnitude(v[i]));
+  }
   return m;
 }
 template <int CTRL> __device__ __forceinline__ uint32_t f8_max_dpp(uint32_t m) { return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, CTRL, 0xf, 0xf, true)); }
@@ -438,9 +444,23 @@ template <int TM, int TN, bool GROUPED> __device__ __forceinline__ bool f8_locat
 // by anyone; put(i, st) writes rows 32 i .. + 31 there, F8_PITCH floats each): 16 lanes then write 128 neighbouring columns of a row.  Stored from the
 // accumulators' layout they were 32 bytes of each of 32 rows per instruction, and with the bounds unrolled 30 KiB of code: 27,000 cycles a tile, as much as 11 steps.
 constexpr int F8_PITCH = 132, F8_STAGE = 32 * F8_PITCH * 4 + 128 * 8;
-__device__ __forceinline__ float f8_relu(float u) { return u < 0.f ? 0.f : u; }      // (a NaN stays one)
+__device__ __forceinline__ float f8_relu(float u) { return __builtin_elementwise_maximum(u, 0.f); }      // (a NaN stays one)
+// Where a wave's 32 G rows go and their weights (G = 4: two rows a lane).  Two dependent loads: in front of the products where registers are left, so that they are not waited for behind them.
+template <int G> struct F8Moves {
+  int to[(G + 1) / 2];
+  float weight[(G + 1) / 2];
+  __device__ __forceinline__ void rows(const F8Args& a, const F8Tile& t, int m) {
+#pragma unroll
+    for (int i = 0; i < (G + 1) / 2; ++i) to[i] = a.y_rows[min(m + i * 64 + (int)(threadIdx.x & 63), t.m1 - 1)];
+  }
+  __device__ __forceinline__ void weights(const F8Args& a) {
+#pragma unroll
+    for (int i = 0; i < (G + 1) / 2; ++i) weight[i] = a.scale[to[i]];
+  }
+};
+template <int OUT, bool GROUPED> constexpr bool f8_moves() { return GROUPED && OUT != QBNN_F8; }
 template <int G, int OUT, bool GROUPED, bool WHOLE, class Put>
-__device__ __forceinline__ void f8_finish_as(const F8Args& a, const F8Tile& t, int m, int nw, uint8_t* stage, Put put) {
+__device__ __forceinline__ void f8_finish_as(const F8Args& a, const F8Tile& t, int m, int nw, uint8_t* stage, const F8Moves<G>& moves, Put put) {
   const int lane = threadIdx.x & 63, n = (lane & 15) * 8;
   const int in = WHOLE ? 8 : a.N - nw - n;                      // columns of this lane that exist
   float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -452,86 +472,141 @@ __device__ __forceinline__ void f8_finish_as(const F8Args& a, const F8Tile& t, i
       for (int c = 0; c < 8; ++c) b[c] = c < in ? bias[c] : 0.f;
   }
   float* st = (float*)stage;
-  // where the wave's rows go and their weights: fetched once, side by side (row by row in the loop below, two dependent loads were 1,500 cycles each time)
   int* const to_row = (int*)(stage + 32 * F8_PITCH * 4);
   float* const to_weight = (float*)(to_row + 32 * G);
-  const bool moved = GROUPED && OUT != QBNN_F8 && a.y_rows;
-  if (moved)
-    for (int r = lane; r < 32 * G; r += 64) {
-      const int to = a.y_rows[min(m + r, t.m1 - 1)];
-      to_row[r] = to;
-      to_weight[r] = a.scale[to];
-    }
+  constexpr bool moved = f8_moves<OUT, GROUPED>();
+  const bool relu = GROUPED ? OUT == QBNN_F8 : a.relu != 0;     // (experts: behind the first product)
+  if constexpr (moved) {
+#pragma unroll
+    for (int i = 0; i < (G + 1) / 2; ++i)
+      if (i * 64 + lane < 32 * G) { to_row[i * 64 + lane] = moves.to[i]; to_weight[i * 64 + lane] = moves.weight[i]; }
+  }
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     put(i, st);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // (the wave's own LDS: no barrier)
     constexpr int AT_ONCE = WHOLE ? 4 : 2;
 #pragma unroll 1
-    for (int p0 = 0; p0 < 8; p0 += AT_ONCE)
+    for (int p0 = 0; p0 < 8; p0 += AT_ONCE) {
+      const int r0 = p0 * 4 + (lane >> 4);
+      float v[AT_ONCE][8], s[AT_ONCE];
+      int64_t to[AT_ONCE];
 #pragma unroll
-      for (int p1 = 0; p1 < AT_ONCE; ++p1) {
-        const int r = (p0 + p1) * 4 + (lane >> 4), row = m + i * 32 + r;
+      for (int p = 0; p < AT_ONCE; ++p) {
+        const int r = r0 + p * 4;
         const f8_v4f lo = *(const f8_v4f*)(st + r * F8_PITCH + n), hi = *(const f8_v4f*)(st + r * F8_PITCH + n + 4);
-        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] += b[c];
-        if (a.relu) {
+        for (int c = 0; c < 4; ++c) { v[p][c] = lo[c]; v[p][4 + c] = hi[c]; }
+        to[p] = m + i * 32 + r;
+        s[p] = 1.f;
+        if constexpr (moved) { to[p] = to_row[i * 32 + r]; s[p] = to_weight[i * 32 + r]; }
+      }
 #pragma unroll
-          for (int c = 0; c < 8; ++c) v[c] = f8_relu(v[c]);
+      for (int p = 0; p < AT_ONCE; ++p)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[p][c] += b[c];
+      if (relu) {
+#pragma unroll
+        for (int p = 0; p < AT_ONCE; ++p)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[p][c] = f8_relu(v[p][c]);
+      }
+      if constexpr (moved) {
+        bool none = false;
+#pragma unroll
+        for (int p = 0; p < AT_ONCE; ++p) none |= s[p] == 0.f;
+        if (__any(none)) {                                      // (an expert of weight 0 adds nothing, whatever it computed)
+#pragma unroll
+          for (int p = 0; p < AT_ONCE; ++p)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[p][c] = s[p] == 0.f ? 0.f : v[p][c];
         }
-        if constexpr (OUT == QBNN_F8) {
+        if constexpr (OUT != F8_HALF) {                         // (there it is one factor with the block's)
 #pragma unroll
-          for (int c = 0; c < 8; ++c) if (!WHOLE && c >= in) v[c] = 0.f;
-          const int e = f8_exponent(f8_max16(f8_max8(v)));
-          if (row < t.m1) {
-            *(f8_v2i*)(a.y + (int64_t)t.sample * a.y_ss + (int64_t)row * a.y_rs + nw + n) = f8_scale8(v, f8_pow2(-e));
-            if (n == 0) f8_put_exponent(a.ye + ((int64_t)t.sample * a.M + row) * a.ye_rs, nw >> 7, (a.N + 127) >> 7, a.ye_rs, e);
+          for (int p = 0; p < AT_ONCE; ++p)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[p][c] *= s[p];
+        }
+      }
+      if constexpr (OUT == QBNN_F8 || OUT == F8_HALF) {
+        uint32_t top[AT_ONCE];
+        bool inf = false;
+#pragma unroll
+        for (int p = 0; p < AT_ONCE; ++p) {
+          float f = 0.f;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            if (!WHOLE && c >= in) v[p][c] = 0.f;
+            f = fmaxf(f, fabsf(v[p][c]));
           }
-        } else if (row < t.m1) {
-          int64_t to = row;
-          if (moved) {
-            to = to_row[i * 32 + r];
-            const float s = to_weight[i * 32 + r];
+          top[p] = __float_as_uint(f);
+          inf |= top[p] == 0x7f800000u;
+        }
+        if (__any(inf)) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) v[c] = s == 0.f ? 0.f : v[c] * s;
+          for (int p = 0; p < AT_ONCE; ++p) top[p] = f8_max8(v[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < AT_ONCE; ++p) {
+          top[p] = f8_max16(top[p]);
+          if constexpr (OUT == F8_HALF) top[p] = f8_magnitude(__uint_as_float(top[p]) * s[p]);      // (a weight that is not finite: no scale, the values say so)
+        }
+        int e[AT_ONCE];
+        f8_v4i o[AT_ONCE];
+#pragma unroll
+        for (int p = 0; p < AT_ONCE; ++p) {
+          e[p] = f8_exponent(top[p]);
+          const float down = OUT == F8_HALF ? s[p] * f8_pow2(-e[p]) : f8_pow2(-e[p]);
+          if constexpr (OUT == QBNN_F8) {
+            const f8_v2i q = f8_scale8(v[p], down);
+            o[p][0] = q[0];
+            o[p][1] = q[1];
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[p][c] = f8_store2<QBNN_F16>(v[p][2 * c] * down, v[p][2 * c + 1] * down);
           }
-          if constexpr (OUT == F8_HALF) {
+        }
 #pragma unroll
-            for (int c = 0; c < 8; ++c) if (!WHOLE && c >= in) v[c] = 0.f;
-            const int e = f8_exponent(f8_max16(f8_max8(v)));
-            const float down = f8_pow2(-e);
-            f8_v4i o;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[c] = f8_store2<QBNN_F16>(v[2 * c] * down, v[2 * c + 1] * down);
-            *(f8_v4i*)(a.y + (to * a.y_rs + nw + n) * 2) = o;
-            if (n == 0) a.ye[to * a.ye_rs + (nw >> 7)] = (uint8_t)(e + 127);
-            continue;
+        for (int p = 0; p < AT_ONCE; ++p) {
+          if (m + i * 32 + r0 + p * 4 >= t.m1) continue;
+          if constexpr (OUT == QBNN_F8) {
+            *(f8_v2i*)(a.y + (int64_t)t.sample * a.y_ss + to[p] * a.y_rs + nw + n) = (f8_v2i){o[p][0], o[p][1]};
+            if (n == 0) f8_put_exponent(a.ye + ((int64_t)t.sample * a.M + to[p]) * a.ye_rs, nw >> 7, (a.N + 127) >> 7, a.ye_rs, e[p]);
+          } else {
+            *(f8_v4i*)(a.y + (to[p] * a.y_rs + nw + n) * 2) = o[p];
+            if (n == 0) a.ye[to[p] * a.ye_rs + (nw >> 7)] = (uint8_t)(e[p] + 127);
           }
-          typedef f8_type<OUT == F8_HALF ? QBNN_F16 : OUT> Out;
-          Out* y = (Out*)a.y + (int64_t)t.sample * a.y_ss + to * a.y_rs + nw + n;
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < AT_ONCE; ++p) {
+          const int r = r0 + p * 4;
+          if (m + i * 32 + r >= t.m1) continue;
+          f8_type<OUT>* y = (f8_type<OUT>*)a.y + (int64_t)t.sample * a.y_ss + to[p] * a.y_rs + nw + n;
           if (!WHOLE && in < 8) {                               // the lane at the end: its values by way of the stage, one by one
-            *(f8_v4f*)(st + r * F8_PITCH + n) = (f8_v4f){v[0], v[1], v[2], v[3]};
-            *(f8_v4f*)(st + r * F8_PITCH + n + 4) = (f8_v4f){v[4], v[5], v[6], v[7]};
+            *(f8_v4f*)(st + r * F8_PITCH + n) = (f8_v4f){v[p][0], v[p][1], v[p][2], v[p][3]};
+            *(f8_v4f*)(st + r * F8_PITCH + n + 4) = (f8_v4f){v[p][4], v[p][5], v[p][6], v[p][7]};
 #pragma unroll 1
-            for (int c = 0; c < in; ++c) y[c] = f8_store<OUT == F8_HALF ? QBNN_F16 : OUT>(st[r * F8_PITCH + n + c]);
+            for (int c = 0; c < in; ++c) y[c] = f8_store<OUT>(st[r * F8_PITCH + n + c]);
           } else if constexpr (OUT == QBNN_F32) {
-            __builtin_memcpy(y, v, sizeof(v));
+            __builtin_memcpy(y, v[p], sizeof(v[p]));
           } else {
             f8_v4i o;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) o[c] = f8_store2<OUT == F8_HALF ? QBNN_F16 : OUT>(v[2 * c], v[2 * c + 1]);
+            for (int c = 0; c < 4; ++c) o[c] = f8_store2<OUT>(v[p][2 * c], v[p][2 * c + 1]);
             __builtin_memcpy(y, &o, sizeof(o));
           }
         }
       }
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
-template <int G, int OUT, bool GROUPED, class Put> __device__ __forceinline__ void f8_finish(const F8Args& a, const F8Tile& t, int m, int nw, uint8_t* stage, Put put) {
+template <int G, int OUT, bool GROUPED, class Put>
+__device__ __forceinline__ void f8_finish(const F8Args& a, const F8Tile& t, int m, int nw, uint8_t* stage, const F8Moves<G>& moves, Put put) {
   if (nw >= a.N || m >= t.m1) return;
-  if (nw + 128 <= a.N) f8_finish_as<G, OUT, GROUPED, true>(a, t, m, nw, stage, put);
-  else f8_finish_as<G, OUT, GROUPED, false>(a, t, m, nw, stage, put);
+  if (nw + 128 <= a.N) f8_finish_as<G, OUT, GROUPED, true>(a, t, m, nw, stage, moves, put);
+  else f8_finish_as<G, OUT, GROUPED, false>(a, t, m, nw, stage, moves, put);
 }
 
 // The exponents of 16 steps of a row: four dwords, used from the bottom and moved down two bytes every two steps.  A load's result may only be waited for
@@ -726,7 +801,9 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
 
   lds_barrier();            // ... and no wave reads another's operands any more
   // lane: activation row r32 of fragment i, weight rows 8 q + 4 h .. + 3 of fragment j in registers 4 q .. + 3
-  f8_finish<MI, OUT, GROUPED>(a, t, t.m0 + wm * MI * 32, n0 + wn * 128, lds + wave * F8_STAGE, [&](int i, float* st) {
+  F8Moves<MI> moves;
+  if constexpr (f8_moves<OUT, GROUPED>()) { moves.rows(a, t, t.m0 + wm * MI * 32); moves.weights(a); }
+  f8_finish<MI, OUT, GROUPED>(a, t, t.m0 + wm * MI * 32, n0 + wn * 128, lds + wave * F8_STAGE, moves, [&](int i, float* st) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -823,11 +900,14 @@ __global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, i
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[i][j] = (f8_v4f){0.f, 0.f, 0.f, 0.f};
 
+  F8Moves<4> moves;
+  if constexpr (f8_moves<OUT, GROUPED>()) moves.rows(a, t, t.m0 + wm * 128);
   request_exponents(0, 0);
 #pragma unroll
   for (int p = 0; p < 16; ++p) request(0, 0, p);
 #pragma unroll
   for (int p = 0; p < 16; ++p) request(1, 1, p);
+  if constexpr (f8_moves<OUT, GROUPED>()) moves.weights(a);
   wait_vmcnt<16>();
   lds_barrier();
 #pragma unroll
@@ -878,7 +958,7 @@ __global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, i
   asm volatile("s_nop 15\n\ts_nop 15");      // the last products are in their registers
   __builtin_amdgcn_sched_barrier(0);
   // lane: activation row r16 of fragment i, weight rows 4 h .. + 3 of fragment j
-  f8_finish<4, OUT, GROUPED>(a, t, t.m0 + wm * 128, n0 + wn * 128, lds + wave * F8_STAGE, [&](int g, float* st) {
+  f8_finish<4, OUT, GROUPED>(a, t, t.m0 + wm * 128, n0 + wn * 128, lds + wave * F8_STAGE, moves, [&](int g, float* st) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
