@@ -148,6 +148,34 @@ def test_linear_result_in_blocks(size):
         assert not t.exponent.cpu()[..., -(-N // 128):].any()
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("out", [None, torch.float32, torch.float8_e4m3fn])
+@pytest.mark.parametrize("S,B,N,K", [(1, 1, 1, 1), (1, 3, 130, 127), (1, 16, 256, 1000), (3, 2, 40, 129), (1, 5, 8192, 2048), (1, 17, 100, 300)])
+def test_linear_quantises_as_the_quantiser_does(S, B, N, K, out, dtype):
+    """A float x and the quantised one: equal bits."""
+    x = rnd(60, S, B, 2 * K, dtype=dtype)[..., ::2] * torch.exp2(torch.arange(K) % 9 - 4.0).to(dtype)
+    x[0, 0, 0] = float("inf")
+    w = q.quantize_fp8(rnd(61, N, K).to(DEV), 128)
+    x = x.to(DEV)
+    a, b = q.linear_fp8(x, w, out_dtype=out), q.linear_fp8(q.quantize_fp8(x), w, out_dtype=out or dtype)
+    if out == torch.float8_e4m3fn:
+        assert torch.equal(a.data.view(torch.uint8), b.data.view(torch.uint8)) and torch.equal(a.exponent, b.exponent)
+    else:
+        assert torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) and torch.equal(a.isnan(), b.isnan()) and a[..., 1:, :].isfinite().all()
+
+
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_experts_quantise_as_the_quantiser_does(dtype, shared):
+    S, T, E, D, H, N, k = 3, 5, 7, 300, 200, 90, 2
+    wide = rnd(62, S, T + 2, D + 5, dtype=dtype).to(DEV)
+    x = wide[:1, 1:T + 1, 3:D + 3] if shared else wide[:, 1:T + 1, 3:D + 3]
+    up, down = (q.quantize_fp8(rnd(i, E, r, c).to(DEV), 128) for i, r, c in ((63, H, D), (64, N, H)))
+    r = q.route_experts(rnd(65, S, T, E).to(DEV), k)
+    a, b = q.experts_fp8(x, r, up, down, out_dtype=dtype), q.experts_fp8(q.quantize_fp8(x), r, up, down, out_dtype=dtype)
+    assert a.isfinite().all() and torch.equal(a, b)
+
+
 def test_linear_rows_stand_alone():
     """A row does not depend on its neighbours: one with NaN and infinities leaves the others their bits, at every row count's kernel."""
     w = q.quantize_fp8(rnd(2, 200, 300).to(DEV), 128)
