@@ -986,11 +986,14 @@ template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, 
   const int spare = GROUPED ? a.groups : 0;        // each group may end inside a tile
   const int per = f8_rows_each<GROUPED>(a, rows);
   const auto tiles = [&](int tm, int tn) { return (int64_t)z * ((rows + tm - 1) / tm + spare / 2) * ((a.N + tn - 1) / tn); };
+  // The largest tile that still gives the 256 CUs work: fewer bytes through LDS per product, but 256 x 256 holds a CU for itself.  Measured the other way round (us):
+  // 128 x 128 for 64 x 128 with 330 - 600 tiles 69 -> 58 (5 x 12 groups of 75, fp16) and 28.6 -> 23.8 (100 x 128 x 500 x 800, fp32), with 32 - 64 tiles 22.6 -> 25.7.
   if (f8_tiled<GROUPED>(a, rows)) {
     if constexpr (!EXACT) {
       if (per > 128 && tiles(256, 256) >= 192) return launch_big<OUT, GROUPED>(a, rows, z, st);
     }
     if (per > 64 && tiles(128, 256) >= 384) return launch_tiled<2, 2, 2, OUT, EXACT, GROUPED>(a, rows, z, st);
+    if (tiles(128, 128) >= 256) return launch_tiled<1, 4, 1, OUT, EXACT, GROUPED>(a, rows, z, st);
     return launch_tiled<1, 2, 1, OUT, EXACT, GROUPED>(a, rows, z, st);
   }
   if constexpr (OUT == F8_HALF) return f8_fail("qbnn_experts_f8: no direct form of this result");
