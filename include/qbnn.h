@@ -689,8 +689,9 @@ int qbnn_route_experts(const qbnn_route* host_desc, void* stream);
  * offsets / rows / weights: of qbnn_route_experts with the same S, T, E, top_k.  x [S or 1][T][D] (x_rows = S T or T; float: quantised into x / x_exp
  * first), w_up [S or 1][E][H][D], w_down [S or 1][E][N][H] (block_rows 128; strides per expert in bytes, up_sets / down_sets = E or S E), biases fp32 (strides per
  * expert in elements).  Hidden rows are quantised in blocks of 128; exact: bit 0 the first product, bit 1 the second (see qbnn_f8_linear); a result whose weight
- * is 0 is left out, whatever it is.  The weighted results are fp32 and summed in the order of j, rounded once to y_type (QBNN_F32 .. QBNN_F16).
- * Workspaces: h [S T top_k][Hp], h_exp [S T top_k][Hs] (Hp, Hs of H columns), o fp32 [S T top_k][N]. */
+ * is 0 is left out, whatever it is.  The weighted results are fp32 and summed in the order of j, rounded once to y_type (QBNN_F32 .. QBNN_F16); where y is bf16
+ * and more than 32 rows go to an expert on average they may wait for the sum as fp16 with one power of two per 128 columns (2^-11 of each, beside the sum's own 2^-8).
+ * Workspaces: h [S T top_k][Hp], h_exp [S T top_k][Hs] (Hp, Hs of H columns), o of S T top_k N 4 bytes, at a multiple of 16. */
 typedef struct qbnn_f8_experts {
   const void* x_float; int64_t x_float_ss, x_float_rs;
   uint8_t* x; uint8_t* x_exp;

@@ -417,8 +417,10 @@ template <int MT, int NT, int NW, int D, int OUT, bool EXACT, bool GROUPED> int 
 // its accumulators are tied in place (the 16 x 16 form's are renamed, which cost 3 register moves per instruction here) and it reads half the operand registers.
 // One barrier per step, in front of the last activation fragment's products: before it the wave waits for its share of the next step's bytes; behind it
 // the buffer just read is requested again and the next step's first fragments are read, each weight fragment's registers as soon as their products are issued.
+constexpr int F8_PITCH = 132, F8_STAGE = 32 * F8_PITCH * 4 + 128 * 8;      // a wave's stage behind the products, see f8_finish
 template <int MI, int WM, int WN> struct F8Tiled {
-  static constexpr int TM = 32 * MI * WM, TN = 128 * WN, WAVES = WM * WN, XB = TM * 128, WB = TN * 128, LDS = 2 * (XB + WB);
+  static constexpr int TM = 32 * MI * WM, TN = 128 * WN, WAVES = WM * WN, XB = TM * 128, WB = TN * 128;
+  static constexpr int LDS = 2 * (XB + WB) > WAVES * F8_STAGE ? 2 * (XB + WB) : WAVES * F8_STAGE;      // the operands, and then the stages
   static constexpr int PX = TM / 8 / WAVES, PW = TN / 8 / WAVES;      // DMA requests (8 rows each) per wave and step
   static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && LDS <= 160 * 1024 && 2 * XB <= 65536 && 2 * WB <= 65536, "immediate offsets of the reads");
 };
@@ -443,7 +445,6 @@ template <int TM, int TN, bool GROUPED> __device__ __forceinline__ bool f8_locat
 // Results of a wave's (32 G) x 128 tile from row m, weight row nw on, 32 rows at a time through `stage` (F8_STAGE bytes of LDS of this wave's own, no longer read
 // by anyone; put(i, st) writes rows 32 i .. + 31 there, F8_PITCH floats each): 16 lanes then write 128 neighbouring columns of a row.  Stored from the
 // accumulators' layout they were 32 bytes of each of 32 rows per instruction, and with the bounds unrolled 30 KiB of code: 27,000 cycles a tile, as much as 11 steps.
-constexpr int F8_PITCH = 132, F8_STAGE = 32 * F8_PITCH * 4 + 128 * 8;
 __device__ __forceinline__ float f8_relu(float u) { return __builtin_elementwise_maximum(u, 0.f); }      // (a NaN stays one)
 // Where a wave's 32 G rows go and their weights (G = 4: two rows a lane).  Two dependent loads: in front of the products where registers are left, so that they are not waited for behind them.
 template <int G> struct F8Moves {
@@ -838,6 +839,7 @@ template <int B> __device__ __forceinline__ void f8_mfma_in_place(f8_v4f& acc, c
   else asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs));
 }
 
+static_assert(4 * F8_STAGE <= 131072, "the stages lie where the operands were");
 constexpr int F8_BIG_LDS = 131072 + 2 * 2048;      // two steps of x and w, two sets of exponents (1 KiB of x, 256 bytes for each wave of w)
 
 template <int OUT, bool GROUPED>

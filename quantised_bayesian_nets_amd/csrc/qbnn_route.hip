@@ -265,7 +265,8 @@ template <int T, int NP> __device__ __forceinline__ void route_exact_row(const R
 // likewise the last group kept above the next), and one lane alone may hold it.  Rows without that proof (1 in 1000 of 256 random fp32 logits, and rows with ties)
 // are listed and done again, a whole wave each, with 64-bit keys.  Masked experts are the integers below all keys, lowest index first.
 // A key that was chosen is not taken out: the next round looks for the largest below it, as the smallest unsigned m - 1 - w (what lies above wraps).
-// Bound: a round is 24 + 12 instructions for 64 / L rows; 32768 x 256 logits are 5 us of reading.
+// Bound: vector issue.  A round is 50 instructions for 64 / L rows, all of a row of 256 with groups and 8 choices 1,000 for 4 rows: 32768 x 256 take 38 us at 2 GHz, where
+// reading them takes 7; 22 - 28 of it are these rounds, the rest waits for the waves that do a row again (10 us each).  Registers held to 128, for 4 waves per SIMD.
 constexpr uint32_t ROUTE_MASKED = 0x00800000u;                  // the order of the lowest finite float: masked experts lie below
 
 // Waves of a workgroup: 64 rows are 64 L / 64 of them, done in turn by 4 where that is all and by 8 where there are more

@@ -118,6 +118,14 @@ def test_linear(size, dtype, out):
     check(y, want, bound + orc.rounding(want, NAME[out]) + bound * orc.HALF_STEP[NAME[out]])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("S,B,N,K", [(70, 128, 500, 130), (66, 100, 512, 256), (9, 200, 1000, 300), (260, 33, 128, 128)])
+def test_linear_many_samples(S, B, N, K, dtype):
+    """Enough tiles to fill the card, full and ragged: every tile shape between the direct form and the largest."""
+    y, want, bound, out = linear_case(70, S, S, S, B, N, K, dtype, 2, True)
+    check(y, want, bound + orc.rounding(want, NAME[out]) + bound * orc.HALF_STEP[NAME[out]])
+
+
 @pytest.mark.parametrize("sx,sw,bias", [(3, 3, 2), (1, 3, 1), (3, 1, 2), (3, 3, 0), (1, 1, 0)])
 @pytest.mark.parametrize("size", [(1, 40, 200), (20, 150, 300), (200, 260, 384)], ids=str)
 def test_linear_samples(size, sx, sw, bias):
@@ -311,7 +319,7 @@ def experts_case(seed, S, T, E, k, D, H, N, dtype, bias, own=True, shared_x=Fals
 
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("case", [(1, 1, 1, 1, 1, 1, 1), (1, 1, 8, 2, 128, 256, 128), (1, 7, 4, 4, 100, 70, 130), (2, 40, 6, 3, 129, 200, 90), (1, 300, 5, 2, 256, 384, 256), (3, 100, 12, 1, 77, 300, 77),
-                                  (1, 700, 3, 2, 200, 260, 300), (1, 20, 100, 6, 64, 64, 64)], ids=str)
+                                  (1, 700, 3, 2, 200, 260, 300), (1, 20, 100, 6, 64, 64, 64), (5, 300, 12, 3, 200, 400, 300), (9, 260, 8, 2, 130, 512, 512)], ids=str)
 def test_experts(case, dtype):
     experts_case(20, *case, dtype, True)
     experts_case(21, *case, dtype, False, own=False, shared_x=True)
