@@ -550,14 +550,29 @@ __device__ __forceinline__ void f8_finish_as(const F8Args& a, const F8Tile& t, i
 #pragma unroll
         for (int p = 0; p < AT_ONCE; ++p) {
           top[p] = f8_max16(top[p]);
-          if constexpr (OUT == F8_HALF) top[p] = f8_magnitude(__uint_as_float(top[p]) * s[p]);      // (a weight that is not finite: no scale, the values say so)
+          if constexpr (OUT == F8_HALF) top[p] = min(__float_as_uint(__uint_as_float(top[p]) * s[p]) & 0x7fffffffu, 0x7f7fffffu);      // (an overflow: the largest scale, the others stay finite)
         }
         int e[AT_ONCE];
+        float by[AT_ONCE];
         f8_v4i o[AT_ONCE];
+        bool far = false;
 #pragma unroll
         for (int p = 0; p < AT_ONCE; ++p) {
           e[p] = f8_exponent(top[p]);
-          const float down = OUT == F8_HALF ? s[p] * f8_pow2(-e[p]) : f8_pow2(-e[p]);
+          by[p] = OUT == F8_HALF ? s[p] * f8_pow2(-e[p]) : f8_pow2(-e[p]);
+          far |= OUT == F8_HALF && !(fabsf(by[p]) < INFINITY);
+        }
+        if (OUT == F8_HALF && __any(far)) {                     // tiny results under a large weight: one after the other
+#pragma unroll
+          for (int p = 0; p < AT_ONCE; ++p) {
+            by[p] = f8_pow2(-e[p]);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[p][c] *= s[p];
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < AT_ONCE; ++p) {
+          const float down = by[p];
           if constexpr (OUT == QBNN_F8) {
             const f8_v2i q = f8_scale8(v[p], down);
             o[p][0] = q[0];

@@ -12,11 +12,18 @@ MAX_EXPERTS, MAX_CHOICES = 1024, 32      # include/qbnn.h: QBNN_ROUTE_MAX_EXPERT
 
 class Routing:
     """What the router decided for [S, T] rows: `weights` float32 and `experts` int32 [S, T, top_k] (best first), and the order in which the experts'
-    products walk the choices: those of (sample s, expert e) are rows[offsets[s E + e] : offsets[s E + e + 1]], flat indices into [S, T, top_k]."""
+    products walk the choices: those of (sample s, expert e) are rows[offsets[s E + e] : offsets[s E + e + 1]], flat indices into [S, T, top_k].  Types and
+    shapes are checked; that offsets and rows are such an order is not."""
 
     __slots__ = ("weights", "experts", "offsets", "rows", "n_experts")
 
     def __init__(self, weights, experts, offsets, rows, n_experts):
+        shape, n = weights.shape, weights.numel()
+        if weights.dtype != torch.float32 or experts.dtype != torch.int32 or offsets.dtype != torch.int32 or rows.dtype != torch.int32:
+            raise TypeError("a Routing holds float32 weights and int32 experts, offsets and rows")
+        if (len(shape) not in (2, 3) or experts.shape != shape or rows.shape != (n,) or offsets.shape != ((shape[0] if len(shape) == 3 else 1) * n_experts + 1,) or
+                not (weights.is_contiguous() and experts.is_contiguous() and offsets.is_contiguous() and rows.is_contiguous())):
+            raise ValueError("weights and experts are [T, top_k] or [S, T, top_k], offsets [S E + 1], rows [S T top_k], all contiguous")
         self.weights, self.experts, self.offsets, self.rows, self.n_experts = weights, experts, offsets, rows, n_experts
 
 
@@ -61,7 +68,9 @@ def route_experts(logits, top_k, score="softmax", bias=None, groups=1, top_group
         logits.data_ptr(), logits.stride(0) if len(lead) == 3 else 0, logits.stride(-2), 0 if bias is None else bias.data_ptr(),
         weights.data_ptr(), experts.data_ptr(), at, at + 4 * (S * E + 1), at + 4 * (S * E + 1 + n),
         S, T, E, top_k, groups, top_groups, score == "sigmoid", bool(renormalize), FLOAT_TYPES[logits.dtype], scale))
-    return Routing(weights, experts, offsets, rows, E)
+    r = Routing.__new__(Routing)                                  # (as its checks ask for)
+    r.weights, r.experts, r.offsets, r.rows, r.n_experts = weights, experts, offsets, rows, E
+    return r
 
 
 def experts_fp8(x, routing, w_up, w_down, b_up=None, b_down=None, out_dtype=None):
@@ -100,7 +109,7 @@ def experts_fp8(x, routing, w_up, w_down, b_up=None, b_down=None, out_dtype=None
     b_up = _bias(b_up, (w_up.shape[:-1],), "like w_up without its columns")
     b_down = _bias(b_down, (w_down.shape[:-1],), "like w_down without its columns")
     held = isinstance(x, F8Tensor)
-    dev = _device(x.data if held else x, routing.weights, w_up.data, w_down.data, b_up, b_down)
+    dev = _device(x.data if held else x, routing.weights, routing.offsets, routing.rows, w_up.data, w_down.data, b_up, b_down)
     y = torch.empty((*lead, N), dtype=out_dtype, device=dev)
     R = S * T * k
     if R == 0:

@@ -60,6 +60,11 @@ def test_router_refuses():
 def test_experts_refuse():
     S, T, E, k, D, H, N = 2, 5, 4, 2, 130, 140, 60
     z = torch.zeros(S, T, k)
+    good = (z, z.int(), torch.zeros(S * E + 1).int(), torch.zeros(S * T * k).int(), E)
+    for i, bad, error in ((0, z.double(), TypeError), (1, z.long(), TypeError), (2, good[2].long(), TypeError), (3, good[3].long(), TypeError), (1, z[:1].int(), ValueError), (2, good[2][1:], ValueError),
+                          (3, good[3][1:], ValueError), (4, 5, ValueError), (0, torch.zeros(T, S, k).transpose(0, 1), ValueError)):
+        with pytest.raises(error):
+            q.Routing(*good[:i], bad, *good[i + 1:])
     r = q.Routing(z, z.int(), torch.zeros(S * E + 1).int(), torch.zeros(S * T * k).int(), E)
     x, up, down = torch.zeros(S, T, D), held((E,), H, D), held((E,), N, H)
     for args, kw, error in (((x, None, up, down), {}, TypeError), ((x, r, x, down), {}, TypeError), ((x, r, held((E,), H, D, 1), down), {}, TypeError), ((x, r, held((), H, D), down), {}, TypeError),

@@ -371,6 +371,21 @@ def test_experts_large_and_infinite_results(T, dtype):
     check(y[:, keep.to(DEV)], want[0][:, keep], bound[0][:, keep])
 
 
+@pytest.mark.parametrize("T", [9, 64, 600])
+def test_experts_at_the_ends_of_the_range(T):
+    """Under a weight of 512: a result past fp32 is infinite and leaves its neighbours as they are, one far below 1 is not lost."""
+    up, bias = q.quantize_fp8(torch.zeros(1, 128, 128, device=DEV), 128), torch.ones(1, 128, device=DEV)      # every hidden value is 1
+    r = q.route_experts(torch.zeros(T, 1, device=DEV), 1, scale=512.0)
+    for high, low in ((120, 110), (-125, -127)):
+        down = torch.zeros(1, 300, 128)
+        down[:, :, 0] = 2.0 ** low
+        down[:, 5, 0] = 2.0 ** high
+        y = q.experts_fp8(torch.zeros(T, 128, device=DEV, dtype=torch.bfloat16), r, up, q.quantize_fp8(down.to(DEV), 128), bias).float()
+        want = torch.full((T, 300), 2.0 ** (low + 9))
+        want[:, 5] = 2.0 ** (high + 9) if high < 0 else float("inf")
+        assert torch.equal(y.cpu(), want)
+
+
 def test_experts_empty():
     r = q.route_experts(torch.zeros(2, 0, 4, device=DEV), 2)
     w = q.quantize_fp8(torch.randn(4, 64, 64, device=DEV), 128)
