@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -832,7 +833,7 @@ template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED> int launch_
   using C = F8Tiled<MI, WM, WN>;
   static std::atomic<uint64_t> attr{0};
   if (int rc = qbnn_ensure_dyn_lds((const void*)linear_f8_tiled_kernel<MI, WM, WN, OUT, EXACT, GROUPED>, &attr, C::LDS)) return rc;
-  const int64_t tm = (rows + C::TM - 1) / C::TM + (GROUPED ? a.groups : 0), tn = (a.N + C::TN - 1) / C::TN;
+  const int64_t tm = (rows + C::TM - 1) / C::TM + (GROUPED ? std::min(a.groups, rows) : 0), tn = (a.N + C::TN - 1) / C::TN;
   if (tm * tn * z > 0x7fffffff) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
   hipLaunchKernelGGL((linear_f8_tiled_kernel<MI, WM, WN, OUT, EXACT, GROUPED>), dim3((unsigned)(tm * tn * z)), dim3(C::WAVES * 64), C::LDS, st, a, (int)tm, (int)tn, z);
   return qbnn_check_launch_msg("qbnn_linear_f8");
@@ -986,7 +987,7 @@ __global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, i
 template <int OUT, bool GROUPED> int launch_big(const F8Args& a, int rows, int z, hipStream_t st) {
   static std::atomic<uint64_t> attr{0};
   if (int rc = qbnn_ensure_dyn_lds((const void*)linear_f8_big_kernel<OUT, GROUPED>, &attr, F8_BIG_LDS)) return rc;
-  const int64_t tm = (rows + 255) / 256 + (GROUPED ? a.groups : 0), tn = (a.N + 255) / 256;
+  const int64_t tm = (rows + 255) / 256 + (GROUPED ? std::min(a.groups, rows) : 0), tn = (a.N + 255) / 256;
   if (tm * tn * z > 0x7fffffff) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
   hipLaunchKernelGGL((linear_f8_big_kernel<OUT, GROUPED>), dim3((unsigned)(tm * tn * z)), dim3(256), F8_BIG_LDS, st, a, (int)tm, (int)tn, z);
   return qbnn_check_launch_msg("qbnn_linear_f8");
@@ -1000,7 +1001,7 @@ template <bool GROUPED> bool f8_tiled(const F8Args& a, int rows) {
   return f8_rows_each<GROUPED>(a, rows) > 32 && far < ((int64_t)1 << 32) && a.Kb < (1 << 16);
 }
 template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, int rows, int z, hipStream_t st) {
-  const int spare = GROUPED ? a.groups : 0;        // each group may end inside a tile
+  const int spare = GROUPED ? std::min(a.groups, rows) : 0;      // each group with rows may end inside a tile
   const int per = f8_rows_each<GROUPED>(a, rows);
   const auto tiles = [&](int tm, int tn) { return (int64_t)z * ((rows + tm - 1) / tm + spare / 2) * ((a.N + tn - 1) / tn); };
   // The largest tile that still gives the 256 CUs work: fewer bytes through LDS per product, but 256 x 256 holds a CU for itself.  Measured the other way round (us):
