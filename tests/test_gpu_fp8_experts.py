@@ -229,14 +229,15 @@ def route_check(logits, k, **kw):
     return r
 
 
-@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 8, 2), (5, 3, 3), (63, 60, 4), (64, 64, 6), (65, 65, 8), (300, 128, 1), (129, 130, 7), (1000, 256, 8), (77, 512, 16), (40, 1024, 32), (4097, 16, 2), (8300, 20, 3)])
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 8, 2), (5, 3, 3), (63, 60, 4), (64, 64, 6), (65, 65, 8), (300, 128, 1), (129, 130, 7), (1000, 256, 8), (77, 512, 16), (40, 1024, 32), (4097, 16, 2), (8300, 20, 3), (8257, 21, 2), (130, 1023, 3)])
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_router(T, E, k, dtype):
     for score, renorm in itertools.product(("softmax", "sigmoid"), (False, True)):
         route_check(rnd(5, T, E, by=2.0, dtype=dtype), k, score=score, renormalize=renorm)
 
 
-@pytest.mark.parametrize("T,E,k,groups,kept", [(70, 8, 2, 2, 1), (33, 60, 5, 4, 3), (100, 256, 8, 8, 4), (9, 12, 3, 12, 5), (50, 512, 6, 64, 2), (21, 64, 4, 1, 1), (64, 192, 32, 3, 1), (13, 1024, 8, 16, 4)])
+@pytest.mark.parametrize("T,E,k,groups,kept", [(70, 8, 2, 2, 1), (33, 60, 5, 4, 3), (100, 256, 8, 8, 4), (9, 12, 3, 12, 5), (50, 512, 6, 64, 2), (21, 64, 4, 1, 1), (64, 192, 32, 3, 1), (13, 1024, 8, 16, 4), (17, 960, 32, 5, 2), (100, 48, 4, 16, 5), (70, 40, 8, 20, 6),
+                                                 (30, 1000, 8, 8, 4), (129, 512, 5, 2, 1), (65, 32, 6, 2, 1)])
 def test_router_groups_and_bias(T, E, k, groups, kept):
     for dtype, score in itertools.product((torch.float32, torch.bfloat16), ("softmax", "sigmoid")):
         l = rnd(6, T, E, by=1.5, dtype=dtype)
@@ -439,6 +440,25 @@ def test_captured_graph_replays():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_another_stream_and_later_reuse():
+    """Everything of a call is on the current stream, and its workspaces stay whole while later calls on that stream take new ones."""
+    x, w = rnd(80, 300, 512).to(DEV), q.quantize_fp8(rnd(81, 400, 512).to(DEV), 128)
+    up, down = q.quantize_fp8(rnd(82, 6, 256, 512, by=0.05).to(DEV), 128), q.quantize_fp8(rnd(83, 6, 512, 256, by=0.05).to(DEV), 128)
+    l = rnd(84, 300, 6).to(DEV)
+
+    def step():
+        r = q.route_experts(l, 2, renormalize=True)
+        return [q.linear_fp8(x, w), q.experts_fp8(x, r, up, down), r.weights]
+    want = step()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = [step() for _ in range(20)]
+    s.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
 
 
 def test_two_streams_at_once():
