@@ -446,6 +446,7 @@ template <int TM, int TN, bool GROUPED> __device__ __forceinline__ bool f8_locat
 // Results of a wave's (32 G) x 128 tile from row m, weight row nw on, 32 rows at a time through `stage` (F8_STAGE bytes of LDS of this wave's own, no longer read
 // by anyone; put(i, st) writes rows 32 i .. + 31 there, F8_PITCH floats each): 16 lanes then write 128 neighbouring columns of a row.  Stored from the
 // accumulators' layout they were 32 bytes of each of 32 rows per instruction, and with the bounds unrolled 30 KiB of code: 27,000 cycles a tile, as much as 11 steps.
+// AT_ONCE passes of 4 rows without a branch between them: one by one each waited for its own reads (30,900 cycles of a routed 256 x 256 tile, now 18,300).
 __device__ __forceinline__ float f8_relu(float u) { return __builtin_elementwise_maximum(u, 0.f); }      // (a NaN stays one)
 // Where a wave's 32 G rows go and their weights (G = 4: two rows a lane).  Two dependent loads: in front of the products where registers are left, so that they are not waited for behind them.
 template <int G> struct F8Moves {
@@ -846,7 +847,7 @@ template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED> int launch_
 //   second half  wait for the next step, barrier; x4 .. x7 times w; reads the next step's x0 .. x3 and w, each fragment into its registers behind its last product
 // The exponents come the same way, a dword (four steps) of each row every two steps: as loads into registers they were waited for together with every
 // request issued before them, which emptied the ring.
-// At this rate the card is bound by power (1.6 - 1.9 GHz on normal data), and the 16 x 16 x 128 form draws less of it than 32 x 32 x 64 (alone: 4,080 against
+// 8192^3: 380 - 450 us, 2.5 - 2.9 PFLOP/s.  At this rate the card is bound by power (1.5 - 1.9 GHz on normal data), and the 16 x 16 x 128 form draws less of it than 32 x 32 x 64 (alone: 4,080 against
 // 3,500 TFLOP/s).  The compiler gives its result other registers than its addend, for which 256 accumulators leave none; so the instruction is written
 // out, in place.  An accumulator is read again 32 instructions later or behind the wait at the end, which is what its hazards ask for.
 template <int B> __device__ __forceinline__ void f8_mfma_in_place(f8_v4f& acc, const f8_v8i& w, const f8_v8i& x, uint32_t ws, uint32_t xs) {      // exponents: byte B
@@ -1042,7 +1043,7 @@ template <bool GROUPED> int launch_linear_any(const F8Args& a, int rows, int z, 
 
 // ---- y[t] = sum over the row's top_k results, in the order of choice --------------------------------------------------------------
 // The results come in fp32: rounded to the 16 bits of y first, each would cost as much as the one rounding of the sum does.  For a bf16 y, halves with block exponents
-// cost 2^-11 of each term beside the sum's 2^-8 and are half of the bytes, which bound this kernel (32768 x 4096: 115 us from fp32).
+// cost 2^-11 of each term beside the sum's 2^-8 and are half of the bytes, which bound this kernel (32768 x 4096: 115 us from fp32, 55 from halves, 5.4 TB/s).
 constexpr int COMBINE_COLUMNS = 8;
 template <int T, bool HALF> __global__ __launch_bounds__(256) void combine_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__ oe, f8_type<T>* __restrict__ y, int rows, int k, int N) {
   const int n0 = (blockIdx.x * 256 + threadIdx.x) * COMBINE_COLUMNS;
