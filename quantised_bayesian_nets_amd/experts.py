@@ -35,10 +35,10 @@ def route_experts(logits, top_k, score="softmax", bias=None, groups=1, top_group
     `groups` equal runs of experts only the `top_groups` with the largest sum of their two largest keys take part.  A logit of -inf or of its type's lowest
     value is masked: behind all others, weight 0.  A NaN makes its row's weights NaN, the row's experts stay valid."""
     _float(logits, "logits")
-    if logits.dim() not in (2, 3):
+    shape = logits.shape
+    if len(shape) not in (2, 3):
         raise ValueError("logits is [T, E] or [S, T, E]")
-    T, E = logits.shape[-2:]
-    S = logits.shape[0] if logits.dim() == 3 else 1
+    S, T, E = shape if len(shape) == 3 else (1, *shape)
     top_groups = groups if top_groups is None else top_groups
     if not 1 <= E <= MAX_EXPERTS:
         raise ValueError("1 to %d experts" % MAX_EXPERTS)
@@ -54,7 +54,7 @@ def route_experts(logits, top_k, score="softmax", bias=None, groups=1, top_group
     dev = _device(logits, bias)
     if logits.stride(-1) != 1 and E > 1:
         logits = logits.contiguous()
-    lead = (*logits.shape[:-1], top_k)
+    lead = (S, T, top_k) if len(shape) == 3 else (T, top_k)
     weights = torch.empty(lead, dtype=torch.float32, device=dev)
     experts = torch.empty(lead, dtype=torch.int32, device=dev)
     n = S * T * top_k
@@ -62,7 +62,7 @@ def route_experts(logits, top_k, score="softmax", bias=None, groups=1, top_group
         return Routing(weights, experts, torch.zeros(S * E + 1, dtype=torch.int32, device=dev), torch.empty(0, dtype=torch.int32, device=dev), E)
     L = _lib.lib()
     plan = torch.empty(S * E + 1 + n + L.qbnn_route_workspace_ints(S, T, E), dtype=torch.int32, device=dev)      # offsets, rows, workspace
-    offsets, rows = plan[:S * E + 1], plan[S * E + 1:S * E + 1 + n]
+    offsets, rows = plan.as_strided((S * E + 1,), (1,)), plan.as_strided((n,), (1,), S * E + 1)
     at = plan.data_ptr()
     _launch("route_experts", dev, L.qbnn_route_experts, _lib.ROUTE.pack(
         logits.data_ptr(), logits.stride(0) if len(lead) == 3 else 0, logits.stride(-2), 0 if bias is None else bias.data_ptr(),
@@ -83,9 +83,11 @@ def experts_fp8(x, routing, w_up, w_down, b_up=None, b_down=None, out_dtype=None
     linear_fp8, for float16 the first and for float32 both take the exact one: a hidden value next to a rounding border moves by a whole step."""
     if not isinstance(routing, Routing):
         raise TypeError("routing is a Routing (route_experts)")
-    for w in (w_up, w_down):
-        if not isinstance(w, F8Tensor) or w.block_rows != BLOCK or len(w.shape) not in (3, 4):
-            raise TypeError("w_up and w_down are F8Tensors with block_rows 128, [E, rows, columns] or [S, E, rows, columns]")
+    if not isinstance(w_up, F8Tensor) or not isinstance(w_down, F8Tensor) or w_up.block_rows != BLOCK or w_down.block_rows != BLOCK:
+        raise TypeError("w_up and w_down are F8Tensors with block_rows 128")
+    us, ws = w_up.shape, w_down.shape
+    if len(us) not in (3, 4) or len(ws) not in (3, 4):
+        raise TypeError("w_up and w_down are [E, rows, columns] or [S, E, rows, columns]")
     if isinstance(x, F8Tensor):
         if x.block_rows != 1:
             raise TypeError("x is a float tensor or an F8Tensor with block_rows 1")
@@ -97,17 +99,17 @@ def experts_fp8(x, routing, w_up, w_down, b_up=None, b_down=None, out_dtype=None
     (*lead, k), E = routing.experts.shape, routing.n_experts
     S, T = lead if len(lead) == 2 else (1, lead[0])
     xs = x.shape
-    H, D = w_up.shape[-2:]
-    N = w_down.shape[-2]
+    *up_sets, H, D = us
+    *down_sets, N, Hd = ws
     if len(xs) not in (2, 3) or xs[-2] != T or xs[-1] != D or (len(xs) == 3 and xs[0] not in (1, S)):
         raise ValueError("x is [%d or 1, %d, %d] for this routing and w_up" % (S, T, D))
-    if w_down.shape[-1] != H or H < 1 or N < 1:
-        raise ValueError("w_up [.., H, D] and w_down [.., N, H] do not fit: %s and %s" % (w_up.shape, w_down.shape))
-    for w in (w_up, w_down):
-        if w.shape[:-2] not in ((E,), (1, E), (S, E)):
-            raise ValueError("the routing has %d experts and %d samples" % (E, S))
-    b_up = _bias(b_up, (w_up.shape[:-1],), "like w_up without its columns")
-    b_down = _bias(b_down, (w_down.shape[:-1],), "like w_down without its columns")
+    if Hd != H or H < 1 or N < 1:
+        raise ValueError("w_up [.., H, D] and w_down [.., N, H] do not fit: %s and %s" % (tuple(us), tuple(ws)))
+    sets = ([E], [1, E], [S, E])
+    if up_sets not in sets or down_sets not in sets:
+        raise ValueError("the routing has %d experts and %d samples" % (E, S))
+    b_up = _bias(b_up, ((*up_sets, H),), "like w_up without its columns")
+    b_down = _bias(b_down, ((*down_sets, N),), "like w_down without its columns")
     held = isinstance(x, F8Tensor)
     dev = _device(x.data if held else x, routing.weights, routing.offsets, routing.rows, w_up.data, w_down.data, b_up, b_down)
     y = torch.empty((*lead, N), dtype=out_dtype, device=dev)
@@ -129,6 +131,6 @@ def experts_fp8(x, routing, w_up, w_down, b_up=None, b_down=None, out_dtype=None
         xf, xf_ss, xf_rs, xq, xe, routing.offsets.data_ptr(), routing.rows.data_ptr(), routing.weights.data_ptr(),
         up.data_ptr(), ue.data_ptr(), H * dp, -(-H // BLOCK) * ds, 0 if b_up is None else b_up.data_ptr(), H,
         down.data_ptr(), de.data_ptr(), N * hp, -(-N // BLOCK) * hs, 0 if b_down is None else b_down.data_ptr(), N,
-        h, he, o, y.data_ptr(), S, T, E, k, x_rows, D, H, N, w_up.shape[:-2].numel(), w_down.shape[:-2].numel(),
+        h, he, o, y.data_ptr(), S, T, E, k, x_rows, D, H, N, E if len(us) == 3 else up_sets[0] * E, E if len(ws) == 3 else down_sets[0] * E,
         0 if out_dtype == torch.bfloat16 else 1 if out_dtype == torch.float16 else 3, x_type, FLOAT_TYPES[out_dtype]))
     return y

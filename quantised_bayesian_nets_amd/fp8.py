@@ -43,7 +43,8 @@ class F8Tensor:
 
     @property
     def shape(self):
-        return torch.Size((*self.data.shape[:-1], self.columns))
+        *lead, _ = self.data.shape
+        return torch.Size((*lead, self.columns))
 
     @property
     def device(self):
