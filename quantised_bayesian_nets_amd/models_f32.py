@@ -36,6 +36,8 @@ class Linear(nn.Module):
 
     def sampled(self, device, eps=None):
         """W_s = mu + eps_s * sigma of the active mc_context: fp32 [S, out_features * in_features]."""
+        if device.type != "cuda":
+            raise RuntimeError("qbnn layers run on an MI355X only (no CPU fallback)")
         S = _MC.samples
         if self._sigma is None or self._sigma.device != device:
             self._sigma = F.softplus(self.std.detach().cpu().float()).to(device).contiguous()   # one-time, same op as the reference
@@ -54,8 +56,6 @@ class Linear(nn.Module):
 
     def forward(self, x, act=0, eps=None):
         """x fp32 [S or 1, B, in_features] -> [S, B, out_features]."""
-        if x.device.type != "cuda":
-            raise RuntimeError("qbnn layers run on an MI355X only (no CPU fallback)")
         S = _MC.samples
         w = self.sampled(x.device, eps)
         n = w.shape[1]
