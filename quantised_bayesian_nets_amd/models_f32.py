@@ -49,7 +49,7 @@ class Linear(nn.Module):
             w = torch.empty((S, n), dtype=torch.float32, device=device)
             if eps is not None:
                 eps = eps.to(device=device, dtype=torch.float32).contiguous()
-            with timed("sample_weights_f32"):
+            with torch.cuda.device(device), timed("sample_weights_f32"):      # the stream of the draws' device, where what reads them runs
                 _lib.check(_lib.lib().qbnn_sample_weights_f32(_lib.ptr(self._mu_dev), _lib.ptr(self._sigma), n, _MC.seed, self.layer_id,
                                                               _MC.sample_begin, S, _lib.ptr(eps), _lib.ptr(w), _lib.current_stream()))
         return w
@@ -63,7 +63,7 @@ class Linear(nn.Module):
         y = torch.empty((S, B, self.out_features), dtype=torch.float32, device=x.device)
         xs = 0 if x.shape[0] == 1 else x[0].numel()
         b = self._bias_dev
-        with timed("linear_f32"):
+        with torch.cuda.device(x.device), timed("linear_f32"):
             _lib.check(_lib.lib().qbnn_linear_f32_mc(_lib.ptr(x.contiguous()), xs, _lib.ptr(w), n, _lib.ptr(b), _lib.ptr(y), y[0].numel(),
                                                      B, self.in_features, self.out_features, act, S, _lib.current_stream()))
         return y
