@@ -35,7 +35,9 @@ class Linear(nn.Module):
         return 0.5 * (2 * torch.log(sp / sigma) - 1 + (sigma / sp).pow(2) + ((0 - mu) / sp).pow(2)).sum()
 
     def sampled(self, device, eps=None):
-        """W_s = mu + eps_s * sigma of the active mc_context: fp32 [S, out_features * in_features]."""
+        """W_s = mu + eps_s * sigma of the active mc_context: fp32 [S, out_features * in_features].  eps: as many values, or None."""
+        if eps is not None and eps.numel() < _MC.samples * self.weight.numel():
+            raise ValueError("eps is [%d, %d]" % (_MC.samples, self.weight.numel()))
         if device.type != "cuda":
             raise RuntimeError("qbnn layers run on an MI355X only (no CPU fallback)")
         S = _MC.samples

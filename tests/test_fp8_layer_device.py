@@ -100,3 +100,14 @@ def test_every_launch_is_on_the_inputs_device(monkeypatch, kind):
     with q.mc_context(3, 1):
         m(Tensor(1, 2, 6))
     assert len(seen) >= 2 and seen[0][0] == "qbnn_sample_weights_f32" and {device for _, device in seen} == {1}
+
+
+@pytest.mark.parametrize("kind", [fp8.Linear, models_f32.Linear])
+def test_noise_for_fewer_samples_is_refused(recorder, kind):
+    """eps is read [samples, out_features * in_features]: one that is shorter would be read past its end."""
+    m = kind(6, 4, True)
+    with q.mc_context(3, 1):
+        for eps in (torch.zeros(24), torch.zeros(2, 24), torch.zeros(3, 23)):
+            with pytest.raises(ValueError, match="eps"):
+                m(torch.zeros(1, 2, 6), eps=eps)
+    assert recorder.calls == []
