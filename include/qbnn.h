@@ -669,10 +669,10 @@ int qbnn_linear_f8_mc(const qbnn_f8_linear* host_desc, void* stream);
 
 /* Router: logits [S][T][E] (strides in elements, experts contiguous) -> weights / experts [S][T][top_k] (descending keys), offsets [S E + 1] and rows
  * [S T top_k]: the flat indices of the choices sorted by (sample, expert), stable.
- *   score s = softmax or sigmoid of the logits; key = s + bias[e] (compared as 64-bit values, ties to the lowest index); with groups > 1 only the
- *   top_groups groups of E / groups neighbours with the largest sum of their two largest keys take part; weight = s, divided by the sum of the chosen with
- *   `renormalize` (0 if that is 0), times scale.  A logit of -inf or of the type's lowest value is masked: behind all others, weight 0.  A NaN in a
- *   row makes its weights NaN; its experts are valid indices all the same.  workspace: qbnn_route_workspace_ints(S, T, E) ints. */
+ *   score s = softmax or sigmoid of the logits; key = s + bias[e] (compared as 64-bit values; of equal ones the larger logit goes first, then the lowest index);
+ *   with groups > 1 only the top_groups groups of E / groups neighbours with the largest sum of their two largest keys take part, and equal keys go by the index
+ *   alone; weight = s, divided by the sum of the chosen with `renormalize` (0 if that is 0), times scale.  A logit of -inf or of the type's lowest value is
+ *   masked: behind all others, weight 0.  A NaN in a row, or +inf under softmax, makes its weights NaN; its experts are valid indices all the same.  workspace: qbnn_route_workspace_ints(S, T, E) ints. */
 typedef struct qbnn_route {
   const void* logits; int64_t logits_ss, logits_rs;
   const float* bias;

@@ -1,10 +1,11 @@
 // libqbnn_hip.so: the router of a layer of experts.
 //   scores    s = softmax(l) or sigmoid(l) over a row's E logits;  key = s + bias (what is compared), weight = s (what is multiplied)
 //   groups    E / groups neighbouring experts each; a group counts its two largest keys, the best `top_groups` groups stay
-//   choice    the top_k largest keys, ties to the lowest index; weights optionally divided by their sum, times `scale`
+//   choice    the top_k largest keys; of equal ones with one group the larger logit first, then the lowest index; weights optionally divided by their sum, times `scale`
 //   order     the (row, choice) pairs of a sample sorted by expert, stable: what the experts' products walk
 // The choice is that of 64-bit keys: two experts whose scores differ only behind fp32's last place are still told apart, so it does not depend on
-// the order in which a row's sum was taken.
+// the order in which a row's sum was taken.  Both scores increase with the logit, so without a bias and groups the logits are compared themselves; the rule for equal
+// keys makes that the same choice as under a bias of zeros, also where scores are equal to the last bit of 64 (sigmoid above 37, softmax 746 below the largest).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -211,7 +212,7 @@ template <int T, int NP> __device__ __forceinline__ void route_exact_row(const R
   if (!by_logit) {
 #pragma unroll 1
     for (int e = lane; e < a.E; e += 64) {
-      const double x = keys[e], z = exp(a.sigmoid ? -x : x - top), p = a.sigmoid ? 1. / (1. + z) : z;
+      const double x = keys[e], z = exp(a.sigmoid ? -x : x == top ? 0. : x - top), p = a.sigmoid ? 1. / (1. + z) : z;      // (infinite logits share the row)
       keys[e] = x > -INFINITY ? p : -1.;
       total += x > -INFINITY ? p : 0.;
     }
@@ -238,6 +239,7 @@ template <int T, int NP> __device__ __forceinline__ void route_exact_row(const R
     key[i] = in ? keys[e] : -INFINITY;
     idx[i] = in ? e : 0x7fffffff;
   }
+  const bool by_score = !by_logit && a.groups == 1;
   for (int j = 0; j < a.k; ++j) {
     double b = key[0];
     int bi = idx[0];
@@ -250,6 +252,27 @@ template <int T, int NP> __device__ __forceinline__ void route_exact_row(const R
     route_join<8>(b, bi);
     route_join<16>(b, bi);
     route_join<32>(b, bi);
+    if (by_score && b > -INFINITY) {                            // of equal keys the one with the larger logit, as without a bias
+      bool tied = false;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) tied |= key[i] == b && idx[i] != bi && idx[i] != 0x7fffffff;
+      if (__any(tied)) {
+        double most = -INFINITY;
+        bi = 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const bool in = key[i] == b && idx[i] != 0x7fffffff;
+          const double v = in ? (double)f8_load<T>(l[idx[i]]) : -INFINITY;
+          if (in && (v > most || (v == most && idx[i] < bi))) { most = v; bi = idx[i]; }
+        }
+        route_join<1>(most, bi);
+        route_join<2>(most, bi);
+        route_join<4>(most, bi);
+        route_join<8>(most, bi);
+        route_join<16>(most, bi);
+        route_join<32>(most, bi);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NP; ++i) if (idx[i] == bi) { key[i] = -INFINITY; idx[i] = 0x7fffffff; }
     if (lane == 0) choice[j] = (uint32_t)bi;
@@ -363,6 +386,7 @@ template <int T, int L, int KEY> __global__ __launch_bounds__(route_waves(L) * 6
           sum += key[i];
         }
         sum = route_sumf<L>(sum);
+        unsure = !(top < INFINITY);                             // infinite logits share the row: not a sum of these terms
         const float over = __builtin_amdgcn_rcpf(sum);
         worst = 2 * 32 * 1.1920929e-7f * over;
 #pragma unroll

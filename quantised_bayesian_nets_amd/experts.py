@@ -30,10 +30,11 @@ class Routing:
 def route_experts(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, renormalize=False, scale=1.0):
     """logits float [T, E] or [S, T, E] -> Routing.
 
-    score "softmax" or "sigmoid" of the logits; what is compared is score + bias[e] (float32 [E], e.g. for balance; compared as 64-bit values, ties to the
-    lowest index), what the results are weighted with is the score, divided by the chosen ones' sum with `renormalize`, times `scale`.  groups > 1: of
-    `groups` equal runs of experts only the `top_groups` with the largest sum of their two largest keys take part.  A logit of -inf or of its type's lowest
-    value is masked: behind all others, weight 0.  A NaN makes its row's weights NaN, the row's experts stay valid."""
+    score "softmax" or "sigmoid" of the logits; what is compared is score + bias[e] (float32 [E], e.g. for balance) as a 64-bit value, and of equal ones the larger
+    logit goes first and then the lowest index: a bias that is the same for all changes no choice.  What the results are weighted with is the score, divided by the
+    chosen ones' sum with `renormalize`, times `scale`.  groups > 1: of `groups` equal runs of experts only the `top_groups` with the largest sum of their two
+    largest keys take part, and equal keys go by the index alone.  A logit of -inf or of its type's lowest value is masked: behind all others, weight 0.  A NaN, or for
+    softmax a logit of +inf, makes its row's weights NaN, the row's experts stay valid."""
     _float(logits, "logits")
     shape = logits.shape
     if len(shape) not in (2, 3):
