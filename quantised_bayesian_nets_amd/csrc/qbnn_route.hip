@@ -45,6 +45,12 @@ template <int T> __device__ __forceinline__ float route_lowest() {
 }
 __device__ __forceinline__ float route_exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896340736f); }      // off by at most (|v| + 2) 2^-23 of it
 
+// e^(l - top) to a unit or two in the last place wherever it lies: the difference's rounding, |l - top| 2^-24 of the result, is put back
+__device__ __forceinline__ float route_softmax_term(float l, float top) {
+  const float d = l - top, b = d - l, lost = (l - (d - b)) - (top + b), z = expf(d);
+  return z > 0.f && z < 1.f ? z + z * lost : z;                 // (0: past the range, and lost may be NaN)
+}
+
 // ---- reductions over the L lanes (a power of two) of a row: each step's partner holds what the step before left in all lanes of its half ------------
 template <int CTRL> __device__ __forceinline__ uint32_t route_dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
 template <int STEP> __device__ __forceinline__ uint32_t route_partner(uint32_t v) {
@@ -499,7 +505,7 @@ template <int T, int L, int KEY> __global__ __launch_bounds__(route_waves(L) * 6
   for (int i = threadIdx.x; i < n; i += NW * 64) {
     const int r = i / a.k, e = (int)choice[i];
     const float l = f8_load<T>(base[(int64_t)r * a.l_rs + e]), top = row_top[r];
-    float p = a.sigmoid ? 1.f / (1.f + route_exp(-l)) : route_exp(l - top) / row_sum[r];
+    float p = a.sigmoid ? 1.f / (1.f + expf(-l)) : route_softmax_term(l, top) / row_sum[r];
     if (!(l > route_lowest<T>())) p = 0.f;
     if (top != top) p = NAN;
     part[i] = p;
