@@ -6,6 +6,7 @@ few large weights (mu + sigma eps has no bound) do not cost the others their pre
 layer run in one launch, there is no CPU path, and nothing is differentiated: the engine evaluates.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, layers, models_f32
 from .layers import _MC
@@ -63,8 +64,8 @@ class F8Tensor:
 
 def _device(*tensors):
     """The device of a call's tensors (None entries left out).  Refuses what the engine would silently get wrong: tensors off the GPU, on several devices, or
-    waiting for a gradient."""
-    dev = None
+    waiting for a gradient (backward, or a tangent in forward mode)."""
+    dev, dual = None, forward_ad._current_level >= 0
     for t in tensors:
         if t is None:
             continue
@@ -74,7 +75,7 @@ def _device(*tensors):
             dev = t.device
         elif t.device != dev:
             raise ValueError("tensors on %s and %s in one call" % (dev, t.device))
-        if t.requires_grad and torch.is_grad_enabled():
+        if t.requires_grad and torch.is_grad_enabled() or dual and forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError("the engine evaluates only: call it under torch.no_grad() or with tensors that do not require a gradient")
     return dev
 
