@@ -28,9 +28,9 @@ extern "C" {
 #endif
 
 /* ABI version of this header: qbnn_version() of the loaded library must equal it (bumped whenever a prototype below changes;
- * 3: the 8-bit floating-point linear layers and routed experts; 2 = round 5: qbnn_block_chain_i8_multi_launch takes a_hi and w_layout, qbnn_block_down_i8_multi_launch w_layout, qbnn_block_desc carries w_layout; round 4's `stream` argument
+ * 4: qbnn_linear_f8_tile, qbnn_experts_f8_tiles; 3: the 8-bit floating-point linear layers and routed experts; 2 = round 5: qbnn_block_chain_i8_multi_launch takes a_hi and w_layout, qbnn_block_down_i8_multi_launch w_layout, qbnn_block_desc carries w_layout; round 4's `stream` argument
  * of the _multi_prepare calls). */
-#define QBNN_ABI_VERSION 3
+#define QBNN_ABI_VERSION 4
 
 #define QBNN_OK 0
 #define QBNN_E_INVALID (-1)     /* bad argument / unsupported shape   */
@@ -663,6 +663,9 @@ typedef struct qbnn_f8_linear {
 } qbnn_f8_linear;
 
 int qbnn_linear_f8_mc(const qbnn_f8_linear* host_desc, void* stream);
+/* The tile that a call takes, without launching it: rows << 16 | weight rows; 16 or 32 rows: operands straight from memory, 64 and more: through LDS.  0: an empty
+ * call, < 0: one that qbnn_linear_f8_mc refuses. */
+int32_t qbnn_linear_f8_tile(const qbnn_f8_linear* host_desc);
 
 #define QBNN_ROUTE_MAX_EXPERTS 1024
 #define QBNN_ROUTE_MAX_CHOICES 32
@@ -691,6 +694,7 @@ int qbnn_route_experts(const qbnn_route* host_desc, void* stream);
  * expert in elements).  Hidden rows are quantised in blocks of 128; exact: bit 0 the first product, bit 1 the second (see qbnn_f8_linear); a result whose weight
  * is 0 is left out, whatever it is.  The weighted results are fp32 and summed in the order of j, rounded once to y_type (QBNN_F32 .. QBNN_F16); where y is bf16
  * and more than 32 rows go to an expert on average they may wait for the sum as fp16 with one power of two per 128 columns (2^-11 of each, beside the sum's own 2^-8).
+ * Gathered rows of 4 GiB and more (x in e4m3: x_rows times D up to a multiple of 128) go through the form for few rows, which is slower.
  * Workspaces: h [S T top_k][Hp], h_exp [S T top_k][Hs] (Hp, Hs of H columns), o of S T top_k N 4 bytes, at a multiple of 16. */
 typedef struct qbnn_f8_experts {
   const void* x_float; int64_t x_float_ss, x_float_rs;
@@ -703,6 +707,7 @@ typedef struct qbnn_f8_experts {
 } qbnn_f8_experts;
 
 int qbnn_experts_f8(const qbnn_f8_experts* host_desc, void* stream);
+int qbnn_experts_f8_tiles(const qbnn_f8_experts* host_desc, int32_t* tiles);      /* of both products, as qbnn_linear_f8_tile */
 
 const char* qbnn_last_error(void);
 int qbnn_version(void);

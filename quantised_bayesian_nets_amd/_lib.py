@@ -121,11 +121,11 @@ EXPORTS = ["qbnn_mlp_bbb_f32_mc", "qbnn_mlp_bbb_f32_workspace_floats", "qbnn_pac
            "qbnn_dequant_softmax_mc", "qbnn_flatten_nchw_mc", "qbnn_flatten_nchw_rows_mc", "qbnn_add_relu_q_mc", "qbnn_sample_weights_f32", "qbnn_linear_f32_mc", "qbnn_head_i8_mc", "qbnn_reduce_moments", "qbnn_finalize_moments", "qbnn_classification_metrics", "qbnn_regression_metrics",
            "qbnn_conv2d_f32_mc", "qbnn_conv2d_f32_fused_mc", "qbnn_conv2d_f32_blocks", "qbnn_observe_partials_f32_mc", "qbnn_grid_to_i8_mc", "qbnn_fake_quant_ex_f32_mc", "qbnn_conv2d_q8_blocks", "qbnn_conv2d_q8_f32_mc", "qbnn_add_q8_blocks", "qbnn_add_q8_f32_mc", "qbnn_fake_quant_add_q8_mc", "qbnn_qat_weights_mc", "qbnn_sample_weights_f32_batch", "qbnn_affine_f32_mc", "qbnn_pool2d_f32_mc", "qbnn_flatten_nchw_f32_mc", "qbnn_softmax_f32_mc", "qbnn_observe_f32_mc", "qbnn_fake_quant_f32_mc", "qbnn_sample_weights_f32_strided", "qbnn_sample_weights_f32_ohwi",
            "qbnn_dropout_mask_f32_mc", "qbnn_dropout_f32_mc", "qbnn_conv2d_f32_drop_mc",
-           "qbnn_quantize_f8", "qbnn_linear_f8_mc", "qbnn_experts_f8", "qbnn_route_workspace_ints", "qbnn_route_experts",
+           "qbnn_quantize_f8", "qbnn_linear_f8_mc", "qbnn_experts_f8", "qbnn_linear_f8_tile", "qbnn_experts_f8_tiles", "qbnn_route_workspace_ints", "qbnn_route_experts",
            "qbnn_last_error", "qbnn_version"]
 
 
-ABI_VERSION = 3      # = QBNN_ABI_VERSION of include/qbnn.h
+ABI_VERSION = 4      # = QBNN_ABI_VERSION of include/qbnn.h
 
 
 def lib_path():
@@ -227,6 +227,8 @@ def lib():
         L.qbnn_quantize_f8.argtypes = [vp, i32, i64, i64, i64, i32, i32, i32, vp, vp, vp]
         L.qbnn_linear_f8_mc.argtypes = [C.c_char_p, vp]
         L.qbnn_experts_f8.argtypes = [C.c_char_p, vp]
+        L.qbnn_linear_f8_tile.argtypes = [C.c_char_p]
+        L.qbnn_experts_f8_tiles.argtypes = [C.c_char_p, C.POINTER(i32)]
         L.qbnn_route_workspace_ints.argtypes = [i32, i32, i32]
         L.qbnn_route_workspace_ints.restype = i64
         L.qbnn_route_experts.argtypes = [C.c_char_p, vp]

@@ -193,11 +193,14 @@ struct F8Args {
   const float* bias; int64_t bias_ss;
   uint8_t* y; uint8_t* ye; int64_t y_ss;        // y_ss in elements
   int M, N, Kb, Sp, relu, y_rs, ye_rs;          // y row pitch in elements, exponent pitch of an e4m3 result
+  int samples, fold;                            // direct form: fold != 0: row tiles of a sample, tiles of all samples numbered over blockIdx.y and z
   // ragged groups: rows offsets[g] .. offsets[g + 1] of the routed order, with weight set g % w_groups
   const int32_t* offsets; int groups, w_groups;
   const int32_t* rows; int topk, x_rows;        // rows != null: x row of routed row i = (rows[i] / topk) % x_rows, else i
   const int32_t* y_rows; const float* scale;    // y_rows != null: result row i goes to y_rows[i], times scale[y_rows[i]]
 };
+
+constexpr int F8_FOLD = 32768;
 
 struct F8Tile { int m0, m1, set, sample; };     // rows m0 .. m1 - 1, weight set, sample (0 for groups: rows are global)
 
@@ -245,6 +248,11 @@ template <int TM, bool GROUPED> __device__ __forceinline__ bool f8_find_tile(con
     return false;
   }
 }
+// The row that offsets into x count from: the tile's first, or x's own first where rows are gathered
+template <bool GROUPED> __device__ __forceinline__ int f8_x_base(const F8Args& a, const F8Tile& t) {
+  if constexpr (GROUPED) { if (a.rows) return 0; }
+  return t.m0;
+}
 template <bool GROUPED> __device__ __forceinline__ int f8_x_row(const F8Args& a, int i) {
   if constexpr (GROUPED) { if (a.rows) return (a.rows[i] / a.topk) % a.x_rows; }
   return i;
@@ -280,7 +288,14 @@ __global__ __launch_bounds__(NW * 64) void linear_f8_direct_kernel(const F8Args 
   __shared__ __attribute__((aligned(16))) f8_v4f red[NW > 1 ? NW : 1][MT * NT * 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, h = lane >> 4;
   F8Tile t;
-  if (!f8_find_tile<16 * MT, GROUPED>(a, blockIdx.y, blockIdx.z, t)) return;
+  int row_tile = blockIdx.y, sample = blockIdx.z;
+  if (a.fold) {
+    const int64_t q = (int64_t)blockIdx.z * F8_FOLD + blockIdx.y;
+    sample = (int)(q / a.fold);
+    row_tile = (int)(q - (int64_t)sample * a.fold);
+    if (sample >= a.samples) return;
+  }
+  if (!f8_find_tile<16 * MT, GROUPED>(a, row_tile, sample, t)) return;
   const int n0 = blockIdx.x * (16 * NT);
   const int64_t pitch = (int64_t)a.Kb * 128;
   const uint8_t* xp[MT]; const uint8_t* xep[MT];
@@ -404,10 +419,14 @@ __global__ __launch_bounds__(NW * 64) void linear_f8_direct_kernel(const F8Args 
   }
 }
 
-template <int MT, int NT, int NW, int D, int OUT, bool EXACT, bool GROUPED> int launch_direct(const F8Args& a, int tiles, int z, hipStream_t st) {
-  if (tiles > 65535 || z > 65535) return f8_fail("qbnn_linear_f8: %ld row tiles x %ld samples do not fit a grid", tiles, z);
-  hipLaunchKernelGGL((linear_f8_direct_kernel<MT, NT, NW, D, OUT, EXACT, GROUPED>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)tiles, (unsigned)z),
-                     dim3(NW * 64), 0, st, a);
+template <int MT, int NT, int NW, int D, int OUT, bool EXACT, bool GROUPED> int launch_direct(const F8Args& a, int64_t tiles, int z, hipStream_t st) {
+  F8Args c = a;
+  dim3 grid((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)tiles, (unsigned)z);
+  if (tiles > 65535 || z > 65535) {                             // (f8_fits: fewer than 2^31 of them)
+    c.samples = z; c.fold = (int)tiles;
+    grid.y = F8_FOLD; grid.z = (unsigned)((tiles * z + F8_FOLD - 1) / F8_FOLD);
+  }
+  hipLaunchKernelGGL((linear_f8_direct_kernel<MT, NT, NW, D, OUT, EXACT, GROUPED>), grid, dim3(NW * 64), 0, st, c);
   return qbnn_check_launch_msg("qbnn_linear_f8");
 }
 
@@ -657,17 +676,16 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
   int n0;
   if (!f8_locate<C::TM, C::TN, GROUPED>(a, tiles_m, tiles_n, samples, t, n0)) return;
   const int64_t pitch = (int64_t)a.Kb * 128;
-  const uint8_t* xg = a.x + (int64_t)t.sample * a.x_ss;
+  const int base = f8_x_base<GROUPED>(a, t);
+  const uint8_t* xg = a.x + (int64_t)t.sample * a.x_ss + base * pitch;
   const uint8_t* wg = a.w + (int64_t)t.set * a.w_ss + n0 * pitch;
-  if constexpr (!GROUPED) xg += t.m0 * pitch;
 
   // per-lane byte offsets of this wave's DMA requests; rows behind the last repeat it (their results are not stored)
   uint32_t xo[C::PX], wo[C::PW];
 #pragma unroll
   for (int p = 0; p < C::PX; ++p) {
     const int r = (p * C::WAVES + wave) * 8 + (lane >> 3), i = min(t.m0 + r, t.m1 - 1);
-    const int row = GROUPED ? f8_x_row<GROUPED>(a, i) : i - t.m0;
-    xo[p] = (uint32_t)(row * pitch) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
+    xo[p] = (uint32_t)((f8_x_row<GROUPED>(a, i) - base) * pitch) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
   }
 #pragma unroll
   for (int p = 0; p < C::PW; ++p) {
@@ -683,10 +701,10 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_f8_tiled_kernel(const 
     for (int p = 0; p < C::PW; ++p) f8_dma16(wg + kb * 128, wo[p], at + 2 * C::XB + buf * C::WB + p * (C::WAVES * 1024));
   };
 
-  const uint8_t* xeg = a.xe + (int64_t)t.sample * a.xe_ss;
+  const uint8_t* xeg = a.xe + (int64_t)t.sample * a.xe_ss + (int64_t)base * a.Sp;
   uint32_t xeo[MI];
 #pragma unroll
-  for (int i = 0; i < MI; ++i) xeo[i] = (uint32_t)f8_x_row<GROUPED>(a, min(t.m0 + (wm * MI + i) * 32 + r32, t.m1 - 1)) * (uint32_t)a.Sp;
+  for (int i = 0; i < MI; ++i) xeo[i] = (uint32_t)(f8_x_row<GROUPED>(a, min(t.m0 + (wm * MI + i) * 32 + r32, t.m1 - 1)) - base) * (uint32_t)a.Sp;
   const uint8_t* we = a.we + (int64_t)t.set * a.we_ss + (int64_t)min((n0 >> 7) + wn, (a.N - 1) >> 7) * a.Sp;
   F8Exponents xs[MI], ws;
 
@@ -834,8 +852,7 @@ template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED> int launch_
   using C = F8Tiled<MI, WM, WN>;
   static std::atomic<uint64_t> attr{0};
   if (int rc = qbnn_ensure_dyn_lds((const void*)linear_f8_tiled_kernel<MI, WM, WN, OUT, EXACT, GROUPED>, &attr, C::LDS)) return rc;
-  const int64_t tm = (rows + C::TM - 1) / C::TM + (GROUPED ? std::min(a.groups, rows) : 0), tn = (a.N + C::TN - 1) / C::TN;
-  if (tm * tn * z > 0x7fffffff) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
+  const int64_t tm = ((int64_t)rows + C::TM - 1) / C::TM + (GROUPED ? std::min(a.groups, rows) : 0), tn = (a.N + C::TN - 1) / C::TN;
   hipLaunchKernelGGL((linear_f8_tiled_kernel<MI, WM, WN, OUT, EXACT, GROUPED>), dim3((unsigned)(tm * tn * z)), dim3(C::WAVES * 64), C::LDS, st, a, (int)tm, (int)tn, z);
   return qbnn_check_launch_msg("qbnn_linear_f8");
 }
@@ -869,19 +886,19 @@ __global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, i
   int n0;
   if (!f8_locate<256, 256, GROUPED>(a, tiles_m, tiles_n, samples, t, n0)) return;
   const int64_t pitch = (int64_t)a.Kb * 128;
-  const uint8_t* xg = a.x + (int64_t)t.sample * a.x_ss;
+  const int base = f8_x_base<GROUPED>(a, t);
+  const uint8_t* xg = a.x + (int64_t)t.sample * a.x_ss + base * pitch;
   const uint8_t* wg = a.w + (int64_t)t.set * a.w_ss + n0 * pitch;
-  if constexpr (!GROUPED) xg += t.m0 * pitch;
   uint32_t xo[8], wo[8];
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
     const int r = (p * 4 + wave) * 8 + (lane >> 3), i = min(t.m0 + r, t.m1 - 1), piece = ((lane & 7) ^ ((r >> 1) & 7)) << 4;
-    xo[p] = (uint32_t)((GROUPED ? f8_x_row<GROUPED>(a, i) : i - t.m0) * pitch) + piece;
+    xo[p] = (uint32_t)((f8_x_row<GROUPED>(a, i) - base) * pitch) + piece;
     wo[p] = (uint32_t)(min(r, a.N - 1 - n0) * pitch) + piece;
   }
-  const uint8_t* xeg = a.xe + (int64_t)t.sample * a.xe_ss;
+  const uint8_t* xeg = a.xe + (int64_t)t.sample * a.xe_ss + (int64_t)base * a.Sp;
   const uint8_t* weg = a.we + (int64_t)t.set * a.we_ss + (int64_t)min((n0 >> 7) + wn, (a.N - 1) >> 7) * a.Sp;
-  const uint32_t xeo = (uint32_t)f8_x_row<GROUPED>(a, min(t.m0 + (int)threadIdx.x, t.m1 - 1)) * (uint32_t)a.Sp;      // of row threadIdx.x
+  const uint32_t xeo = (uint32_t)(f8_x_row<GROUPED>(a, min(t.m0 + (int)threadIdx.x, t.m1 - 1)) - base) * (uint32_t)a.Sp;      // of row threadIdx.x
   const uint32_t lds0 = lds_addr_of(lds) + wave * 1024, ldse = lds_addr_of(lds) + E0 + wave * 256;
   const int last = a.Kb - 1;
   // requests past the last step repeat its bytes, into buffers that are not read again (no branch in the loop)
@@ -988,43 +1005,63 @@ __global__ __launch_bounds__(256, 1) void linear_f8_big_kernel(const F8Args a, i
 template <int OUT, bool GROUPED> int launch_big(const F8Args& a, int rows, int z, hipStream_t st) {
   static std::atomic<uint64_t> attr{0};
   if (int rc = qbnn_ensure_dyn_lds((const void*)linear_f8_big_kernel<OUT, GROUPED>, &attr, F8_BIG_LDS)) return rc;
-  const int64_t tm = (rows + 255) / 256 + (GROUPED ? std::min(a.groups, rows) : 0), tn = (a.N + 255) / 256;
-  if (tm * tn * z > 0x7fffffff) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
+  const int64_t tm = ((int64_t)rows + 255) / 256 + (GROUPED ? std::min(a.groups, rows) : 0), tn = (a.N + 255) / 256;
   hipLaunchKernelGGL((linear_f8_big_kernel<OUT, GROUPED>), dim3((unsigned)(tm * tn * z)), dim3(256), F8_BIG_LDS, st, a, (int)tm, (int)tn, z);
   return qbnn_check_launch_msg("qbnn_linear_f8");
 }
 
 // Whether the products go through LDS tiles.  rows: the rows of one sample, or all routed rows.  Offsets are 32 bits wide there: of a gathered row's bytes from the
-// first, of any row's exponents, of a weight row's in its tile.
+// first, of a row's in its tile.
 template <bool GROUPED> int f8_rows_each(const F8Args& a, int rows) { return GROUPED ? (rows + a.groups - 1) / a.groups : rows; }
 template <bool GROUPED> bool f8_tiled(const F8Args& a, int rows) {
-  const int64_t far = GROUPED ? (int64_t)(a.rows ? a.x_rows : rows) * a.Kb * 128 : (int64_t)rows * a.Sp;
+  const int64_t far = GROUPED && a.rows ? (int64_t)a.x_rows * a.Kb * 128 : 0;
   return f8_rows_each<GROUPED>(a, rows) > 32 && far < ((int64_t)1 << 32) && a.Kb < (1 << 16);
 }
-template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, int rows, int z, hipStream_t st) {
+// The form of a call: rows x weight rows of a tile, the direct form up to 32 rows and through LDS from 64 on.
+struct F8Form { int tm, tn; };
+template <bool GROUPED> F8Form f8_form(const F8Args& a, int rows, int z, int type, bool exact) {
   const int spare = GROUPED ? std::min(a.groups, rows) : 0;      // each group with rows may end inside a tile
   const int per = f8_rows_each<GROUPED>(a, rows);
   const auto tiles = [&](int tm, int tn) { return (int64_t)z * ((rows + tm - 1) / tm + spare / 2) * ((a.N + tn - 1) / tn); };
   // The largest tile that still gives the 256 CUs work: fewer bytes through LDS per product, but 256 x 256 holds a CU for itself.  Measured the other way round (us):
   // 128 x 128 for 64 x 128 with 330 - 600 tiles 69 -> 58 (5 x 12 groups of 75, fp16) and 28.6 -> 23.8 (100 x 128 x 500 x 800, fp32), with 32 - 64 tiles 22.6 -> 25.7.
   if (f8_tiled<GROUPED>(a, rows)) {
-    if constexpr (!EXACT) {
-      if (per > 128 && tiles(256, 256) >= 192) return launch_big<OUT, GROUPED>(a, rows, z, st);
-    }
-    if (per > 64 && tiles(128, 256) >= 384) return launch_tiled<2, 2, 2, OUT, EXACT, GROUPED>(a, rows, z, st);
-    if (tiles(128, 128) >= 256) return launch_tiled<1, 4, 1, OUT, EXACT, GROUPED>(a, rows, z, st);
-    return launch_tiled<1, 2, 1, OUT, EXACT, GROUPED>(a, rows, z, st);
+    if (!exact && per > 128 && tiles(256, 256) >= 192) return {256, 256};
+    if (per > 64 && tiles(128, 256) >= 384) return {128, 256};
+    if (tiles(128, 128) >= 256) return {128, 128};
+    return {64, 128};
   }
+  const int tm = per <= 16 ? 16 : 32;
+  if (type == QBNN_F8) return {tm, 128};
+  return {tm, GROUPED || tm == 32 ? 64 : 16};
+}
+// Whether the form's workgroups fit a grid (2^32 threads along x, 2^31 pairs of row tile and sample in the direct form): asked before a call's first launch
+template <bool GROUPED> int f8_fits(const F8Args& a, int rows, int z, int type, bool exact) {
+  const F8Form f = f8_form<GROUPED>(a, rows, z, type, exact);
+  const int64_t tm = ((int64_t)rows + f.tm - 1) / f.tm + (GROUPED ? std::min(a.groups, rows) : 0), tn = ((int64_t)a.N + f.tn - 1) / f.tn;
+  const int64_t along = f.tm <= 32 ? tn * 512 : tm * tn * z * 256;
+  if (along >= ((int64_t)1 << 32) || tm * z >= ((int64_t)1 << 31) - F8_FOLD) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
+  return QBNN_OK;
+}
+template <int OUT, bool EXACT, bool GROUPED> int launch_linear(const F8Args& a, int rows, int z, hipStream_t st) {
+  const F8Form f = f8_form<GROUPED>(a, rows, z, OUT, EXACT);
+  if constexpr (!EXACT) {
+    if (f.tm == 256) return launch_big<OUT, GROUPED>(a, rows, z, st);
+  }
+  if (f.tm == 128 && f.tn == 256) return launch_tiled<2, 2, 2, OUT, EXACT, GROUPED>(a, rows, z, st);
+  if (f.tm == 128) return launch_tiled<1, 4, 1, OUT, EXACT, GROUPED>(a, rows, z, st);
+  if (f.tm == 64) return launch_tiled<1, 2, 1, OUT, EXACT, GROUPED>(a, rows, z, st);
+  const int64_t tiles = ((int64_t)rows + f.tm - 1) / f.tm + (GROUPED ? std::min(a.groups, rows) : 0);
   if constexpr (OUT == F8_HALF) return f8_fail("qbnn_experts_f8: no direct form of this result");
   else if constexpr (OUT == QBNN_F8) {
-    if (per <= 16) return launch_direct<1, 8, 4, 2, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
-    return launch_direct<2, 8, 4, 1, OUT, EXACT, GROUPED>(a, (rows + 31) / 32 + spare, z, st);
+    if (f.tm == 16) return launch_direct<1, 8, 4, 2, OUT, EXACT, GROUPED>(a, tiles, z, st);
+    return launch_direct<2, 8, 4, 1, OUT, EXACT, GROUPED>(a, tiles, z, st);
   } else {
-    if (per <= 16) {
-      if (GROUPED) return launch_direct<1, 4, 4, 2, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
-      return launch_direct<1, 1, 8, 4, OUT, EXACT, GROUPED>(a, (rows + 15) / 16 + spare, z, st);
+    if (f.tm == 16) {
+      if constexpr (GROUPED) return launch_direct<1, 4, 4, 2, OUT, EXACT, GROUPED>(a, tiles, z, st);
+      else return launch_direct<1, 1, 8, 4, OUT, EXACT, GROUPED>(a, tiles, z, st);
     }
-    return launch_direct<2, 4, 4, 2, OUT, EXACT, GROUPED>(a, (rows + 31) / 32 + spare, z, st);
+    return launch_direct<2, 4, 4, 2, OUT, EXACT, GROUPED>(a, tiles, z, st);
   }
 }
 // what the two entries ask for: every type for dense rows (fp32 exact), e4m3 and fp32 of either form and halves for groups
@@ -1126,63 +1163,104 @@ QBNN_EXPORT int qbnn_quantize_f8(const void* x, int32_t x_type, int64_t x_batch_
   return quantize(x, x_type, x_batch_stride, x_row_stride, batch, R, K, block_rows, q, exponents, (hipStream_t)stream);
 }
 
-QBNN_EXPORT int qbnn_linear_f8_mc(const qbnn_f8_linear* d, void* stream) {
+namespace {
+// A call's arguments checked and laid out; whether its launches fit is known before the first
+int linear_args(const qbnn_f8_linear* d, F8Args& a) {
   if (!d || d->N <= 0 || d->K <= 0 || d->K > 0x7fffff00 || d->N > 0x7fffff00 || d->M < 0 || d->n_samples < 0 || d->y_type < QBNN_F32 || d->y_type > QBNN_F8 ||
       (d->x_float && !float_type(d->x_type)))
     return f8_fail("qbnn_linear_f8_mc: bad argument");
+  a = {};
   if (d->M == 0 || d->n_samples == 0) return QBNN_OK;
   if (!d->x || !d->x_exp || !d->w || !d->w_exp || !d->y || (d->y_type == QBNN_F8 && !d->y_exp)) return f8_fail("qbnn_linear_f8_mc: bad argument");
   if (!aligned(d->x, d->x_ss, 16) || !aligned(d->w, d->w_ss, 16) || !aligned(d->x_exp, d->x_exp_ss, 4) || !aligned(d->w_exp, d->w_exp_ss, 4) ||
       (d->y_type == QBNN_F8 && !aligned(d->y, 0, 16)))
     return f8_fail("qbnn_linear_f8_mc: e4m3 operands start at multiples of 16 bytes, exponents of 4");
-  if (d->x_float)
-    if (int rc = quantize(d->x_float, d->x_type, d->x_float_ss, d->x_float_rs, d->x_ss ? d->n_samples : 1, d->M, d->K, 1, d->x, d->x_exp, (hipStream_t)stream)) return rc;
-  F8Args a = {};
   set_columns(a, d->K);
   a.x = d->x; a.xe = d->x_exp; a.x_ss = d->x_ss; a.xe_ss = d->x_exp_ss;
   a.w = d->w; a.we = d->w_exp; a.w_ss = d->w_ss; a.we_ss = d->w_exp_ss;
   a.bias = d->bias; a.bias_ss = d->bias_ss; a.relu = d->relu;
   set_result(a, d->y, d->y_exp, d->M, d->N, d->y_type);
-  return launch_linear_any<false>(a, a.M, d->n_samples, d->y_type, 0, (hipStream_t)stream);
+  return f8_fits<false>(a, a.M, d->n_samples, d->y_type, d->y_type == QBNN_F32);
 }
-
-QBNN_EXPORT int qbnn_experts_f8(const qbnn_f8_experts* d, void* stream) {
+// half: the second product's results wait for their sum as halves.  They do where the result is bf16, behind tiles, and take R Nb 257 bytes of the R N 4.
+int experts_args(const qbnn_f8_experts* d, F8Args& up, F8Args& down, int& rows, bool& half) {
+  rows = 0;
   if (!d || d->S < 0 || d->T < 0 || d->E <= 0 || d->top_k <= 0 || d->D <= 0 || d->H <= 0 || d->N <= 0 || d->D > 0x7fffff00 || d->H > 0x7fffff00 || d->N > 0x7fffff00 ||
       !float_type(d->y_type) || (d->x_float && !float_type(d->x_type)) || (d->up_sets != d->E && d->up_sets != d->S * d->E) ||
       (d->down_sets != d->E && d->down_sets != d->S * d->E) || (int64_t)d->S * d->T * d->top_k > 0x7fffffff || (int64_t)d->S * d->E > 0x7fffffff)
     return f8_fail("qbnn_experts_f8: bad argument");
-  const int rows = d->S * d->T * d->top_k;
-  if (rows == 0) return QBNN_OK;
+  const int n = d->S * d->T * d->top_k;
+  if (n == 0) return QBNN_OK;
   if (!d->x || !d->x_exp || !d->offsets || !d->rows || !d->weights || !d->w_up || !d->up_exp || !d->w_down || !d->down_exp || !d->h || !d->h_exp || !d->o || !d->y ||
       (d->x_rows != d->T && d->x_rows != d->S * d->T))
     return f8_fail("qbnn_experts_f8: bad argument");
   if (!aligned(d->x, 0, 16) || !aligned(d->w_up, d->up_ss, 16) || !aligned(d->w_down, d->down_ss, 16) || !aligned(d->h, 0, 16) || !aligned(d->x_exp, 0, 4) ||
       !aligned(d->up_exp, d->up_exp_ss, 4) || !aligned(d->down_exp, d->down_exp_ss, 4) || !aligned(d->h_exp, 0, 4) || !aligned(d->o, 0, 16))
     return f8_fail("qbnn_experts_f8: e4m3 operands start at multiples of 16 bytes, exponents of 4");
+  up = {};
+  up.offsets = d->offsets; up.groups = d->S * d->E;
+  down = up;
+  set_columns(up, d->D);
+  up.x = d->x; up.xe = d->x_exp; up.rows = d->rows; up.topk = d->top_k; up.x_rows = d->x_rows;
+  up.w = d->w_up; up.we = d->up_exp; up.w_ss = d->up_ss; up.we_ss = d->up_exp_ss; up.w_groups = d->up_sets;
+  up.bias = d->b_up; up.bias_ss = d->b_up_ss; up.relu = 1;
+  set_result(up, d->h, d->h_exp, n, d->H, QBNN_F8);
+  set_columns(down, d->H);
+  down.x = d->h; down.xe = d->h_exp;
+  down.w = d->w_down; down.we = d->down_exp; down.w_ss = d->down_ss; down.we_ss = d->down_exp_ss; down.w_groups = d->down_sets;
+  down.bias = d->b_down; down.bias_ss = d->b_down_ss;
+  down.y_rows = d->rows; down.scale = d->weights;
+  set_result(down, d->o, nullptr, n, d->N, QBNN_F32);
+  half = d->y_type == QBNN_BF16 && !(d->exact & 2) && d->N >= 128 && f8_tiled<true>(down, n);
+  if (half) {
+    const int Nb = (d->N + 127) / 128;
+    down.y_rs = Nb * 128; down.ye_rs = Nb;
+    down.ye = (uint8_t*)d->o + (int64_t)n * down.y_rs * 2;
+  }
+  if (int rc = f8_fits<true>(up, n, 1, QBNN_F8, d->exact & 1)) return rc;
+  if (int rc = f8_fits<true>(down, n, 1, half ? F8_HALF : QBNN_F32, d->exact >> 1 & 1)) return rc;
+  rows = n;
+  return QBNN_OK;
+}
+int32_t tile_of(F8Form f) { return f.tm << 16 | f.tn; }
+}  // namespace
+
+QBNN_EXPORT int qbnn_linear_f8_mc(const qbnn_f8_linear* d, void* stream) {
+  F8Args a;
+  if (int rc = linear_args(d, a)) return rc;
+  if (a.M == 0) return QBNN_OK;
+  if (d->x_float)
+    if (int rc = quantize(d->x_float, d->x_type, d->x_float_ss, d->x_float_rs, d->x_ss ? d->n_samples : 1, d->M, d->K, 1, d->x, d->x_exp, (hipStream_t)stream)) return rc;
+  return launch_linear_any<false>(a, a.M, d->n_samples, d->y_type, 0, (hipStream_t)stream);
+}
+
+QBNN_EXPORT int32_t qbnn_linear_f8_tile(const qbnn_f8_linear* d) {
+  F8Args a;
+  if (int rc = linear_args(d, a)) return rc;
+  return a.M == 0 ? 0 : tile_of(f8_form<false>(a, a.M, d->n_samples, d->y_type, d->y_type == QBNN_F32));
+}
+
+QBNN_EXPORT int qbnn_experts_f8(const qbnn_f8_experts* d, void* stream) {
+  F8Args up, down;
+  int rows;
+  bool half;
+  if (int rc = experts_args(d, up, down, rows, half)) return rc;
+  if (rows == 0) return QBNN_OK;
   hipStream_t st = (hipStream_t)stream;
   if (d->x_float)
     if (int rc = quantize(d->x_float, d->x_type, d->x_float_ss, d->x_float_rs, d->x_rows / d->T, d->T, d->D, 1, d->x, d->x_exp, st)) return rc;
-  F8Args a = {};
-  a.offsets = d->offsets; a.groups = d->S * d->E;
-  set_columns(a, d->D);
-  a.x = d->x; a.xe = d->x_exp; a.rows = d->rows; a.topk = d->top_k; a.x_rows = d->x_rows;
-  a.w = d->w_up; a.we = d->up_exp; a.w_ss = d->up_ss; a.we_ss = d->up_exp_ss; a.w_groups = d->up_sets;
-  a.bias = d->b_up; a.bias_ss = d->b_up_ss; a.relu = 1;
-  set_result(a, d->h, d->h_exp, rows, d->H, QBNN_F8);
-  if (int rc = launch_linear_any<true>(a, rows, 1, QBNN_F8, d->exact & 1, st)) return rc;
-  set_columns(a, d->H);
-  a.x = d->h; a.xe = d->h_exp; a.rows = nullptr;
-  a.w = d->w_down; a.we = d->down_exp; a.w_ss = d->down_ss; a.we_ss = d->down_exp_ss; a.w_groups = d->down_sets;
-  a.bias = d->b_down; a.bias_ss = d->b_down_ss; a.relu = 0;
-  a.y_rows = d->rows; a.scale = d->weights;
-  // halves where the result is bf16, behind tiles; they take R Nb 257 bytes of the R N 4
-  const bool half = d->y_type == QBNN_BF16 && !(d->exact & 2) && d->N >= 128 && f8_tiled<true>(a, rows);
-  set_result(a, d->o, nullptr, rows, d->N, QBNN_F32);
-  if (half) {
-    const int Nb = (d->N + 127) / 128;
-    a.y_rs = Nb * 128; a.ye_rs = Nb;
-    a.ye = (uint8_t*)d->o + (int64_t)rows * a.y_rs * 2;
-  }
-  if (int rc = launch_linear_any<true>(a, rows, 1, half ? F8_HALF : QBNN_F32, d->exact >> 1 & 1, st)) return rc;
-  return launch_combine(d->o, half ? a.ye : nullptr, d->S * d->T, d->top_k, d->N, d->y, d->y_type, st);
+  if (int rc = launch_linear_any<true>(up, rows, 1, QBNN_F8, d->exact & 1, st)) return rc;
+  if (int rc = launch_linear_any<true>(down, rows, 1, half ? F8_HALF : QBNN_F32, d->exact >> 1 & 1, st)) return rc;
+  return launch_combine(d->o, half ? down.ye : nullptr, d->S * d->T, d->top_k, d->N, d->y, d->y_type, st);
+}
+
+QBNN_EXPORT int qbnn_experts_f8_tiles(const qbnn_f8_experts* d, int32_t* tiles) {
+  F8Args up, down;
+  int rows;
+  bool half;
+  if (int rc = experts_args(d, up, down, rows, half)) return rc;
+  if (!tiles) return f8_fail("qbnn_experts_f8_tiles: bad argument");
+  tiles[0] = rows ? tile_of(f8_form<true>(up, rows, 1, QBNN_F8, d->exact & 1)) : 0;
+  tiles[1] = rows ? tile_of(f8_form<true>(down, rows, 1, half ? F8_HALF : QBNN_F32, d->exact >> 1 & 1)) : 0;
+  return QBNN_OK;
 }
