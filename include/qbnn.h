@@ -649,7 +649,7 @@ int qbnn_quantize_f8(const void* x, int32_t x_type, int64_t x_batch_stride, int6
                      int32_t block_rows, uint8_t* q, uint8_t* exponents, void* stream);
 
 /* y[s][m][n] = act( sum_k x[s][m][k] w[s][n][k] + bias[s][n] ).  For fp32 results products and sums in fp32 ("exact"), at half the
- * matrix rate; for the others the e4m3 matrix instruction, which cuts the products of 8 neighbouring columns off 2^-13 below the largest of them
+ * matrix rate, and so for results of up to 16 rows a sample; for the others the e4m3 matrix instruction, which cuts the products of 8 neighbouring columns off 2^-13 below the largest of them
  * before it adds them, and sums in fp32 from there (1.3e-5 of the result's norm on normal data).  x: block_rows 1, w: block_rows 128.  Strides
  * per sample in bytes for the operands (0 = shared by the samples), in elements for the bias; y [n_samples][M][N] dense, or for QBNN_F8 in
  * the operand format (y_exp, block_rows 1).  Replaces the fp32 / int8 product of a stochastic Linear (bbb/linear.py:42-50). */
@@ -691,7 +691,8 @@ int qbnn_route_experts(const qbnn_route* host_desc, void* stream);
  *   y[s][t] = sum_j weights[s][t][j] ( relu(x[s][t] w_up[e]^T + b_up[e]) w_down[e]^T + b_down[e] ),  e = experts[s][t][j]
  * offsets / rows / weights: of qbnn_route_experts with the same S, T, E, top_k.  x [S or 1][T][D] (x_rows = S T or T; float: quantised into x / x_exp
  * first), w_up [S or 1][E][H][D], w_down [S or 1][E][N][H] (block_rows 128; strides per expert in bytes, up_sets / down_sets = E or S E), biases fp32 (strides per
- * expert in elements).  Hidden rows are quantised in blocks of 128; exact: bit 0 the first product, bit 1 the second (see qbnn_f8_linear); a result whose weight
+ * expert in elements).  Hidden rows are quantised in blocks of 128; exact: bit 0 the first product, bit 1 the second (see qbnn_f8_linear; both are
+ * where the experts get 16 rows or fewer on average); a result whose weight
  * is 0 is left out, whatever it is.  The weighted results are fp32 and summed in the order of j, rounded once to y_type (QBNN_F32 .. QBNN_F16); where y is bf16
  * and more than 32 rows go to an expert on average they may wait for the sum as fp16 with one power of two per 128 columns (2^-11 of each, beside the sum's own 2^-8).
  * Gathered rows of 4 GiB and more (x in e4m3: x_rows times D up to a multiple of 128) go through the form for few rows, which is slower.

@@ -80,8 +80,8 @@ def experts_fp8(x, routing, w_up, w_down, b_up=None, b_down=None, out_dtype=None
     x: float, or an F8Tensor with block_rows 1, [T, D] or [S or 1, T, D] as the routing's rows; w_up F8Tensor [E, H, D], w_down [E, N, H] (block_rows 128; [S, E, ..]
     gives each sample its own); b_up / b_down float32 [E, H] / [E, N] or [S, E, ..].  The hidden rows are quantised as they leave the first product; the weighted
     results are summed in fp32 and rounded once, to `out_dtype` (x's type; bfloat16 for an F8Tensor; large bfloat16 calls hold the terms as fp16 with a power of two per
-    128 columns).  For a bfloat16 result both products take the fast form of
-    linear_fp8, for float16 the first and for float32 both take the exact one: a hidden value next to a rounding border moves by a whole step.  Inputs of 4 GiB and more
+    128 columns).  Where the experts get more than 16 rows on average, for a bfloat16 result both products take the fast form of linear_fp8, for float16 the second; they
+    are exact otherwise: a hidden value next to a rounding border moves by a whole step.  Inputs of 4 GiB and more
     in e4m3 (2^20 rows of 4096 columns) go through the form for few rows, which is slower."""
     if not isinstance(routing, Routing):
         raise TypeError("routing is a Routing (route_experts)")
