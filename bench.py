@@ -616,9 +616,9 @@ def main():
         # (FETCH_SIZE x2 + WRITE_SIZE, separate --pmc runs) -- but ONLY while that file was measured on this very kernel source
         # and workload shape; otherwise null (never a stale number)
         traffic, traffic_note = None, "no PMC summary for this kernel source: run tools/profile_round.sh"
-        # the PMC summary measured on THIS kernel source if there is one, else the latest round's (by round number, not by name order)
-        cands = sorted((f for f in os.listdir(os.path.join(ROOT, "profiles")) if re.match(r"r\d+_pmc_traffic\.json$", f)),
-                       key=lambda f: int(re.match(r"r(\d+)_", f).group(1)))
+        # the PMC summary measured on THIS kernel source and these compiler flags if there is one, else the latest (pmc_traffic.json before the numbered ones, by number)
+        cands = sorted((f for f in os.listdir(os.path.join(ROOT, "profiles")) if re.match(r"(r\d+_)?pmc_traffic\.json$", f)),
+                       key=lambda f: int(f[1:f.index("_")]) if f[0] == "r" else 1 << 30)
         for f in cands:
             if json.load(open(os.path.join(ROOT, "profiles", f))).get("kernel_source_sha16") == kernel_source_sha16():
                 cands = [f]

@@ -25,8 +25,8 @@ UNRECORDED = {"qbnn_f8.hip", "qbnn_route.hip", "qbnn_f8.h"}
 
 
 def kernel_source_sha16():
-    """Hash of every kernel source of the recorded workloads: measurement files (profiles/*_pmc_traffic.json) are keyed to it."""
-    h = hashlib.sha256()
+    """Hash of every kernel source of the recorded workloads and of the flags they are compiled with: measurement files (profiles/*pmc_traffic.json) are keyed to it."""
+    h = hashlib.sha256(" ".join(HIPCC_FLAGS + EXTRA).encode())
     for p in sorted(SRC + [os.path.join(CSRC, x) for x in HEADERS]):
         if os.path.basename(p) not in UNRECORDED:
             h.update(open(p, "rb").read())
