@@ -31,8 +31,8 @@ static inline int f8_fail(const char* fmt, long a = 0, long b = 0) {
 struct QuantF8Args {
   const void* x; int64_t x_bs, x_rs;       // batch / row stride in elements; columns are contiguous
   uint8_t* q; uint8_t* e;                  // [batch][R][Kp], [batch][Rb][Sp]
-  int R, K, Kb, Sp; int64_t blocks;        // blocks = batch * Rb * Kb
-  uint32_t kb_magic, r_magic; int kb_shift, r_shift;      // division by Kb and R: n * magic >> (32 + shift), n < 2^31 (rows form)
+  int R, K, Kb, Sp; int64_t blocks, first; // blocks = batch * Rb * Kb; first: that of the launch (blocks form)
+  uint32_t kb_magic, r_magic; int kb_shift, r_shift;      // division by Kb and R: n * magic >> (31 + shift), n < 2^31 (rows form)
 };
 // n / d for n < 2^31: the smallest p with 2^p >= d gives an error below 1 / d
 static void f8_magic(uint32_t d, uint32_t& magic, int& shift) {
@@ -117,7 +117,7 @@ template <int T, int U, bool TAIL> __global__ __launch_bounds__(256) void quanti
 template <int T> __global__ __launch_bounds__(256) void quantize_f8_blocks_kernel(const QuantF8Args a) {
   __shared__ uint32_t red[4];
   const int Rb = (a.R + 127) >> 7;
-  const int64_t b = blockIdx.x;
+  const int64_t b = a.first + blockIdx.x;
   const int64_t br = b / a.Kb;
   const int kb = (int)(b - br * a.Kb), j = threadIdx.x & 15, sub = threadIdx.x >> 4;
   const int64_t bt = br / Rb;
@@ -151,8 +151,8 @@ template <int T> __global__ __launch_bounds__(256) void quantize_f8_blocks_kerne
 template <int T> int launch_quantize_rows(QuantF8Args a, int64_t batch, hipStream_t st) {
   if (a.x_bs == a.R * a.x_rs && batch * a.R < ((int64_t)1 << 31)) { a.R = (int)(batch * a.R); batch = 1; }      // one matrix
   f8_magic((uint32_t)a.Kb, a.kb_magic, a.kb_shift);
-  // launches of fewer than 2^31 blocks and rows
-  const int64_t rows = batch * a.R, most = ((int64_t)1 << 30) / a.Kb;
+  // launches of up to 2^29 blocks and rows: fewer than 2^32 threads
+  const int64_t rows = batch * a.R, most = ((int64_t)1 << 29) / a.Kb;
   const int64_t step = rows <= most ? rows : batch == 1 ? most : (most / a.R ? most / a.R * a.R : 0);
   if (step == 0) return f8_fail("qbnn_quantize_f8: a matrix of %ld blocks in a batch", (long)((int64_t)a.R * a.Kb));
   f8_magic((uint32_t)(batch == 1 ? (step < a.R ? step : a.R) : a.R), a.r_magic, a.r_shift);
@@ -179,9 +179,12 @@ template <int T> int launch_quantize_rows(QuantF8Args a, int64_t batch, hipStrea
 }
 template <int T> int launch_quantize(const QuantF8Args& a, int64_t batch, int block_rows, hipStream_t st) {
   if (block_rows == 1) return launch_quantize_rows<T>(a, batch, st);
-  if (a.blocks > 0x7fffffff) return f8_fail("qbnn_quantize_f8: too many blocks (%ld)", (long)a.blocks);
-  hipLaunchKernelGGL((quantize_f8_blocks_kernel<T>), dim3((unsigned)a.blocks), dim3(256), 0, st, a);
-  return qbnn_check_launch_msg("qbnn_quantize_f8");
+  QuantF8Args c = a;
+  for (c.first = 0; c.first < a.blocks; c.first += 1 << 23) {      // (2^31 threads: a launch of 2^32 or more loses the rest of them without an error)
+    hipLaunchKernelGGL((quantize_f8_blocks_kernel<T>), dim3((unsigned)std::min(a.blocks - c.first, (int64_t)1 << 23)), dim3(256), 0, st, c);
+    if (int rc = qbnn_check_launch_msg("qbnn_quantize_f8")) return rc;
+  }
+  return QBNN_OK;
 }
 
 // ================================================================================================================================

@@ -40,6 +40,15 @@ def test_more_samples_than_a_grid_axis_holds(out):
             assert torch.equal(y[a], z)
 
 
+def test_quantiser_of_more_blocks_than_a_launch_takes():
+    """2^24 workgroups of 256 threads are more than one launch's threads: matrices of one row, whose blocks of 128 x 128 are those of 1 x 128."""
+    x = torch.randn((1 << 24) + 77, 1, 5, generator=torch.Generator(DEV).manual_seed(1), device=DEV)
+    a, b = q.quantize_fp8(x, 128), q.quantize_fp8(x)
+    for t in (slice(0, 1000), slice((1 << 23) - 500, (1 << 23) + 500), slice(-1000, None)):
+        assert torch.equal(a.data[t].view(torch.uint8), b.data[t].view(torch.uint8)) and torch.equal(a.exponent[t], b.exponent[t])
+    assert torch.equal(a.data.view(torch.int32), b.data.view(torch.int32)) and torch.equal(a.exponent, b.exponent)
+
+
 def check_rows(x, r, up, down, y, at):
     """Rows `at` of a bfloat16 call against the 64-bit form."""
     xv = orc.quantised(x[at].double().cpu().numpy(), 1)[None]
