@@ -641,6 +641,7 @@ QBNN_EXPORT int qbnn_route_experts(const qbnn_route* r, void* stream) {
     return route_fail("qbnn_route_experts: bad argument (E %ld, top_k %ld)", r ? r->E : 0, r ? r->top_k : 0);
   const int64_t rows = (int64_t)r->S * r->T * r->top_k;
   if (rows > 0x7fffffff || (int64_t)r->S * r->E >= 0x7fffffff) return route_fail("qbnn_route_experts: %ld routed rows do not fit 31 bits", (long)rows);
+  if (r->T >= 1 << 29) return route_fail("qbnn_route_experts: %ld rows of a sample are more than a launch has threads for", r->T);      // 512 for each 64 of them, 2^32 in all
   if (rows == 0) return route_fail("qbnn_route_experts: no rows");
   if (!r->logits || !r->weights || !r->experts || !r->rows || !r->workspace || r->S > 65535) return route_fail("qbnn_route_experts: bad argument");
   RouteArgs a;

@@ -49,7 +49,7 @@ def route_experts(logits, top_k, score="softmax", bias=None, groups=1, top_group
         raise ValueError("groups divides the experts (at most 64 groups), 1 <= top_groups <= groups")
     if not 1 <= top_k <= min(MAX_CHOICES, E // groups * top_groups):
         raise ValueError("top_k is at most %d and the experts of top_groups groups" % MAX_CHOICES)
-    if S * T * top_k >= 1 << 31 or S > 65535:
+    if S * T * top_k >= 1 << 31 or T >= 1 << 29 or S > 65535:
         raise ValueError("too many rows for one call")
     bias = _bias(bias, ((E,),), "[E]")
     dev = _device(logits, bias)
