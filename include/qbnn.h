@@ -650,7 +650,8 @@ int qbnn_quantize_f8(const void* x, int32_t x_type, int64_t x_batch_stride, int6
 
 /* y[s][m][n] = act( sum_k x[s][m][k] w[s][n][k] + bias[s][n] ).  For fp32 results products and sums in fp32 ("exact"), at half the
  * matrix rate, and so for results of up to 16 rows a sample; for the others the e4m3 matrix instruction, which cuts the products of 8 neighbouring columns off 2^-13 below the largest of them
- * before it adds them, and sums in fp32 from there (1.3e-5 of the result's norm on normal data).  x: block_rows 1, w: block_rows 128.  Strides
+ * before it adds them, and sums in fp32 from there (1.3e-5 of the result's norm on normal data).  The exact form holds operands to 2^-133 (blocks whose largest
+ * magnitude is 2^-109 or more lose nothing by that).  x: block_rows 1, w: block_rows 128.  Strides
  * per sample in bytes for the operands (0 = shared by the samples), in elements for the bias; y [n_samples][M][N] dense, or for QBNN_F8 in
  * the operand format (y_exp, block_rows 1).  Replaces the fp32 / int8 product of a stochastic Linear (bbb/linear.py:42-50). */
 typedef struct qbnn_f8_linear {

@@ -867,7 +867,7 @@ template <int MI, int WM, int WN, int OUT, bool EXACT, bool GROUPED> int launch_
 //   second half  wait for the next step, barrier; x4 .. x7 times w; reads the next step's x0 .. x3 and w, each fragment into its registers behind its last product
 // The exponents come the same way, a dword (four steps) of each row every two steps: as loads into registers they were waited for together with every
 // request issued before them, which emptied the ring.
-// 8192^3: 380 - 450 us, 2.5 - 2.9 PFLOP/s.  At this rate the card is bound by power (1.5 - 1.9 GHz on normal data), and the 16 x 16 x 128 form draws less of it than 32 x 32 x 64 (alone: 4,080 against
+// 8192^3: 370 us replayed from a graph, 2.97 PFLOP/s (447 under the profiler from idle).  At this rate the card is bound by power (1.5 - 1.9 GHz on normal data), and the 16 x 16 x 128 form draws less of it than 32 x 32 x 64 (alone: 4,080 against
 // 3,500 TFLOP/s).  The compiler gives its result other registers than its addend, for which 256 accumulators leave none; so the instruction is written
 // out, in place.  An accumulator is read again 32 instructions later or behind the wait at the end, which is what its hazards ask for.
 template <int B> __device__ __forceinline__ void f8_mfma_in_place(f8_v4f& acc, const f8_v8i& w, const f8_v8i& x, uint32_t ws, uint32_t xs) {      // exponents: byte B
@@ -1085,7 +1085,7 @@ template <bool GROUPED> int launch_linear_any(const F8Args& a, int rows, int z, 
 
 // ---- y[t] = sum over the row's top_k results, in the order of choice --------------------------------------------------------------
 // The results come in fp32: rounded to the 16 bits of y first, each would cost as much as the one rounding of the sum does.  For a bf16 y, halves with block exponents
-// cost 2^-11 of each term beside the sum's 2^-8 and are half of the bytes, which bound this kernel (32768 x 4096: 115 us from fp32, 55 from halves, 5.4 TB/s).
+// cost 2^-11 of each term beside the sum's 2^-8 and are half of the bytes, which bound this kernel (32768 x 4096: 115 us from fp32, 55 from halves, 6.1 TB/s).
 constexpr int COMBINE_COLUMNS = 8;
 template <int T, bool HALF> __global__ __launch_bounds__(256) void combine_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__ oe, f8_type<T>* __restrict__ y, int rows, int k, int N) {
   const int n0 = (blockIdx.x * 256 + threadIdx.x) * COMBINE_COLUMNS;

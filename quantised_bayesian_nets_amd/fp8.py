@@ -145,7 +145,8 @@ def linear_fp8(x, w, bias=None, relu=False, out_dtype=None):
     bias float32 [N] or [S, N].  A leading 1 is shared by the samples.  Returns [S, B, N] ([B, N] if both operands are matrices) in `out_dtype`
     (x's type; bfloat16 for an F8Tensor), or an F8Tensor (block_rows 1) with out_dtype torch.float8_e4m3fn.  Sums are taken in fp32;
     for a result of 16 or 8 bits of more than 16 rows a sample the matrix unit cuts the products of 8 neighbouring columns off 2^-13 below the largest of them first (1.3e-5 of the
-    result's norm), for a float32 result or fewer rows nothing is cut, at half the matrix rate."""
+    result's norm), for a float32 result or fewer rows nothing is cut, at half the matrix rate (of
+    blocks with magnitudes below 2^-109 alone, what lies below 2^-133 is)."""
     if not isinstance(w, F8Tensor) or w.block_rows != BLOCK:
         raise TypeError("w is an F8Tensor with block_rows 128 (quantize_fp8(w, 128))")
     if isinstance(x, F8Tensor):
