@@ -1015,7 +1015,7 @@ template <int OUT, bool GROUPED> int launch_big(const F8Args& a, int rows, int z
 
 // Whether the products go through LDS tiles.  rows: the rows of one sample, or all routed rows.  Offsets are 32 bits wide there: of a gathered row's bytes from the
 // first, of a row's in its tile.
-template <bool GROUPED> int f8_rows_each(const F8Args& a, int rows) { return GROUPED ? (rows + a.groups - 1) / a.groups : rows; }
+template <bool GROUPED> int f8_rows_each(const F8Args& a, int rows) { return GROUPED ? (int)(((int64_t)rows + a.groups - 1) / a.groups) : rows; }
 template <bool GROUPED> bool f8_tiled(const F8Args& a, int rows) {
   const int64_t far = GROUPED && a.rows ? (int64_t)a.x_rows * a.Kb * 128 : 0;
   return f8_rows_each<GROUPED>(a, rows) > 32 && far < ((int64_t)1 << 32) && a.Kb < (1 << 16);
@@ -1025,7 +1025,7 @@ struct F8Form { int tm, tn; };
 template <bool GROUPED> F8Form f8_form(const F8Args& a, int rows, int z, int type, bool exact) {
   const int spare = GROUPED ? std::min(a.groups, rows) : 0;      // each group with rows may end inside a tile
   const int per = f8_rows_each<GROUPED>(a, rows);
-  const auto tiles = [&](int tm, int tn) { return (int64_t)z * ((rows + tm - 1) / tm + spare / 2) * ((a.N + tn - 1) / tn); };
+  const auto tiles = [&](int tm, int tn) { return (__int128)z * (((int64_t)rows + tm - 1) / tm + spare / 2) * (((int64_t)a.N + tn - 1) / tn); };
   // The largest tile that still gives the 256 CUs work: fewer bytes through LDS per product, but 256 x 256 holds a CU for itself.  Measured the other way round (us):
   // 128 x 128 for 64 x 128 with 330 - 600 tiles 69 -> 58 (5 x 12 groups of 75, fp16) and 28.6 -> 23.8 (100 x 128 x 500 x 800, fp32), with 32 - 64 tiles 22.6 -> 25.7.
   if (f8_tiled<GROUPED>(a, rows)) {
@@ -1042,7 +1042,7 @@ template <bool GROUPED> F8Form f8_form(const F8Args& a, int rows, int z, int typ
 template <bool GROUPED> int f8_fits(const F8Args& a, int rows, int z, int type, bool exact) {
   const F8Form f = f8_form<GROUPED>(a, rows, z, type, exact);
   const int64_t tm = ((int64_t)rows + f.tm - 1) / f.tm + (GROUPED ? std::min(a.groups, rows) : 0), tn = ((int64_t)a.N + f.tn - 1) / f.tn;
-  const int64_t along = f.tm <= 32 ? tn * 512 : tm * tn * z * 256;
+  const __int128 along = f.tm <= 32 ? (__int128)tn * 512 : (__int128)tm * tn * z * 256;
   if (along >= ((int64_t)1 << 32) || tm * z >= ((int64_t)1 << 31) - F8_FOLD) return f8_fail("qbnn_linear_f8: %ld tiles x %ld samples do not fit a grid", (long)(tm * tn), z);
   return QBNN_OK;
 }

@@ -47,3 +47,5 @@ def test_a_call_that_fits_no_grid_is_refused_before_anything_runs():
     assert linear(1 << 30, 1, 128, S=4, y_type=0) == -1 and b"do not fit a grid" in L.qbnn_last_error()
     assert L.qbnn_linear_f8_mc(call, None) == -1 and b"do not fit a grid" in L.qbnn_last_error()
     assert linear(1, 64, 64, S=(1 << 31) - 1) == -1
+    assert linear((1 << 31) - 1, (1 << 31) - 300, 128, S=1 << 30, shared=True) == -1 and b"do not fit a grid" in L.qbnn_last_error()      # 2^78 tiles: not lost in 64 bits
+    assert linear((1 << 31) - 1, 64, 128, y_type=3) == (256, 256)
